@@ -1,0 +1,616 @@
+// Tree speculation outside attention: the ancestor bit rows of a tree of drafted tokens, its
+// verification against the target's probabilities, and the move of the accepted path's
+// cache rows (tree attention itself is in tree_attention.cu).
+//
+// A sequence's tree: nodes 0 .. n-1 in rows q_start[b] .. q_start[b+1]-1, node 0 the root (the
+// last emitted token), every other node with a parent of lower index.  A parent that is
+// negative or not below its node stands for "none".
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+#include "launch.cuh"
+#include "ptx.cuh"
+
+namespace xtu {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int TREE_MAX_NODES = 1024;   // nodes of one sequence: the shared arrays below
+
+// rows of sequence b, at most `most`; a longer one is cut and reported (site)
+__device__ __forceinline__ int tree_nodes(const int* q_start, int b, int most, XtuStatus* st, int site) {
+  const int n = q_start[b + 1] - q_start[b];
+  if (n > most) report_error(st, XTU_ERR_BOUNDS, site, n);
+  return n < 0 ? 0 : n > most ? most : n;
+}
+
+// ---------------------------------------------------------------------------------------
+// ancestor bits: row i gets bit j for j = i and for every ancestor j; depth = ancestors.
+// grid (B, node chunks of 128).  A node's ancestors have falling indices, so one walk up the
+// parents in shared memory meets the words of the row in falling order and writes each once.
+// Latency bound: the walk is `depth` dependent shared-memory reads.
+__global__ void __launch_bounds__(128) tree_mask_kernel(const int* __restrict__ parents,
+                                                        const int* __restrict__ q_start, int max_nodes, int W,
+                                                        int* __restrict__ mask, int* __restrict__ depth,
+                                                        XtuStatus* st) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ int par[TREE_MAX_NODES];
+  const int b = blockIdx.x;
+  const int n = tree_nodes(q_start, b, max_nodes, st, 240);
+  const int q0 = q_start[b];
+  const int i0 = blockIdx.y * 128;
+  if (i0 >= n) return;
+  const int last = min(n, i0 + 128);
+  for (int i = threadIdx.x; i < last; i += 128) par[i] = parents[q0 + i];
+  __syncthreads();
+  const int i = i0 + threadIdx.x;
+  if (i >= n) return;
+  int* row = mask + (size_t)(q0 + i) * W;
+  int w = i >> 5, cur = i, d = 0;
+  for (int z = W - 1; z > w; --z) row[z] = 0;
+  uint32_t bits = 1u << (i & 31);
+  for (;;) {
+    const int p = par[cur];
+    if (p < 0 || p >= cur) break;
+    if ((p >> 5) != w) {
+      row[w] = (int)bits;
+      for (int z = w - 1; z > (p >> 5); --z) row[z] = 0;
+      w = p >> 5;
+      bits = 0;
+    }
+    bits |= 1u << (p & 31);
+    cur = p;
+    ++d;
+  }
+  row[w] = (int)bits;
+  for (int z = w - 1; z >= 0; --z) row[z] = 0;
+  depth[q0 + i] = d;
+}
+
+// ---------------------------------------------------------------------------------------
+// the first node i >= from whose parent is `cur`, or -1 (whole warp)
+__device__ __forceinline__ int next_child(const int* par, int n, int from, int cur) {
+  const int lane = threadIdx.x & 31;
+  for (int base = from & ~31; base < n; base += 32) {
+    const int i = base + lane;
+    const unsigned m = __ballot_sync(0xffffffffu, i >= from && i < n && par[i] == cur);
+    if (m) return base + __ffs(m) - 1;
+  }
+  return -1;
+}
+
+// greedy acceptance: from the root, the first child (index order) whose token is the target's
+// token at the current node, until none is.  One warp per sequence.
+__global__ void __launch_bounds__(32) tree_verify_greedy_kernel(
+    const int* __restrict__ target, const int* __restrict__ tokens, const int* __restrict__ parents,
+    const int* __restrict__ q_start, int P, int* __restrict__ accepted, int* __restrict__ path,
+    int* __restrict__ out, int* __restrict__ last_row, XtuStatus* st) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ int par[TREE_MAX_NODES], tok[TREE_MAX_NODES], tgt[TREE_MAX_NODES];
+  const int b = blockIdx.x, lane = threadIdx.x;
+  const int n = tree_nodes(q_start, b, P, st, 241);
+  const int q0 = q_start[b];
+  for (int i = lane; i < n; i += 32) {
+    const int p = parents[q0 + i];
+    par[i] = (p >= 0 && p < i) ? p : -1;
+    tok[i] = tokens[q0 + i];
+    tgt[i] = target[q0 + i];
+  }
+  __syncwarp();
+  int* pb = path + (size_t)b * P;
+  int* ob = out + (size_t)b * P;
+  int cur = 0, a = 0;
+  if (n > 0) {
+    if (lane == 0) pb[0] = 0;
+    for (int from = 1;;) {
+      const int c = next_child(par, n, from, cur);
+      if (c < 0) break;
+      from = c + 1;
+      if (tok[c] != tgt[cur]) continue;
+      if (lane == 0) {
+        ob[a] = tok[c];
+        pb[a + 1] = c;
+      }
+      ++a;
+      cur = c;
+    }
+    if (lane == 0) ob[a] = tgt[cur];
+  }
+  const int used = n > 0 ? a + 1 : 0;
+  for (int i = used + lane; i < P; i += 32) pb[i] = ob[i] = -1;
+  if (lane == 0) {
+    accepted[b] = a;
+    last_row[b] = n > 0 ? q0 + cur : -1;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// acceptance by given random numbers.  At node v the weights start as w = p_v (Z = 1); its
+// children are tried in index order, child c with token x:
+//   point-mass drafts   accepted when u_c (1 - r) < w[x], r the probability of the rejected
+//                       siblings' tokens; a rejection sets w[x] = 0
+//   drawn from q_v      accepted when u_c q_v[x] Z < w[x]; a rejection sets
+//                       w <- max(0, w / Z - q_v), Z <- sum w
+// and a node whose children are all rejected emits the smallest t with
+// w[0] + .. + w[t] > u_draw * sum w.
+//
+// Rows of the vocabulary are the traffic (one per sequence, two with q, a pass for every
+// rejection of a drawn child), so a cluster of C CTAs shares a sequence's row: each sums a
+// slice, rank 0 walks the tree and tells the others what to do through their shared
+// memory.  Every decision is rank 0's, so all CTAs meet at the same cluster barriers
+// whatever the inputs hold.  Weights and sums are 64-bit: with 150K terms a 32-bit sum is off
+// by more than many tokens' weight, and the drawn token would depend on the split.
+struct TvCmd {
+  int op;        // 0 sum the weights, 1 draw here, 2 done
+  int row;       // row of probs
+  int rej;       // rejected children of it so far
+  int owner;     // draw: rank that holds the drawn token
+  int slot;      // draw: position in the output row
+  int any;       // draw: take the last positive weight (the target lies past the sum)
+  double target; // draw: target less the slices before the owner's
+};
+
+constexpr int TV_THREADS = 512;
+constexpr int TV_WARPS = TV_THREADS / 32;
+constexpr int TV_MAX_C = 8;
+
+__device__ __forceinline__ float tv_load1(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float tv_load1(const __nv_bfloat16* p) { return __bfloat162float(__ldg(p)); }
+
+// 16 bytes of a row: 4 floats or 8 bf16
+__device__ __forceinline__ void tv_loadv(const float* p, float (&v)[4]) {
+  const float4 x = __ldg(reinterpret_cast<const float4*>(p));
+  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+__device__ __forceinline__ void tv_loadv(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+  v[0] = bf16_lo(x.x); v[1] = bf16_hi(x.x); v[2] = bf16_lo(x.y); v[3] = bf16_hi(x.y);
+  v[4] = bf16_lo(x.z); v[5] = bf16_hi(x.z); v[6] = bf16_lo(x.w); v[7] = bf16_hi(x.w);
+}
+
+template <typename E>
+struct TvShared {
+  int par[TREE_MAX_NODES];
+  int tok[TREE_MAX_NODES];
+  float u[TREE_MAX_NODES], pt[TREE_MAX_NODES], qt[TREE_MAX_NODES];
+  int rejected[TREE_MAX_NODES];       // tokens of the rejected children of the current node
+  double z[TREE_MAX_NODES];           // z[r]: sum of the weights after r rejections (z[0] = 1)
+  double slice[TV_MAX_C];             // rank 0: the CTAs' sums
+  double warp_sum[TV_WARPS];
+  TvCmd cmd;
+};
+
+// weight of an element after `rej` rejections (drawn children), from its p and q
+__device__ __forceinline__ double tv_weight(float p, float q, const double* z, int rej) {
+  double w = p > 0.f ? (double)p : 0.0;      // NaN and negative entries weigh nothing
+  const double qd = q > 0.f ? (double)q : 0.0;
+  for (int r = 0; r < rej; ++r) {
+    const double x = (r == 0 ? w : w / z[r]) - qd;
+    w = x > 0.0 ? x : 0.0;
+  }
+  return w;
+}
+
+template <typename E, bool DRAFT>
+__global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
+    const E* __restrict__ probs, long long ldp, const E* __restrict__ draft, long long ldq, int V, int vec,
+    const int* __restrict__ tokens, const int* __restrict__ parents, const int* __restrict__ q_start,
+    const float* __restrict__ u_accept, const float* __restrict__ u_draw, int P, int* __restrict__ accepted,
+    int* __restrict__ path, int* __restrict__ out, int* __restrict__ last_row, XtuStatus* st) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ TvShared<E> s;
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int VE = 16 / sizeof(E);
+  // this warp's slice of the vocabulary: whole 32 x VE steps
+  const int step = 32 * VE;
+  const int per = (((V + C * TV_WARPS - 1) / (C * TV_WARPS)) + step - 1) / step * step;
+  const long long first = (long long)(rank * TV_WARPS + warp) * per;
+  const int lo = (int)(first < V ? first : V), hi = (int)(first + per < V ? first + per : V);
+
+  int n = 0, q0 = 0;
+  int cur = 0, from = 1, a = 0, rej = 0;     // rank 0, warp 0: the walk
+  double gone = 0.0;                         // point mass: probability of the rejected tokens
+  bool plain = false;                        // nothing was left: draw from p itself
+  int* pb = path + (size_t)b * P;
+  int* ob = out + (size_t)b * P;
+  if (rank == 0) {
+    n = tree_nodes(q_start, b, P, st, 242);
+    q0 = q_start[b];
+    for (int i = tid; i < n; i += TV_THREADS) {
+      const int p = parents[q0 + i], t = tokens[q0 + i];
+      const bool ok = p >= 0 && p < i;
+      s.par[i] = ok ? p : -1;
+      s.tok[i] = t;
+      s.u[i] = u_accept[q0 + i];
+      const bool in = ok && t >= 0 && t < V;   // a token outside the vocabulary is never accepted
+      s.pt[i] = in ? tv_load1(probs + (long long)(q0 + p) * ldp + t) : -1.f;
+      if (DRAFT) s.qt[i] = in ? tv_load1(draft + (long long)(q0 + p) * ldq + t) : 0.f;
+    }
+    __syncthreads();
+  }
+  for (bool have_sum = false;;) {
+    if (rank == 0 && warp == 0) {
+      TvCmd c{};
+      if (n == 0) {
+        c.op = 2;
+      } else {
+        if (have_sum) {                       // the sum that was asked for
+          double tot = 0.0;
+          for (int r = 0; r < C; ++r) tot += s.slice[r];
+          s.z[rej] = tot > 0.0 ? tot : 1.0;
+          __syncwarp();
+          c.op = -1;
+        }
+        int next = -1;
+        // walk on, unless the sum was that of the final weights (no child left)
+        for (;;) {
+          next = plain ? -1 : next_child(s.par, n, from, cur);
+          if (next < 0) break;
+          from = next + 1;
+          const int x = s.tok[next];
+          bool take;
+          if (DRAFT) {
+            double w = tv_weight(s.pt[next], s.qt[next], s.z, rej);
+            const double q = s.qt[next] > 0.f ? (double)s.qt[next] : 0.0;
+            const double z = rej > 0 ? s.z[rej] : 1.0;
+            take = s.pt[next] >= 0.f && (double)s.u[next] * q * z < w;
+          } else {
+            bool dup = false;
+            for (int r = lane; r < rej; r += 32) dup |= s.rejected[r] == x;
+            dup = __any_sync(0xffffffffu, dup);
+            take = !dup && s.pt[next] >= 0.f && (double)s.u[next] * (1.0 - gone) < (double)s.pt[next];
+            if (!take && !dup && s.pt[next] > 0.f) gone += (double)s.pt[next];
+          }
+          if (take) {
+            if (lane == 0) {
+              ob[a] = x;
+              pb[a + 1] = next;
+            }
+            ++a;
+            cur = next;
+            rej = 0;
+            gone = 0.0;
+            have_sum = false;
+            continue;
+          }
+          if (lane == 0) s.rejected[rej] = x;
+          ++rej;
+          __syncwarp();
+          have_sum = false;
+          if (DRAFT) break;                   // the next test (or the draw) needs the new sum
+        }
+        c.row = q0 + cur;
+        c.rej = plain ? 0 : rej;
+        if (!have_sum) {
+          c.op = 0;
+        } else {                              // the sum of the final weights is known: draw
+          double tot = 0.0;
+          for (int r = 0; r < C; ++r) tot += s.slice[r];
+          if (!(tot > 0.0) && !plain) {       // nothing left of p: the draw is from p itself
+            plain = true;
+            c.op = 0;
+            c.rej = 0;
+          } else {
+            const double t = (double)u_draw[b] * tot;
+            double before = 0.0;
+            int owner = -1, last = 0;
+            double at = 0.0;
+            for (int r = 0; r < C; ++r) {
+              const double x = s.slice[r];
+              if (owner < 0 && x > 0.0 && before + x > t) {
+                owner = r;
+                at = t - before;
+              }
+              if (x > 0.0) last = r;
+              before += x;
+            }
+            c.op = 1;
+            c.any = owner < 0;
+            c.owner = owner < 0 ? last : owner;
+            c.target = at;
+            c.slot = a;
+          }
+        }
+      }
+      have_sum = c.op == 0;
+      // lanes 0 .. C-1 each hand the command to one CTA (the rejected tokens and sums with it)
+      if (lane < C) *cl.map_shared_rank(&s.cmd, lane) = c;
+      if (c.op != 2)
+        for (int r = 1; r < C; ++r)
+          for (int i = lane; i < c.rej; i += 32) {
+            if (DRAFT) {
+              cl.map_shared_rank(s.z, r)[i] = s.z[i];
+            } else {
+              cl.map_shared_rank(s.rejected, r)[i] = s.rejected[i];
+            }
+          }
+    }
+    cl.sync();
+    const TvCmd c = s.cmd;
+    if (c.op == 2) break;
+    const E* pr = probs + (long long)c.row * ldp;
+    const E* qr = DRAFT ? draft + (long long)c.row * ldq : nullptr;
+    auto weight = [&](int i, float p, float q) -> double {
+      if constexpr (DRAFT) {
+        return tv_weight(p, q, s.z, c.rej);
+      } else {
+        for (int r = 0; r < c.rej; ++r)
+          if (s.rejected[r] == i) return 0.0;
+        return p > 0.f ? (double)p : 0.0;
+      }
+    };
+    if (c.op == 0) {
+      double sum = 0.0;
+      if (vec) {
+        for (int i = lo + lane * VE; i < hi; i += step) {
+          float p[VE], q[VE];
+          tv_loadv(pr + i, p);
+          if (DRAFT && c.rej > 0) tv_loadv(qr + i, q);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) sum += weight(i + e, p[e], DRAFT && c.rej > 0 ? q[e] : 0.f);
+        }
+      } else {
+        for (int i = lo + lane; i < hi; i += 32)
+          sum += weight(i, tv_load1(pr + i), DRAFT && c.rej > 0 ? tv_load1(qr + i) : 0.f);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) s.warp_sum[warp] = sum;
+      __syncthreads();
+      if (tid == 0) {
+        double tot = 0.0;
+        for (int w = 0; w < TV_WARPS; ++w) tot += s.warp_sum[w];
+        cl.map_shared_rank(s.slice, 0)[rank] = tot;
+      }
+      cl.sync();
+      continue;
+    }
+    if (rank == c.owner) {
+      // the warp whose slice holds the target (warp_sum is of these weights), then the element
+      double before = 0.0;
+      int mine = -1, last = 0;
+      double at = 0.0;
+      for (int w = 0; w < TV_WARPS; ++w) {
+        const double x = s.warp_sum[w];
+        if (!c.any && mine < 0 && x > 0.0 && before + x > c.target) {
+          mine = w;
+          at = c.target - before;
+        }
+        if (x > 0.0) last = w;
+        before += x;
+      }
+      const bool any = mine < 0;
+      if (warp == (any ? last : mine)) {
+        double run = 0.0;
+        int found = -1, best = 0;
+        for (int base = lo; base < hi && found < 0; base += 32) {
+          const int i = base + lane;
+          const double w = i < hi ? weight(i, tv_load1(pr + i), DRAFT && c.rej > 0 ? tv_load1(qr + i) : 0.f) : 0.0;
+          double cum = w;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double up = __shfl_up_sync(0xffffffffu, cum, o);
+            if (lane >= o) cum += up;
+          }
+          const unsigned pos = __ballot_sync(0xffffffffu, w > 0.0);
+          const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && run + cum > at);
+          if (pos) best = base + 31 - __clz(pos);
+          if (hit && !any) found = base + __ffs(hit) - 1;
+          run += __shfl_sync(0xffffffffu, cum, 31);
+        }
+        if (lane == 0) ob[c.slot] = found >= 0 ? found : best;
+      }
+    }
+    break;
+  }
+  if (rank == 0 && warp == 0) {
+    const int used = n > 0 ? a + 1 : 0;
+    if (lane == 0) {
+      if (n > 0) pb[0] = 0;
+      accepted[b] = a;
+      last_row[b] = n > 0 ? q0 + cur : -1;
+    }
+    for (int i = used + lane; i < P; i += 32) pb[i] = ob[i] = -1;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// the accepted path's rows behind the committed context: slot ctx + path[j] -> ctx + j
+// (j = 1 .. accepted) in every layer.  One CTA per (sequence, layer); a thread owns 16 bytes of
+// the row (fp8 V, transposed inside its block: one value column) and moves them for every
+// j in order.  A path rises (path[j] >= j), so no later source lies at an earlier
+// destination, and reading four rows ahead of writing them is safe.
+constexpr int TC_LAYERS = 64;   // layers of one launch (their pointers travel as parameters)
+struct TcLayers {
+  void* k[TC_LAYERS];
+  void* v[TC_LAYERS];
+};
+
+__global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant__ TcLayers layers,
+                                                          const int* __restrict__ path, int P,
+                                                          const int* __restrict__ accepted,
+                                                          const int* __restrict__ q_start,
+                                                          const int* __restrict__ kv_len,
+                                                          const int* __restrict__ bt, int bt_stride, int bt_cols,
+                                                          int num_blocks, int Hkv, int kb, int vb, int fp8_v, int Dv) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ int src[256], dst[256];   // flat cache rows (page * 64 + offset), -1: nothing to move
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int n = q_start[b + 1] - q_start[b];
+  const int ctx = kv_len[b] - n;
+  const int acc = min(min(accepted[b], P - 1), n - 1);
+  if (ctx < 0) return;
+  uint8_t* kc = static_cast<uint8_t*>(layers.k[blockIdx.y]);
+  uint8_t* vc = static_cast<uint8_t*>(layers.v[blockIdx.y]);
+  const int kch = kb >> 4, vch = vb >> 4;   // 16-byte pieces of one head's K and V row
+  for (int j0 = 1; j0 <= acc; j0 += 256) {
+    __syncthreads();
+    const int j = j0 + tid;
+    int f = -1, t = -1;
+    if (j <= acc) {
+      const int node = path[(size_t)b * P + j];
+      if (node > j && node < n) {           // node == j: already in place
+        const int fs = ctx + node, ts = ctx + j;
+        if ((fs >> 6) < bt_cols) {
+          const int fp = bt[(size_t)b * bt_stride + (fs >> 6)], tp = bt[(size_t)b * bt_stride + (ts >> 6)];
+          if (fp >= 0 && fp < num_blocks && tp >= 0 && tp < num_blocks) {
+            f = fp * 64 + (fs & 63);
+            t = tp * 64 + (ts & 63);
+          }
+        }
+      }
+    }
+    src[tid] = f;
+    dst[tid] = t;
+    __syncthreads();
+    const int cnt = min(256, acc - j0 + 1);
+    const int kw = Hkv * kch, all = kw + (fp8_v ? Hkv * Dv : Hkv * vch);
+    for (int c = tid; c < all; c += 256) {
+      if (c >= kw && fp8_v) {               // column d of head h: byte (page, h, d, offset)
+        const int col = c - kw;
+        for (int i = 0; i < cnt; ++i) {
+          const int f1 = src[i], t1 = dst[i];
+          if (f1 < 0) continue;
+          const size_t hd = (size_t)Hkv * Dv;
+          vc[((t1 >> 6) * hd + col) * 64 + (t1 & 63)] = vc[((f1 >> 6) * hd + col) * 64 + (f1 & 63)];
+        }
+        continue;
+      }
+      uint8_t* base = c < kw ? kc : vc;
+      const int ch = c < kw ? kch : vch, cc = c < kw ? c : c - kw;
+      const int h = cc / ch, o = cc - h * ch;
+      const size_t rb = (size_t)ch << 4;
+      auto at = [&](int row) {
+        return reinterpret_cast<uint4*>(base + (((size_t)(row >> 6) * Hkv + h) * 64 + (row & 63)) * rb) + o;
+      };
+      for (int i = 0; i < cnt; i += 4) {
+        uint4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i + u < cnt && src[i + u] >= 0) x[u] = *at(src[i + u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i + u < cnt && src[i + u] >= 0) *at(dst[i + u]) = x[u];
+      }
+    }
+  }
+}
+
+template <typename E, bool DRAFT>
+int tv_launch(const void* probs, long long ldp, const void* draft, long long ldq, int V, const int* tokens,
+              const int* parents, const int* q_start, const float* u_accept, const float* u_draw, int B, int P,
+              int* accepted, int* path, int* out, int* last_row, void* status, cudaStream_t s) {
+  // CTAs per sequence: a slice of at least 4096 elements each
+  const int C = V <= 4096 ? 1 : V <= 8192 ? 2 : V <= 16384 ? 4 : 8;
+  constexpr int VE = 16 / sizeof(E);
+  const bool vec = V % VE == 0 && ldp % VE == 0 && (reinterpret_cast<uintptr_t>(probs) & 15) == 0 &&
+                   (!DRAFT || (ldq % VE == 0 && (reinterpret_cast<uintptr_t>(draft) & 15) == 0));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C, B);
+  cfg.blockDim = dim3(TV_THREADS);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_verify_kernel<E, DRAFT>, static_cast<const E*>(probs), ldp,
+                                           static_cast<const E*>(draft), ldq, V, (int)vec, tokens, parents, q_start,
+                                           u_accept, u_draw, P, accepted, path, out, last_row,
+                                           reinterpret_cast<XtuStatus*>(status));
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return -(int)e;
+  }
+  return 1;
+}
+
+}  // namespace
+}  // namespace xtu
+
+using namespace xtu;
+
+extern "C" {
+
+// parents [T] -> mask [T, W] (W words of 32 nodes) and depth [T]; max_nodes <= 1024, W >= ceil(max_nodes / 32)
+int xtu_tree_mask(const int* parents, const int* q_start, int B, int max_nodes, int W, int* mask, int* depth,
+                  void* status, cudaStream_t s) {
+  if (B <= 0 || max_nodes <= 0) return 0;
+  if (max_nodes > TREE_MAX_NODES || W * 32 < max_nodes) return -2;
+  const cudaError_t e = launch_pdl(tree_mask_kernel, dim3(B, (max_nodes + 127) / 128), dim3(128), 0, s, parents,
+                                   q_start, max_nodes, W, mask, depth, reinterpret_cast<XtuStatus*>(status));
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? 1 : -(int)e;
+}
+
+// accepted [B], path [B, P], out [B, P], last_row [B]; P = the largest tree
+int xtu_tree_verify_greedy(const int* target, const int* tokens, const int* parents, const int* q_start, int B, int P,
+                           int* accepted, int* path, int* out, int* last_row, void* status, cudaStream_t s) {
+  if (B <= 0 || P <= 0) return 0;
+  if (P > TREE_MAX_NODES) return -2;
+  const cudaError_t e = launch_pdl(tree_verify_greedy_kernel, dim3(B), dim3(32), 0, s, target, tokens, parents,
+                                   q_start, P, accepted, path, out, last_row, reinterpret_cast<XtuStatus*>(status));
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? 1 : -(int)e;
+}
+
+// probs [T, V] (row stride ldp elements), draft the same or null; bf16: both bf16, else fp32
+int xtu_tree_verify(const void* probs, long long ldp, const void* draft, long long ldq, int bf16, int V,
+                    const int* tokens, const int* parents, const int* q_start, const float* u_accept,
+                    const float* u_draw, int B, int P, int* accepted, int* path, int* out, int* last_row,
+                    void* status, cudaStream_t s) {
+  if (B <= 0 || P <= 0) return 0;
+  if (P > TREE_MAX_NODES || V <= 0 || B > 65535) return -2;
+#define XTU_TV(E, D)                                                                                              \
+  return tv_launch<E, D>(probs, ldp, draft, ldq, V, tokens, parents, q_start, u_accept, u_draw, B, P, accepted, \
+                         path, out, last_row, status, s)
+  if (bf16) {
+    if (draft) XTU_TV(__nv_bfloat16, true);
+    XTU_TV(__nv_bfloat16, false);
+  }
+  if (draft) XTU_TV(float, true);
+  XTU_TV(float, false);
+#undef XTU_TV
+}
+
+// k_ptrs / v_ptrs: host arrays of L cache addresses, or null: layer l at k_base + l * k_step
+// bytes.  kb / vb: bytes of one head's K / V row (vb 16-byte pieces; fp8_v: V is [Dv][64]
+// inside a block and vb is unused).
+int xtu_tree_commit(const long long* k_ptrs, const long long* v_ptrs, long long k_base, long long k_step,
+                    long long v_base, long long v_step, int L, const int* path, int P, const int* accepted,
+                    const int* q_start, const int* kv_len, const int* bt, int bt_stride, int bt_cols, int B,
+                    int num_blocks, int Hkv, int kb, int vb, int fp8_v, int Dv, cudaStream_t s) {
+  if (B <= 0 || L <= 0 || P <= 1) return 0;
+  if (kb % 16 != 0 || (!fp8_v && vb % 16 != 0)) return -2;
+  int launches = 0;
+  for (int l0 = 0; l0 < L; l0 += TC_LAYERS) {
+    const int m = L - l0 < TC_LAYERS ? L - l0 : TC_LAYERS;
+    TcLayers t{};
+    for (int l = 0; l < m; ++l) {
+      t.k[l] = reinterpret_cast<void*>(k_ptrs ? k_ptrs[l0 + l] : k_base + (l0 + l) * k_step);
+      t.v[l] = reinterpret_cast<void*>(v_ptrs ? v_ptrs[l0 + l] : v_base + (l0 + l) * v_step);
+    }
+    const cudaError_t e = launch_pdl(tree_commit_kernel, dim3(B, m), dim3(256), 0, s, t, path, P, accepted, q_start,
+                                     kv_len, bt, bt_stride, bt_cols, num_blocks, Hkv, kb, vb, fp8_v, Dv);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return -(int)e;
+    }
+    ++launches;
+  }
+  return launches;
+}
+
+}  // extern "C"

@@ -1,0 +1,811 @@
+// Attention of a tree of drafted tokens over a paged GQA cache (sm_100a).
+//
+// Sequence b holds ctx committed keys and, behind them in node order, the keys of its n tree
+// nodes; the query of node i sees
+//   * the context, or with a sliding window the keys t > ctx + depth[i] - window of it, and
+//   * the nodes j whose bit is set in row i of the mask (its ancestors and itself; with a
+//     window those of depth[j] > depth[i] - window),
+//   o_i = sum_t p_it v_t,  p_it = exp(s q_i . k_t - m) / (sum_t exp(s q_i . k_t - m) [+ exp(sink - m)]).
+// A row that sees nothing is zero.  Keys that a row does not see never reach its result,
+// whatever bits they hold (see "masked pages").
+//
+// Rows: the G = Hq / Hkv heads of a KV head and the nodes form n * G query rows (row r = node
+// r / G, head r % G), so one pass over the keys serves them all.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <cfloat>
+#include <climits>
+#include <cstdint>
+#include "launch.cuh"
+#include "ptx.cuh"
+
+namespace xtu {
+namespace {
+
+constexpr int TA_PAGE = 64;          // keys per cache block
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct TaParams {
+  const __nv_bfloat16* q;   // [T, Hq, D]
+  long long q_ts;           // elements between tokens
+  int q_hs;                 // elements between heads
+  __nv_bfloat16* o;         // [T, Hq, DV] contiguous
+  const int* q_start;       // [B + 1]
+  const int* kv_len;        // [B] context + nodes
+  const int* block_table;   // [B, bt_stride], bt_cols columns
+  int bt_stride, bt_cols;
+  const int* mask;          // [T, W]
+  int W;
+  const int* depth;         // [T] (window > 0 only)
+  int window;
+  int Hq, Hkv, G, T;
+  float scale_log2;         // softmax scale * log2(e) (fp8: times the K scale)
+  float out_scale;          // fp8: the V scale, else 1
+  const float* sinks;       // [Hq] or null
+  int splits;
+  float* ws_o;              // [splits, T, Hq, DV] normalised partials (splits > 1)
+  float* ws_lse;            // [splits, T, Hq] m + log2(l), -FLT_MAX for an empty one
+  const void* v_raw;        // V cache (non-finite values of masked pages)
+  int num_blocks;
+  XtuStatus* status;
+};
+
+__device__ __forceinline__ float ta_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------------------------------
+// visibility
+// ---------------------------------------------------------------------------------------
+struct TaRow {
+  const int* words;   // mask row, null: the row sees nothing
+  int ctx, n;         // committed keys, nodes
+  int low;            // first context key inside the window
+  int deep;           // window: nodes of depth <= deep are outside (INT_MIN: none)
+};
+
+__device__ __forceinline__ TaRow ta_row(const TaParams& p, int q0, int n, int ctx, int node, bool valid) {
+  TaRow r;
+  r.words = valid ? p.mask + (size_t)(q0 + node) * p.W : nullptr;
+  r.ctx = ctx;
+  r.n = n;
+  r.low = 0;
+  r.deep = INT_MIN;
+  if (p.window > 0 && valid) {
+    const int far = min(max(__ldg(p.depth + q0 + node), 0), n - 1) - p.window;
+    r.low = max(0, ctx + far + 1);
+    r.deep = far;
+  }
+  return r;
+}
+
+// bits of keys key0 .. key0 + 31 that the row sees
+__device__ __forceinline__ uint32_t ta_see32(const TaParams& p, const TaRow& r, int q0, int key0) {
+  if (r.words == nullptr) return 0u;
+  const int off = key0 - r.ctx;              // node index of key0
+  uint32_t bits = 0u;
+  if (off > -32 && off < r.n) {
+    const int lo = off >= 0 ? off >> 5 : -1;
+    const uint32_t w0 = lo >= 0 && lo < p.W ? (uint32_t)__ldg(r.words + lo) : 0u;
+    const uint32_t w1 = lo + 1 < p.W ? (uint32_t)__ldg(r.words + lo + 1) : 0u;
+    const int sh = off & 31;
+    bits = sh ? __funnelshift_r(w0, w1, sh) : (off >= 0 ? w0 : w1);
+    const int left = r.n - off;              // nodes from key0 on
+    if (left < 32) bits &= (1u << left) - 1u;
+    if (r.deep >= 0) {                       // ancestors outside the window
+      for (uint32_t m = bits; m; m &= m - 1) {
+        const int e = __ffs(m) - 1;
+        if (__ldg(p.depth + q0 + off + e) <= r.deep) bits &= ~(1u << e);
+      }
+    }
+  }
+  if (off < 0) {                             // context keys key0 .. ctx - 1
+    uint32_t c = off <= -32 ? 0xffffffffu : (1u << -off) - 1u;
+    const int cut = r.low - key0;
+    if (cut >= 32) c = 0u;
+    else if (cut > 0) c &= ~((1u << cut) - 1u);
+    bits = (off <= -32 ? 0u : bits & ~((1u << -off) - 1u)) | c;
+  }
+  return bits;
+}
+
+__device__ __forceinline__ bool ta_sees(const TaParams& p, const TaRow& r, int q0, int key) {
+  return (ta_see32(p, r, q0, key & ~31) >> (key & 31)) & 1u;
+}
+
+__device__ __forceinline__ float ta_v_at(const TaParams& p, bool f8, int DV, int page, int kh, int off, int d) {
+  if (f8) {
+    const uint8_t x = static_cast<const uint8_t*>(p.v_raw)[(((size_t)page * p.Hkv + kh) * DV + d) * TA_PAGE + off];
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(x, __NV_E4M3);
+    return __half2float(__half(h));
+  }
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p.v_raw)[(((size_t)page * p.Hkv + kh) * TA_PAGE + off) * DV + d]);
+}
+
+// ---------------------------------------------------------------------------------------
+// warp-level kernel: up to 64 query rows per CTA
+// ---------------------------------------------------------------------------------------
+// One CTA = one (row tile of 16 MT rows, kv split, kv head, sequence).  Warp 0 streams 64-key
+// pages of K and V through a shared-memory ring with TMA; CW consumer warps take m-tile
+// w % MT and key subset w / MT of every page: S = Q K^T (mma.sync m16n8k16), online softmax
+// in the exp2 domain with a lazily raised maximum, O += P V.  The key subsets meet in
+// shared memory at the end.
+template <int D, int DV, bool F8, int MT>
+struct TmCfg {
+  static constexpr int CW = MT == 1 ? 4 : 8;                     // consumer warps
+  static constexpr int ESZ = F8 ? 1 : 2;
+  static constexpr int K_BYTES = TA_PAGE * D * ESZ, V_BYTES = TA_PAGE * DV * ESZ;
+  static constexpr int STAGE = K_BYTES + V_BYTES;
+  static constexpr bool QSM = D > 128;                           // Q fragments from shared memory
+  static constexpr int QLD = D + 8;
+  static constexpr int Q_BYTES = QSM ? (MT * 16 * QLD * 2 + 1023) / 1024 * 1024 : 0;
+  static constexpr int BUDGET = 220 * 1024 - Q_BYTES;
+  static constexpr int STAGES = BUDGET / STAGE > 8 ? 8 : BUDGET / STAGE;
+  static constexpr int THREADS = 32 * (1 + CW);
+  static constexpr int BYTES = 1024 + Q_BYTES + STAGES * STAGE + 2 * STAGES * 8 + 64;
+  static_assert(STAGES >= 2, "ring");
+  static_assert(CW * 16 * DV * 4 <= STAGES * STAGE, "merge buffer");
+  static_assert(D % 64 == 0 && DV % 64 == 0 && (!F8 || (D <= 128 && DV <= 128)), "head sizes");
+};
+
+__device__ __forceinline__ void tm_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void tm_mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void tm_e4m3(uint32_t w, uint32_t& lo, uint32_t& hi) {   // exact
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+
+__device__ __forceinline__ uint32_t tm_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ void tm_ldsm4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+
+__device__ __forceinline__ void tm_ldsm4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+
+// 16-byte piece `ch` of key row `r` in a bf16 page ([64 keys][128 bytes] boxes, 128B swizzle)
+__device__ __forceinline__ uint32_t tm_piece(uint32_t base, int r, int ch) {
+  return base + (ch >> 3) * 8192 + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+}
+
+// fp8 pages: byte b of row r (rows of 128 bytes: 128B swizzle, of 64 bytes: 64B swizzle)
+template <int ROWB>
+__device__ __forceinline__ uint32_t tm_f8_off(int r, int b) {
+  if (ROWB == 128) return r * 128 + ((((b >> 4) ^ (r & 7)) << 4) | (b & 15));
+  return r * 64 + ((((b >> 4) ^ ((r >> 1) & 3)) << 4) | (b & 15));
+}
+
+__device__ __forceinline__ uint32_t tm_lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ uint4 tm_lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+// non-finite bf16 values of a packed pair as a mask of the halves to clear
+__device__ __forceinline__ uint32_t bad_bf16x2(uint32_t w) {
+  return ((w & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((w & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
+}
+__device__ __forceinline__ uint32_t bad_e4m3x4(uint32_t w) {   // NaN is 0x7F / 0xFF
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (((w >> (8 * i)) & 0x7Fu) == 0x7Fu) m |= 0xFFu << (8 * i);
+  return m;
+}
+
+template <int D, int DV, bool F8, int MT>
+__global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mma_kernel(
+    const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+    const __grid_constant__ TaParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  using C = TmCfg<D, DV, F8, MT>;
+  constexpr int CW = C::CW, STAGES = C::STAGES;
+  constexpr int NS = CW / MT;            // key subsets of a page
+  constexpr int KW = TA_PAGE / NS;       // keys of a warp per page
+  constexpr int NKT = KW / 8, DK = D / 16, DN = DV / 8;
+  extern __shared__ uint8_t tm_smem[];
+  const uint32_t sa = smem_u32(tm_smem);
+  uint8_t* base = tm_smem + (((sa + 1023u) & ~1023u) - sa);
+  __nv_bfloat16* sq = reinterpret_cast<__nv_bfloat16*>(base);
+  uint8_t* ring = base + C::Q_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + STAGES * C::STAGE);
+  uint64_t* empty = full + STAGES;
+  __shared__ int s_bad;                  // a masked page held a non-finite value
+  __shared__ float cm[CW * 16], cl[CW * 16];   // maximum and sum of each warp's rows
+  const int b = blockIdx.z, kh = blockIdx.y;
+  const int tile = blockIdx.x / p.splits, sp = blockIdx.x - tile * p.splits;
+  const int q0 = __ldg(p.q_start + b), n = __ldg(p.q_start + b + 1) - q0;
+  const int L = __ldg(p.kv_len + b), ctx = L - n;
+  const int r0 = tile * 16 * MT;
+  if (r0 >= n * p.G) return;             // uniform: no such row tile here
+  const int nrows = min(16 * MT, n * p.G - r0);
+  if (threadIdx.x == 0) {
+    s_bad = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], CW);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+  // pages of this split; with a window none below the first key that the tile's rows can see
+  // (the root's window reaches furthest back)
+  const int npages = min((L + TA_PAGE - 1) / TA_PAGE, p.bt_cols);
+  const int jfirst = p.window > 0 ? max(0, ctx - p.window + 1) / TA_PAGE : 0;
+  const int per = (npages - jfirst + p.splits - 1) / p.splits;
+  const int j0 = min(npages, jfirst + sp * per), j1 = min(npages, j0 + per);
+  const int nj = max(0, j1 - j0);
+  // pages below `open` and at or past `shut` are seen whole by every row; the others
+  // ("masked pages": the tree's own, the last, and with a window those it cuts) are not
+  const int shut = ctx / TA_PAGE;
+  const int open = p.window > 0 ? (max(0, ctx + n - p.window) + TA_PAGE - 1) / TA_PAGE : 0;   // depth < n
+  auto masked = [&](int page) { return page >= shut || page < open; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    // ---------------- producer
+    if (lane == 0) {
+      prefetch_tmap(&tk);
+      prefetch_tmap(&tv);
+    }
+    bool ok = true;
+    int issued = 0;
+    const int* bt = p.block_table + (size_t)b * p.bt_stride + j0;
+    for (int c0 = 0; c0 < nj && ok; c0 += 32) {
+      const int page = c0 + lane < nj ? __ldg(bt + c0 + lane) : 0;
+      const int cnt = min(32, nj - c0);
+      for (int k = 0; k < cnt; ++k) {
+        const int pg = __shfl_sync(0xffffffffu, page, k);
+        // a page id outside the cache reads zero fill (TMA bounds); the bounds-check build reports it
+        if (lane == 0) (void)XTU_IN_BOUNDS(pg >= 0 && pg < p.num_blocks, p.status, 243, pg);
+        if (lane == 0) {
+          const int i = c0 + k, slot = i % STAGES;
+          if (i >= STAGES && !mbar_wait(&empty[slot], ((i / STAGES) - 1) & 1, p.status, 140)) {
+            ok = false;
+          } else {
+            ++issued;
+            mbar_arrive_expect_tx(&full[slot], C::STAGE);
+            uint8_t* dst = ring + slot * C::STAGE;
+            const int pr = pg >= 0 && pg < p.num_blocks ? pg : p.num_blocks;   // past the end: zero fill
+            const int row = (pr * p.Hkv + kh) * TA_PAGE;
+            if constexpr (F8) {   // K [64 keys][D bytes]; V^T [DV rows][64 bytes]
+              tma_load_2d(dst, &tk, &full[slot], 0, row);
+              tma_load_2d(dst + C::K_BYTES, &tv, &full[slot], 0, (pr * p.Hkv + kh) * DV);
+            } else {
+#pragma unroll
+              for (int x = 0; x < D / 64; ++x) tma_load_2d(dst + x * 8192, &tk, &full[slot], x * 64, row);
+#pragma unroll
+              for (int x = 0; x < DV / 64; ++x)
+                tma_load_2d(dst + C::K_BYTES + x * 8192, &tv, &full[slot], x * 64, row);
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) break;
+      }
+    }
+    if (!ok && lane == 0) {   // let the copies in flight land (bounded) before the CTA exits
+      for (int j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j)
+        mbar_wait(&full[j % STAGES], (j / STAGES) & 1, nullptr, 0, 50000000ull);
+    }
+    return;
+  }
+  // ---------------- consumers
+  const int cw = warp - 1, ctid = threadIdx.x - 32;
+  const int mt = cw % MT, ks = cw / MT;
+  const int g4 = lane >> 2, tq = lane & 3;
+  TaRow row[2];
+  uint32_t qa[C::QSM ? 1 : DK][4];
+#pragma unroll
+  for (int h2 = 0; h2 < 2; ++h2) {
+    const int r = mt * 16 + g4 + h2 * 8;
+    const bool valid = r < nrows;
+    const int node = valid ? (r0 + r) / p.G : 0, hh = valid ? (r0 + r) - node * p.G : 0;
+    row[h2] = ta_row(p, q0, n, ctx, node, valid);
+    const __nv_bfloat16* qrow = p.q + (long long)(q0 + node) * p.q_ts + (long long)(kh * p.G + hh) * p.q_hs;
+    if constexpr (F8) {
+      // k-step s of lane tq covers d = tq * D/4 + 4 s + {0,1 | 2,3}: the order in which a lane
+      // reads K bytes, four at a time.  Q is rounded to f16 (11 bits of bf16's 8: exact
+      // within f16's range)
+#pragma unroll
+      for (int k = 0; k < DK; ++k) {
+        const uint2 v = valid ? __ldg(reinterpret_cast<const uint2*>(qrow + tq * (D / 4) + 4 * k)) : make_uint2(0u, 0u);
+        qa[k][h2] = tm_f16x2(bf16_lo(v.x), bf16_hi(v.x));
+        qa[k][2 + h2] = tm_f16x2(bf16_lo(v.y), bf16_hi(v.y));
+      }
+    } else if constexpr (!C::QSM) {
+#pragma unroll
+      for (int k = 0; k < DK; ++k) {
+        qa[k][h2] = valid ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * k + 2 * tq)) : 0u;
+        qa[k][2 + h2] = valid ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * k + 8 + 2 * tq)) : 0u;
+      }
+    }
+  }
+  if constexpr (C::QSM) {
+    for (int i = ctid; i < MT * 16 * (D / 8); i += 32 * CW) {
+      const int r = i / (D / 8), c = (i - r * (D / 8)) * 8;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (r < nrows) {
+        const int node = (r0 + r) / p.G, hh = (r0 + r) - node * p.G;
+        v = __ldg(reinterpret_cast<const uint4*>(p.q + (long long)(q0 + node) * p.q_ts +
+                                                 (long long)(kh * p.G + hh) * p.q_hs + c));
+      }
+      *reinterpret_cast<uint4*>(sq + r * C::QLD + c) = v;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory");
+  }
+  float o[DN][4];
+#pragma unroll
+  for (int i = 0; i < DN; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  bool ok = true;
+  for (int i = 0; i < nj; ++i) {
+    const int slot = i % STAGES;
+    if (ok && !mbar_wait(&full[slot], (i / STAGES) & 1, p.status, 141)) ok = false;
+    const bool msk = masked(j0 + i);
+    const uint32_t kb = smem_u32(ring + slot * C::STAGE), vb = kb + C::K_BYTES;
+    if (msk) {
+      // masked pages: 0 * p must stay 0 for keys that a row does not see, so V's non-finite
+      // values become zero here and join the rows that do see them at the end.  Every
+      // consumer warp passes these two barriers, a timed-out one too.
+      if (ok) {
+        uint32_t* vw = reinterpret_cast<uint32_t*>(ring + slot * C::STAGE + C::K_BYTES);
+        bool any = false;
+        for (int w = ctid; w < C::V_BYTES / 4; w += 32 * CW) {
+          const uint32_t x = vw[w], bad = F8 ? bad_e4m3x4(x) : bad_bf16x2(x);
+          if (bad) {
+            vw[w] = x & ~bad;
+            any = true;
+          }
+        }
+        if (any) s_bad = 1;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory");
+    }
+    if (!ok) continue;
+    const int key_lo = ks * KW;                              // this warp's first key in the page
+    const int kabs = (j0 + i) * TA_PAGE + key_lo;
+    // ---- S = Q K^T
+    float s[NKT][4];
+#pragma unroll
+    for (int nt = 0; nt < NKT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+    if constexpr (F8) {
+#pragma unroll
+      for (int nt = 0; nt < NKT; ++nt) {
+        // n-position g4 of tile nt is key 16 (nt/2) + 4 (g4/2) + 2 (nt%2) + g4%2 of the warp's keys,
+        // so that a lane's four P values below are four consecutive keys
+        const int r = key_lo + 16 * (nt >> 1) + 4 * (g4 >> 1) + 2 * (nt & 1) + (g4 & 1);
+        uint32_t w[D / 16];
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const uint4 v = tm_lds128(kb + tm_f8_off<D>(r, tq * (D / 4) + 16 * c));
+          w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+        }
+#pragma unroll
+        for (int k = 0; k < DK; ++k) {
+          uint32_t b0, b1;
+          tm_e4m3(w[k], b0, b1);
+          tm_mma_f16(s[nt], qa[k], b0, b1);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int kc = 0; kc < DK / 2; ++kc) {
+        uint32_t a0[4], a1[4];
+        if constexpr (C::QSM) {
+          const uint32_t qb = smem_u32(sq + (mt * 16 + (lane & 15)) * C::QLD + kc * 32 + (lane >> 4) * 8);
+          tm_ldsm4(qb, a0[0], a0[1], a0[2], a0[3]);
+          tm_ldsm4(qb + 32, a1[0], a1[1], a1[2], a1[3]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NKT; ++nt) {
+          uint32_t b0, b1, b2, b3;
+          tm_ldsm4(tm_piece(kb, key_lo + nt * 8 + (lane & 7), kc * 4 + (lane >> 3)), b0, b1, b2, b3);
+          if constexpr (C::QSM) {
+            tm_mma(s[nt], a0, b0, b1);
+            tm_mma(s[nt], a1, b2, b3);
+          } else {
+            tm_mma(s[nt], qa[2 * kc], b0, b1);
+            tm_mma(s[nt], qa[2 * kc + 1], b2, b3);
+          }
+        }
+      }
+    }
+    // ---- scale, mask, online softmax (rows h2 = 0: g4, 1: g4 + 8)
+    uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+    if (msk) {
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        see[h2] = ta_see32(p, row[h2], q0, kabs & ~31) >> (kabs & 31);
+        static_assert(KW <= 32, "a warp's keys lie in one aligned word");
+      }
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int nt = 0; nt < NKT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = F8 ? 16 * (nt >> 1) + 4 * tq + 2 * (nt & 1) + (e & 1) : nt * 8 + 2 * tq + (e & 1);
+        float v = s[nt][e] * p.scale_log2;
+        if (msk) v = (see[e >> 1] >> key) & 1u ? v : -INFINITY;
+        s[nt][e] = v;
+        mx[e >> 1] = fmaxf(mx[e >> 1], v);
+      }
+    bool need = false;
+    float mnew[2];
+#pragma unroll
+    for (int h2 = 0; h2 < 2; ++h2) {
+      mx[h2] = fmaxf(mx[h2], __shfl_xor_sync(0xffffffffu, mx[h2], 1));
+      mx[h2] = fmaxf(mx[h2], __shfl_xor_sync(0xffffffffu, mx[h2], 2));
+      mnew[h2] = fmaxf(m[h2], mx[h2]);
+      need |= mnew[h2] > m[h2] + 8.f;
+    }
+    // the maximum moves only when it grows by more than 2^8: P stays below 2^8, and O is rarely rescaled
+    if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        const bool up = mnew[h2] > m[h2] + 8.f;
+        const float f = up ? ta_ex2(m[h2] - mnew[h2]) : 1.f;
+        if (up) m[h2] = mnew[h2];
+        l[h2] *= f;
+#pragma unroll
+        for (int i2 = 0; i2 < DN; ++i2) {
+          o[i2][2 * h2] *= f;
+          o[i2][2 * h2 + 1] *= f;
+        }
+      }
+    }
+    const float mb[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    uint32_t pa[NKT / 2][4];
+#pragma unroll
+    for (int nt = 0; nt < NKT; ++nt) {
+      float pv[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pv[e] = ta_ex2(s[nt][e] - mb[e >> 1]);
+        l[e >> 1] += pv[e];
+      }
+      // P is rounded to the MMA's 16-bit type (bf16: half a step of 2^-8); l keeps the 32-bit sum
+      pa[nt >> 1][(nt & 1) * 2 + 0] = F8 ? tm_f16x2(pv[0], pv[1]) : pack_bf16x2(pv[0], pv[1]);
+      pa[nt >> 1][(nt & 1) * 2 + 1] = F8 ? tm_f16x2(pv[2], pv[3]) : pack_bf16x2(pv[2], pv[3]);
+    }
+    // ---- O += P V
+#pragma unroll
+    for (int kk = 0; kk < NKT / 2; ++kk) {
+      if constexpr (F8) {
+#pragma unroll
+        for (int dn = 0; dn < DN; ++dn) {
+          uint32_t b0, b1;
+          tm_e4m3(tm_lds32(vb + tm_f8_off<64>(dn * 8 + g4, key_lo + 16 * kk + 4 * tq)), b0, b1);
+          tm_mma_f16(o[dn], pa[kk], b0, b1);
+        }
+      } else {
+        const int r = key_lo + kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+        for (int dn2 = 0; dn2 < DN / 2; ++dn2) {
+          uint32_t b0, b1, b2, b3;
+          tm_ldsm4_t(tm_piece(vb, r, 2 * dn2 + (lane >> 4)), b0, b1, b2, b3);
+          tm_mma(o[2 * dn2], pa[kk], b0, b1);
+          tm_mma(o[2 * dn2 + 1], pa[kk], b2, b3);
+        }
+      }
+    }
+    fence_proxy_async_smem();   // generic-proxy accesses of the slot before the TMA that refills it
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[slot]);
+  }
+  // ---- merge the key subsets of each m-tile (every copy has landed: the ring is free)
+#pragma unroll
+  for (int h2 = 0; h2 < 2; ++h2) {
+    l[h2] += __shfl_xor_sync(0xffffffffu, l[h2], 1);
+    l[h2] += __shfl_xor_sync(0xffffffffu, l[h2], 2);
+  }
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory");
+  float* co = reinterpret_cast<float*>(ring);             // [CW][16][DV]
+  {
+    float* mine = co + cw * 16 * DV;
+#pragma unroll
+    for (int i = 0; i < DN; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[(g4 + (e >> 1) * 8) * DV + i * 8 + 2 * tq + (e & 1)] = o[i][e];
+    if (tq == 0) {
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        cm[cw * 16 + g4 + h2 * 8] = ok ? m[h2] : -INFINITY;
+        cl[cw * 16 + g4 + h2 * 8] = ok ? l[h2] : 0.f;
+      }
+    }
+  }
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory");
+  constexpr int C4 = DV / 4;
+  for (int idx = ctid; idx < nrows * C4; idx += 32 * CW) {
+    const int r = idx / C4, c = (idx - r * C4) * 4;
+    const int rm = r >> 4, rr = r & 15;
+    float M = -INFINITY;
+#pragma unroll
+    for (int s2 = 0; s2 < NS; ++s2) M = fmaxf(M, cm[(s2 * MT + rm) * 16 + rr]);
+    const float Mb = M == -INFINITY ? 0.f : M;
+    float Ls = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s2 = 0; s2 < NS; ++s2) {
+      const int w = s2 * MT + rm;
+      const float wgt = ta_ex2(cm[w * 16 + rr] - Mb);
+      Ls += wgt * cl[w * 16 + rr];
+      const float4 v = *reinterpret_cast<const float4*>(co + (w * 16 + rr) * DV + c);
+      acc[0] += wgt * v.x;
+      acc[1] += wgt * v.y;
+      acc[2] += wgt * v.z;
+      acc[3] += wgt * v.w;
+    }
+    const int node = (r0 + r) / p.G, hh = (r0 + r) - node * p.G;
+    const int tok = q0 + node, head = kh * p.G + hh;
+    // the sink joins the denominator only (once: here, or in the merge of the splits)
+    if (p.sinks != nullptr && p.splits == 1 && M != -INFINITY) Ls += ta_ex2(__ldg(p.sinks + head) * LOG2E - M);
+    const float inv = Ls > 0.f || Ls != Ls ? p.out_scale / Ls : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= inv;
+    if (s_bad) {   // rare: non-finite values of masked pages, for the rows that see them
+      const TaRow rw = ta_row(p, q0, n, ctx, node, true);
+      for (int pg = j0; pg < j1; ++pg) {
+        if (!masked(pg)) continue;
+        const int page = __ldg(p.block_table + (size_t)b * p.bt_stride + pg);
+        if (page < 0 || page >= p.num_blocks) continue;
+        for (int k2 = 0; k2 < TA_PAGE; ++k2) {
+          if (!ta_sees(p, rw, q0, pg * TA_PAGE + k2)) continue;
+          for (int e = 0; e < 4; ++e) {
+            const float v = ta_v_at(p, F8, DV, page, kh, k2, c + e);
+            if (!isfinite(v)) acc[e] += v;
+          }
+        }
+      }
+    }
+    if (p.splits == 1) {
+      uint2 pk;
+      pk.x = pack_bf16x2(acc[0], acc[1]);
+      pk.y = pack_bf16x2(acc[2], acc[3]);
+      *reinterpret_cast<uint2*>(p.o + ((size_t)tok * p.Hq + head) * DV + c) = pk;
+    } else {
+      *reinterpret_cast<float4*>(p.ws_o + (((size_t)sp * p.T + tok) * p.Hq + head) * DV + c) =
+          make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (c == 0)
+        p.ws_lse[((size_t)sp * p.T + tok) * p.Hq + head] = Ls > 0.f || Ls != Ls ? M + __log2f(Ls) : -FLT_MAX;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// the splits' normalised partials by their log-sum-exp: one warp per (token, head)
+// ---------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) tree_attn_merge_kernel(const float* __restrict__ ws_o,
+                                                              const float* __restrict__ ws_lse, int splits,
+                                                              int rows, int Hq, int DV, const int* __restrict__ q_start,
+                                                              int B, const float* __restrict__ sinks,
+                                                              __nv_bfloat16* __restrict__ o) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int used = q_start[B] * Hq;            // rows behind the last sequence stay as they are
+  if (w >= min(rows, used) || w < q_start[0] * Hq) return;
+  const float sk = sinks != nullptr ? __ldg(sinks + w % Hq) * LOG2E : -FLT_MAX;
+  // lane s holds split s (at most 64 splits: two per lane)
+  const float a = lane < splits ? __ldg(ws_lse + (size_t)lane * rows + w) : -FLT_MAX;
+  const float c = lane + 32 < splits ? __ldg(ws_lse + (size_t)(lane + 32) * rows + w) : -FLT_MAX;
+  float M = fmaxf(a, c);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  const bool some = __any_sync(0xffffffffu, a != -FLT_MAX || c != -FLT_MAX);   // NaN counts as some
+  M = fmaxf(M, sk);
+  const float wa = a == -FLT_MAX ? 0.f : ta_ex2(a - M), wc = c == -FLT_MAX ? 0.f : ta_ex2(c - M);
+  float sum = wa + wc;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+  if (sk != -FLT_MAX) sum += ta_ex2(sk - M);
+  const float inv = some ? 1.f / sum : 0.f;
+  for (int d0 = 0; d0 < DV; d0 += 128) {
+    const int d = d0 + lane * 4;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, s < 32 ? wa : wc, s & 31);
+      const float ls = __shfl_sync(0xffffffffu, s < 32 ? a : c, s & 31);
+      if (ls == -FLT_MAX || d >= DV) continue;   // empty: nothing was written
+      const float4 v = __ldg(reinterpret_cast<const float4*>(ws_o + ((size_t)s * rows + w) * DV + d));
+      acc[0] += ws * v.x;
+      acc[1] += ws * v.y;
+      acc[2] += ws * v.z;
+      acc[3] += ws * v.w;
+    }
+    if (d >= DV) continue;
+    uint2 pk;
+    pk.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    pk.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<uint2*>(o + (size_t)w * DV + d) = pk;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------
+typedef CUresult (*TaEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+TaEncode ta_encode() {
+  static const TaEncode fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* ptr = nullptr;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<TaEncode>(ptr)
+               : nullptr;
+  }();
+  return fn;
+}
+
+// [rows, cols] matrix, boxes of box_rows x box_cols
+int ta_map(CUtensorMap* map, CUtensorMapDataType t, int esz, const void* base, uint64_t rows, uint32_t cols,
+           uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle sw) {
+  const TaEncode enc = ta_encode();
+  if (!enc) return -100;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return -101;
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {(cuuint64_t)cols * esz};
+  const cuuint32_t box[2] = {box_cols, box_rows}, es[2] = {1, 1};
+  const CUresult r = enc(map, t, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -1000 - (int)r;
+}
+
+// the kernel's shared-memory limit, once per device
+template <typename K>
+int ta_allow(K kern, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -102;
+  if (done[dev]) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return -(int)e;
+  }
+  done[dev] = true;
+  return 0;
+}
+
+template <int D, int DV, bool F8, int MT>
+int tm_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int tiles, int B, cudaStream_t s) {
+  using C = TmCfg<D, DV, F8, MT>;
+  static bool done[64] = {};
+  if (const int rc = ta_allow(tree_attn_mma_kernel<D, DV, F8, MT>, C::BYTES, done)) return rc;
+  const cudaError_t e = launch_pdl(tree_attn_mma_kernel<D, DV, F8, MT>, dim3(tiles * p.splits, p.Hkv, B),
+                                   dim3(C::THREADS), C::BYTES, s, tk, tv, p);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? 1 : -(int)e;
+}
+
+template <int D, int DV, bool F8>
+int tm_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int B, cudaStream_t s) {
+  if (rows <= 16) return tm_launch<D, DV, F8, 1>(tk, tv, p, 1, B, s);
+  if (rows <= 32) return tm_launch<D, DV, F8, 2>(tk, tv, p, 1, B, s);
+  return tm_launch<D, DV, F8, 4>(tk, tv, p, (rows + 63) / 64, B, s);
+}
+
+}  // namespace
+}  // namespace xtu
+
+using namespace xtu;
+
+extern "C" {
+
+// q [T, Hq, D] (strides q_ts, q_hs), caches [num_blocks, Hkv, 64, D | DV] bf16, or fp8 K
+// [num_blocks, Hkv, 64, D] and V [num_blocks, Hkv, DV, 64]; o [T, Hq, DV] bf16.  ws: splits *
+// T * Hq * (DV + 2) floats when splits > 1 (<= 64).  Returns the launches, < 0 on error.
+int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_cache, const void* v_cache, int fp8,
+                       void* o, const int* q_start, const int* kv_len, const int* block_table, int bt_stride,
+                       int bt_cols, const int* mask, int W, const int* depth, int window, int B, int max_nodes, int T,
+                       int Hq, int Hkv, int D, int DV, int num_blocks, float scale, float k_scale, float v_scale,
+                       const float* sinks, int splits, float* ws, void* status, cudaStream_t s) {
+  if (B <= 0 || T <= 0 || max_nodes <= 0) return 0;
+  if (Hkv <= 0 || Hq % Hkv != 0 || B > 65535 || Hkv > 65535 || W <= 0) return -2;
+  if (splits < 1 || splits > 64 || (splits > 1 && ws == nullptr)) return -3;
+  if (window > 0 && depth == nullptr) return -4;
+  TaParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_ts = q_ts;
+  p.q_hs = q_hs;
+  p.o = static_cast<__nv_bfloat16*>(o);
+  p.q_start = q_start;
+  p.kv_len = kv_len;
+  p.block_table = block_table;
+  p.bt_stride = bt_stride;
+  p.bt_cols = bt_cols;
+  p.mask = mask;
+  p.W = W;
+  p.depth = depth;
+  p.window = window > 0 ? window : 0;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.G = Hq / Hkv;
+  p.T = T;
+  p.scale_log2 = scale * LOG2E * (fp8 ? k_scale : 1.f);
+  p.out_scale = fp8 ? v_scale : 1.f;
+  p.sinks = sinks;
+  p.splits = splits;
+  p.ws_o = ws;
+  p.ws_lse = ws ? ws + (size_t)splits * T * Hq * DV : nullptr;
+  p.v_raw = v_cache;
+  p.num_blocks = num_blocks;
+  p.status = reinterpret_cast<XtuStatus*>(status);
+  const uint64_t krows = (uint64_t)num_blocks * Hkv * TA_PAGE;
+  CUtensorMap tk, tv;
+  int rc;
+  if (fp8) {
+    rc = ta_map(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, k_cache, krows, D, TA_PAGE, D,
+                D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc == 0)
+      rc = ta_map(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, v_cache, (uint64_t)num_blocks * Hkv * DV, TA_PAGE, DV,
+                  TA_PAGE, CU_TENSOR_MAP_SWIZZLE_64B);
+  } else {
+    rc = ta_map(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, k_cache, krows, D, TA_PAGE, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == 0)
+      rc = ta_map(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, v_cache, krows, DV, TA_PAGE, 64,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  if (rc) return rc;
+  const int rows = max_nodes * p.G;
+  int r = -6;   // head sizes not served
+  if (fp8 && D == 64 && DV == 64) r = tm_rows<64, 64, true>(tk, tv, p, rows, B, s);
+  else if (fp8 && D == 128 && DV == 128) r = tm_rows<128, 128, true>(tk, tv, p, rows, B, s);
+  else if (fp8) return -6;
+  else if (D == 64 && DV == 64) r = tm_rows<64, 64, false>(tk, tv, p, rows, B, s);
+  else if (D == 128 && DV == 128) r = tm_rows<128, 128, false>(tk, tv, p, rows, B, s);
+  else if (D == 192 && DV == 128) r = tm_rows<192, 128, false>(tk, tv, p, rows, B, s);
+  else if (D == 256 && DV == 256) r = tm_rows<256, 256, false>(tk, tv, p, rows, B, s);
+  if (r < 0 || splits == 1) return r;
+  const int heads = T * Hq;
+  const cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((heads + 7) / 8), dim3(256), 0, s,
+                                   (const float*)p.ws_o, (const float*)p.ws_lse, splits, heads, Hq, DV, q_start, B,
+                                   sinks, p.o);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? r + 1 : -(int)e;
+}
+
+}  // extern "C"

@@ -26,7 +26,7 @@ _CUDA_LIB = _LIB_DIR / ("libxtu_cuda_checked.so" if os.environ.get("XTU_CHECKED"
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
-c_int, c_float, c_void_p = ctypes.c_int, ctypes.c_float, ctypes.c_void_p
+c_int, c_float, c_void_p, c_longlong = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong
 P = c_void_p  # device pointer / stream handle
 
 # name -> argtypes (all return int status: 0 ok, <0 error)
@@ -70,6 +70,14 @@ _SIGS: dict[str, list] = {
     "xtu_deltanet_spec_commit": [P, P, c_int, c_int, P, P, ctypes.c_longlong, P, P, ctypes.c_longlong, P],
     "xtu_grouped_gemm_ex": [P, P, P, P, c_int, P, c_int, c_int, c_int, c_int, c_int, P, P, c_int, c_int, P, P,
                             c_float, c_float, c_float, P, c_int, P, P],
+    "xtu_tree_mask": [P, P, c_int, c_int, c_int, P, P, P, P],
+    "xtu_tree_attention": [P, c_longlong, c_int, P, P, c_int, P, P, P, P, c_int, c_int, P, c_int, P, c_int, c_int,
+                           c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_float, P, c_int, P, P,
+                           P],
+    "xtu_tree_verify_greedy": [P, P, P, P, c_int, c_int, P, P, P, P, P, P],
+    "xtu_tree_verify": [P, c_longlong, P, c_longlong, c_int, c_int, P, P, P, P, P, c_int, c_int, P, P, P, P, P, P],
+    "xtu_tree_commit": [P, P, c_longlong, c_longlong, c_longlong, c_longlong, c_int, P, c_int, P, P, P, P, c_int,
+                        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P],
     "xtu_ipc_handle_size": [],
     "xtu_ipc_handle": [P, P, ctypes.POINTER(ctypes.c_longlong)],
     "xtu_ipc_open": [P, ctypes.c_longlong, ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p)],

@@ -1,0 +1,506 @@
+"""Tree speculation: one step verifies a tree of drafted tokens per sequence.
+
+A chain of drafts (``engine/spec_decode.py``) gives up at its first wrong token; a tree keeps
+alternatives.  The nodes of sequence b are the rows ``q_start[b] .. q_start[b+1] - 1`` of the step:
+node 0 the root (the last emitted token), every other node a drafted token below a parent of
+lower index (``parents``, node indices inside the sequence, -1 for the root).  A step
+
+1. ``tree_mask``       turns the parents into ancestor bit rows and depths (a node's position is
+                       context length + depth),
+2. writes the nodes' K / V behind the context, node i at slot context + i
+   (``basic.rope_and_cache`` with those slots and positions),
+3. ``tree_attention``  attends from every node to the context and to its ancestors, beside
+                       :func:`attention.paged_attention` and over the same paged caches,
+4. ``verify_tree_greedy`` / ``verify_tree``  choose the accepted path and the token after it,
+5. ``commit_tree``     moves the accepted nodes' K / V to the slots behind the context, in every layer.
+
+The kernels are in ``csrc/cuda/tree.cu`` and ``csrc/cuda/tree_attention.cu``; on CPU tensors the
+``*_ref`` restatements run.  All calls work on the current stream of their tensors' device, copy
+nothing to the host and can be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _native as N
+from .attention import KV_BLOCK, _gather_kv, dequant_fp8_cache
+
+MAX_NODES = 1024          # nodes of one sequence's tree
+MAX_SPLITS = 64
+_FP8 = torch.float8_e4m3fn
+# (K width, V width) that the GPU kernels serve
+HEAD_DIMS = ((64, 64), (128, 128), (192, 128), (256, 256))
+FP8_HEAD_DIMS = ((64, 64), (128, 128))
+
+
+@dataclass
+class TreeMetadata:
+    """A step's trees.  ``kv_len`` counts the context and the nodes, as in ``AttnMetadata``."""
+    num_seqs: int
+    q_start: torch.Tensor        # int32 [B+1]
+    kv_len: torch.Tensor         # int32 [B] context + nodes
+    block_table: torch.Tensor    # int32 [B, max_blocks]
+    mask: torch.Tensor           # int32 [T, W] bit j of row i: node i sees node j (of its sequence)
+    max_nodes: int               # largest tree of the step
+    max_kv_len: int
+    depth: torch.Tensor | None = None   # int32 [T]; sliding-window layers need it
+    num_splits: int = 0          # KV splits; 0: chosen from the sizes
+
+
+@dataclass
+class TreeVerdict:
+    accepted: torch.Tensor       # int32 [B] accepted drafts
+    path: torch.Tensor           # int32 [B, max_nodes] the root and the accepted nodes, then -1
+    tokens: torch.Tensor         # int32 [B, max_nodes] accepted tokens and the one after them, then -1
+    last_row: torch.Tensor       # int32 [B] row of the last accepted node (-1: a sequence without nodes)
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _ints(name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}, not "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _max_nodes(n: int) -> None:
+    if not 1 <= n <= MAX_NODES:
+        raise ValueError(f"max_nodes must be 1 .. {MAX_NODES}, not {n}")
+
+
+def _elsewhere(device: torch.device) -> bool:
+    return device.type == "cuda" and device.index != torch.cuda.current_device()
+
+
+# ---------------------------------------------------------------------------
+# mask
+# ---------------------------------------------------------------------------
+def tree_mask_ref(parents: torch.Tensor, q_start: torch.Tensor, max_nodes: int, mask: torch.Tensor,
+                  depth: torch.Tensor) -> None:
+    par, qs = parents.tolist(), q_start.tolist()
+    W = mask.shape[1]
+    for b in range(len(qs) - 1):
+        rows = []
+        for i in range(qs[b + 1] - qs[b]):
+            p = par[qs[b] + i]
+            rows.append((rows[p] if 0 <= p < i else 0) | 1 << i)
+            words = [rows[i] >> 32 * w & 0xFFFFFFFF for w in range(W)]
+            mask[qs[b] + i] = torch.tensor([w - (1 << 32) if w >> 31 else w for w in words], dtype=torch.int32)
+            depth[qs[b] + i] = rows[i].bit_count() - 1
+
+
+def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, max_nodes: int, mask: torch.Tensor | None = None,
+              depth: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """parents int32 [T] -> (mask int32 [T, ceil(max_nodes / 32)], depth int32 [T]).
+
+    Bit j of row i: j is node i or an ancestor of it.  A parent that is negative or not below its
+    node means none.  Rows behind the last sequence are left as they are."""
+    _max_nodes(max_nodes)
+    dev = parents.device
+    T, B = parents.shape[0], q_start.shape[0] - 1
+    _ints("parents", parents, (T,), dev)
+    _ints("q_start", q_start, (B + 1,), dev)
+    W = (max_nodes + 31) // 32
+    mask = mask if mask is not None else torch.empty(T, W, dtype=torch.int32, device=dev)
+    depth = depth if depth is not None else torch.empty(T, dtype=torch.int32, device=dev)
+    _ints("mask", mask, (T, W), dev)
+    _ints("depth", depth, (T,), dev)
+    if not parents.is_cuda:
+        tree_mask_ref(parents, q_start, max_nodes, mask, depth)
+        return mask, depth
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return tree_mask(parents, q_start, max_nodes, mask, depth)
+    N.call("xtu_tree_mask", parents.data_ptr(), q_start.data_ptr(), B, max_nodes, W, mask.data_ptr(),
+           depth.data_ptr(), N.status_buffer(dev).data_ptr(), N.stream_ptr(dev))
+    return mask, depth
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+def tree_attention_ref(q, k_cache, v_cache, meta: TreeMetadata, scale: float, out: torch.Tensor, window: int = 0,
+                       sinks: torch.Tensor | None = None, k_scale: float = 1.0, v_scale: float = 1.0) -> torch.Tensor:
+    """q [T, Hq, D] -> out [T, Hq, Dv] (fp32 math, sequence by sequence)."""
+    if k_cache.dtype == _FP8:
+        k_cache, v_cache = dequant_fp8_cache(k_cache, v_cache, k_scale, v_scale)
+    Hk = k_cache.shape[1]
+    G = q.shape[1] // Hk
+    qs, kl = meta.q_start.tolist(), meta.kv_len.tolist()
+    for b in range(meta.num_seqs):
+        r0, n = qs[b], qs[b + 1] - qs[b]
+        if n == 0:
+            continue
+        ctx = kl[b] - n
+        k = _gather_kv(k_cache, meta.block_table[b], kl[b]).float().repeat_interleave(G, dim=1)
+        v = _gather_kv(v_cache, meta.block_table[b], kl[b]).float().repeat_interleave(G, dim=1)
+        node = torch.arange(n, device=q.device)
+        tree = (meta.mask[r0:r0 + n].long()[:, node >> 5] >> (node & 31) & 1).bool()            # [i, j]
+        see = torch.ones(n, kl[b], dtype=torch.bool, device=q.device)
+        if window > 0:
+            far = meta.depth[r0:r0 + n].long().clamp(0, n - 1)[:, None] - window
+            see[:, :ctx] = torch.arange(ctx, device=q.device)[None] > ctx + far
+            tree &= meta.depth[r0:r0 + n].long()[None] > far
+        see[:, ctx:] = tree
+        s = torch.einsum("qhd,khd->hqk", q[r0:r0 + n].float(), k) * scale
+        s = s.masked_fill(~see[None], float("-inf"))
+        m = s.amax(-1, keepdim=True)
+        if sinks is not None:
+            sk = sinks.float()[:, None, None]
+            m = torch.maximum(m, sk)
+        m = m.masked_fill(m == float("-inf"), 0.0)
+        p = torch.exp(s - m)
+        z = p.sum(-1, keepdim=True)
+        if sinks is not None:
+            z = z + torch.exp(sk - m)
+        p = torch.where(see.any(-1)[None, :, None], p / z, 0.0)
+        # a key that no row sees (stale cache contents) must not meet 0 * NaN
+        v = torch.where(see.any(0)[:, None, None], v, 0.0)
+        out[r0:r0 + n] = torch.einsum("hqk,khd->qhd", p, v).to(out.dtype)
+    return out
+
+
+def tree_splits(num_seqs: int, num_kv_heads: int, rows: int, seen: int, num_sms: int = 148) -> int:
+    """KV splits of a step: as many CTAs (row tiles of 64 x KV heads x sequences x splits, one per
+    SM) as one wave holds, each with 4 pages of keys or more."""
+    ctas = max(1, -(-rows // 64) * num_kv_heads * num_seqs)
+    pages = -(-seen // KV_BLOCK)
+    return max(1, min(num_sms // ctas, pages // 4, MAX_SPLITS))
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta: TreeMetadata,
+                   scale: float | None = None, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                   window: int = 0, sinks: torch.Tensor | None = None, k_scale: float = 1.0,
+                   v_scale: float = 1.0) -> torch.Tensor:
+    """Tree nodes' queries q [T, Hq, D] bf16 over the paged cache -> [T, Hq, Dv] bf16.
+
+    Node i sees its sequence's context and the nodes of its mask row; with ``window`` > 0 only
+    keys at positions above its own minus the window (node j lies at context + ``meta.depth[j]``).
+    ``sinks`` fp32 [Hq]: learned logits in the denominator.  A row that sees nothing is zero.
+    Keys outside a row's view never reach it, whatever the cache holds there; rows behind the
+    last sequence are left as they are.
+
+    Caches as in :func:`attention.paged_attention`: bf16 ``[blocks, Hkv, 64, D]`` / ``[.., Dv]`` with
+    (D, Dv) in ``HEAD_DIMS``, or fp8 (e4m3) K and per-block transposed V with ``FP8_HEAD_DIMS``.  MLA
+    latent caches are not served.  ``workspace``: fp32, ``splits * T * Hq * (Dv + 2)`` elements when
+    the KV range is split; allocated when None or too small.  One that is passed in belongs to
+    the call until its work is done: calls that may overlap take one each."""
+    _need(q.dim() == 3 and q.dtype == torch.bfloat16 or not q.is_cuda, "q must be [T, Hq, D] bfloat16")
+    T, Hq, D = q.shape
+    dev = q.device
+    _need(k_cache.dim() == 4 and v_cache is not None and v_cache.dim() == 4, "tree attention takes a K and a V cache")
+    nb, Hk, bs, Dk = k_cache.shape
+    fp8 = k_cache.dtype == _FP8
+    Dv = v_cache.shape[2] if fp8 else v_cache.shape[3]
+    _need(tuple(v_cache.shape) == ((nb, Hk, Dv, bs) if fp8 else (nb, Hk, bs, Dv)) and Dk == D
+          and v_cache.dtype == k_cache.dtype, "K and V caches do not match each other or q")
+    _need(Hq % Hk == 0, f"{Hq} query heads do not divide over {Hk} KV heads")
+    B = meta.num_seqs
+    _max_nodes(meta.max_nodes)
+    _need(k_cache.device == dev and v_cache.device == dev, f"the caches must be on {dev}")
+    _ints("q_start", meta.q_start, (B + 1,), dev)
+    _ints("kv_len", meta.kv_len, (B,), dev)
+    bt = meta.block_table
+    _need(bt.dtype == torch.int32 and bt.dim() == 2 and bt.shape[0] >= B and bt.stride(1) == 1 and bt.device == dev,
+          "block_table must be int32 [B, blocks] with contiguous rows")
+    W = meta.mask.shape[1]
+    _ints("mask", meta.mask, (T, W), dev)
+    _need(32 * W >= meta.max_nodes, f"a mask of {W} words is too narrow for {meta.max_nodes} nodes")
+    if window > 0:
+        _need(meta.depth is not None, "a sliding window needs the nodes' depths")
+        _ints("depth", meta.depth, (T,), dev)
+    if sinks is not None:
+        _need(sinks.dtype == torch.float32 and sinks.is_contiguous() and sinks.numel() == Hq and sinks.device == dev,
+              f"sinks must be fp32 [{Hq}]")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if out is None:
+        out = torch.empty(T, Hq, Dv, dtype=q.dtype, device=dev)
+    _need(tuple(out.shape) == (T, Hq, Dv) and out.dtype == q.dtype and out.is_contiguous() and out.device == dev,
+          f"out must be contiguous {q.dtype} [{T}, {Hq}, {Dv}]")
+    if not q.is_cuda:
+        return tree_attention_ref(q, k_cache, v_cache, meta, scale, out, window, sinks, k_scale, v_scale)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return tree_attention(q, k_cache, v_cache, meta, scale, out, workspace, window, sinks, k_scale, v_scale)
+    _need(fp8 or k_cache.dtype == torch.bfloat16, "the cache must be bfloat16 or float8_e4m3fn")
+    _need((D, Dv) in (FP8_HEAD_DIMS if fp8 else HEAD_DIMS),
+          f"{'fp8 ' if fp8 else ''}head sizes {D} / {Dv} are not served ({FP8_HEAD_DIMS if fp8 else HEAD_DIMS})")
+    _need(bs == KV_BLOCK, f"the GPU kernels read KV blocks of {KV_BLOCK} tokens, not {bs}")
+    _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "the caches must be contiguous")
+    _need(nb > 0 and (nb + 1) * Hk * max(bs, Dv) < 2 ** 31, "the cache has more rows than 31 bits count")
+    _need(q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0 and q.data_ptr() % 16 == 0,
+          "q rows must be contiguous and start on 16-byte boundaries")
+    rows = meta.max_nodes * (Hq // Hk)
+    seen = min(meta.max_kv_len, window + meta.max_nodes + KV_BLOCK) if window > 0 else meta.max_kv_len
+    splits = meta.num_splits if meta.num_splits > 0 else tree_splits(B, Hk, rows, seen)
+    _need(splits <= MAX_SPLITS, f"at most {MAX_SPLITS} splits")
+    ws = None
+    if splits > 1:
+        need = splits * T * Hq * (Dv + 2)
+        ws = workspace
+        if ws is not None:
+            _need(ws.dtype == torch.float32 and ws.is_contiguous() and ws.device == dev and ws.data_ptr() % 16 == 0,
+                  "workspace must be contiguous fp32 on q's device")
+        if ws is None or ws.numel() < need:
+            ws = torch.empty(need, dtype=torch.float32, device=dev)
+    N.call("xtu_tree_attention", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
+           int(fp8), out.data_ptr(), meta.q_start.data_ptr(), meta.kv_len.data_ptr(), bt.data_ptr(), bt.stride(0),
+           bt.shape[1], meta.mask.data_ptr(), W, N.ptr(meta.depth), int(window), B, meta.max_nodes, T, Hq, Hk, D, Dv,
+           nb, float(scale), float(k_scale), float(v_scale), N.ptr(sinks), splits, N.ptr(ws),
+           N.status_buffer(dev).data_ptr(), N.stream_ptr(dev))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# verification
+# ---------------------------------------------------------------------------
+def _verdict(B: int, max_nodes: int, device) -> TreeVerdict:
+    buf = torch.empty(2 * B * (max_nodes + 1), dtype=torch.int32, device=device)
+    n = B * max_nodes
+    return TreeVerdict(accepted=buf[2 * n:2 * n + B], path=buf[:n].view(B, max_nodes),
+                       tokens=buf[n:2 * n].view(B, max_nodes), last_row=buf[2 * n + B:])
+
+
+def _children(parents: list, n: int, at: int) -> list:
+    return [i for i in range(1, n) if parents[i] == at and at < i]
+
+
+def _walk(tokens, parents, q_start, max_nodes, choose, final) -> TreeVerdict:
+    """The verification of every sequence on the host: ``choose(row, children)`` -> the accepted
+    child or None, ``final(row, children, b)`` -> the token after the path."""
+    qs, par, tok = q_start.tolist(), parents.tolist(), tokens.tolist()
+    v = _verdict(len(qs) - 1, max_nodes, tokens.device)
+    for t in (v.path, v.tokens, v.last_row):
+        t.fill_(-1)
+    v.accepted.zero_()
+    for b in range(len(qs) - 1):
+        q0, n = qs[b], qs[b + 1] - qs[b]
+        if n == 0:
+            continue
+        mine, path = par[q0:q0 + n], [0]
+        while True:
+            kids = _children(mine, n, path[-1])
+            c = choose(q0, path[-1], kids)
+            if c is None:
+                break
+            path.append(c)
+        v.accepted[b] = len(path) - 1
+        v.path[b, :len(path)] = torch.tensor(path, dtype=torch.int32)
+        v.tokens[b, :len(path)] = torch.tensor([tok[q0 + i] for i in path[1:]] + [final(q0, path[-1], kids, b)],
+                                               dtype=torch.int32)
+        v.last_row[b] = q0 + path[-1]
+    return v
+
+
+def _tree_args(tokens, parents, q_start, max_nodes):
+    _max_nodes(max_nodes)
+    T, B, dev = tokens.shape[0], q_start.shape[0] - 1, tokens.device
+    _ints("tokens", tokens, (T,), dev)
+    _ints("parents", parents, (T,), dev)
+    _ints("q_start", q_start, (B + 1,), dev)
+    return T, B, dev
+
+
+def verify_tree_greedy_ref(target, tokens, parents, q_start, max_nodes) -> TreeVerdict:
+    tgt, tok = target.tolist(), tokens.tolist()
+    return _walk(tokens, parents, q_start, max_nodes,
+                 lambda q0, at, kids: next((c for c in kids if tok[q0 + c] == tgt[q0 + at]), None),
+                 lambda q0, at, kids, b: tgt[q0 + at])
+
+
+def verify_tree_greedy(target: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, q_start: torch.Tensor,
+                       max_nodes: int) -> TreeVerdict:
+    """Greedy verification: ``target`` int32 [T] holds the model's token after every node.  From the
+    root the path takes the first child (lowest index) whose token is the target's, and ends
+    with the target's token after the last accepted node (``verify_greedy`` for trees)."""
+    T, B, dev = _tree_args(tokens, parents, q_start, max_nodes)
+    _ints("target", target, (T,), dev)
+    if not tokens.is_cuda:
+        return verify_tree_greedy_ref(target, tokens, parents, q_start, max_nodes)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return verify_tree_greedy(target, tokens, parents, q_start, max_nodes)
+    v = _verdict(B, max_nodes, dev)
+    N.call("xtu_tree_verify_greedy", target.data_ptr(), tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), B,
+           max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
+           N.status_buffer(dev).data_ptr(), N.stream_ptr(dev))
+    return v
+
+
+def verify_tree_ref(probs, tokens, parents, q_start, max_nodes, u_accept, u_draw, draft_probs=None) -> TreeVerdict:
+    tok, ua, ud = tokens.tolist(), u_accept.tolist(), u_draw.tolist()
+    V = probs.shape[1]
+    state = {}
+
+    def weights(row):       # NaN and negative entries weigh nothing
+        w = probs[row].double()
+        return torch.where(w > 0, w, 0.0)
+
+    def choose(q0, at, kids):
+        w, z, gone = weights(q0 + at), 1.0, 0.0
+        d = None
+        if draft_probs is not None:
+            d = draft_probs[q0 + at].double()
+            d = torch.where(d > 0, d, 0.0)
+        state["w"] = w
+        for c in kids:
+            x = tok[q0 + c]
+            p = float(w[x]) if 0 <= x < V else 0.0
+            if d is None:
+                seen = any(tok[q0 + e] == x for e in kids[:kids.index(c)])
+                if 0 <= x < V and not seen and float(probs[q0 + at, x]) >= 0 and ua[q0 + c] * (1.0 - gone) < p:
+                    return c
+                if 0 <= x < V:
+                    gone += p
+                    w[x] = 0.0
+            else:
+                if 0 <= x < V and ua[q0 + c] * float(d[x]) * z < p:
+                    return c
+                w = torch.clamp(w / z - d, min=0)
+                z = float(w.sum())
+                z = z if z > 0 else 1.0
+                state["w"] = w
+        return None
+
+    def final(q0, at, kids, b):
+        w = state["w"]
+        if not float(w.sum()) > 0:
+            w = weights(q0 + at)
+        pos = torch.nonzero(w > 0)
+        if pos.numel() == 0:
+            return 0
+        cum = w.cumsum(0)
+        hit = torch.nonzero((cum > ud[b] * float(cum[-1])) & (w > 0))
+        return int(hit[0]) if hit.numel() else int(pos[-1])
+
+    return _walk(tokens, parents, q_start, max_nodes, choose, final)
+
+
+def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, q_start: torch.Tensor,
+                max_nodes: int, u_accept: torch.Tensor, u_draw: torch.Tensor,
+                draft_probs: torch.Tensor | None = None) -> TreeVerdict:
+    """Rejection-sampling verification with given random numbers (``verify_sampled`` for trees).
+
+    probs [T, V] fp32 or bf16: the request's (filtered) sampling distribution after every node;
+    u_accept fp32 [T] one uniform number in [0, 1) per node, u_draw fp32 [B] one per sequence.
+    At a node the children are tried in index order:
+
+    * ``draft_probs`` None, drafts chosen outright (a greedy drafter's likeliest tokens): child c
+      with token x is accepted when u_c (1 - r) < p(x), r the probability of the siblings
+      rejected before it; a rejected token's probability is removed.  A sibling that repeats
+      a rejected token is rejected.
+    * ``draft_probs`` [T, V] (the type of probs): the children of a node were drawn independently
+      from its row q.  With w = p and Z = 1 at first, a child is accepted when u_c q(x) Z < w(x);
+      each rejection sets w to max(0, w / Z - q) and Z to its sum.
+
+    A node whose children are all rejected (or that has none) ends the path and emits the smallest
+    token t with w(0) + .. + w(t) > u_draw * sum(w), in the weights that are left (in p when
+    nothing is left of them).  Every emitted token is then a sample of the target's
+    distribution.  NaN and negative entries weigh nothing, and a draft outside the vocabulary is
+    never accepted."""
+    T, B, dev = _tree_args(tokens, parents, q_start, max_nodes)
+    _need(probs.dim() == 2 and probs.shape[0] == T and probs.shape[1] > 0 and probs.device == dev
+          and probs.stride(1) == 1 and probs.dtype in (torch.float32, torch.bfloat16),
+          f"probs must be fp32 or bf16 [{T}, V] with contiguous rows on {dev}")
+    if draft_probs is not None:
+        _need(draft_probs.shape == probs.shape and draft_probs.dtype == probs.dtype and draft_probs.device == dev
+              and draft_probs.stride(1) == 1, "draft_probs must match probs")
+    for name, u, n in (("u_accept", u_accept, T), ("u_draw", u_draw, B)):
+        _need(u.dtype == torch.float32 and tuple(u.shape) == (n,) and u.is_contiguous() and u.device == dev,
+              f"{name} must be contiguous fp32 [{n}] on {dev}")
+    if not tokens.is_cuda:
+        return verify_tree_ref(probs, tokens, parents, q_start, max_nodes, u_accept, u_draw, draft_probs)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return verify_tree(probs, tokens, parents, q_start, max_nodes, u_accept, u_draw, draft_probs)
+    v = _verdict(B, max_nodes, dev)
+    N.call("xtu_tree_verify", probs.data_ptr(), probs.stride(0), N.ptr(draft_probs),
+           0 if draft_probs is None else draft_probs.stride(0), int(probs.dtype == torch.bfloat16), probs.shape[1],
+           tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(), B,
+           max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
+           N.status_buffer(dev).data_ptr(), N.stream_ptr(dev))
+    return v
+
+
+# ---------------------------------------------------------------------------
+# cache commit
+# ---------------------------------------------------------------------------
+def commit_tree_ref(k_caches, v_caches, path, accepted, q_start, kv_len, block_table) -> None:
+    qs, kl, acc, pth = q_start.tolist(), kv_len.tolist(), accepted.tolist(), path.tolist()
+    fp8 = k_caches[0].dtype == _FP8
+    for b in range(len(kl)):
+        n = qs[b + 1] - qs[b]
+        ctx = kl[b] - n
+        for j in range(1, min(acc[b], path.shape[1] - 1, n - 1) + 1):
+            if not j < pth[b][j] < n:
+                continue
+            f, t = ctx + pth[b][j], ctx + j
+            fb, tb = int(block_table[b, f // KV_BLOCK]), int(block_table[b, t // KV_BLOCK])
+            for k, v in zip(k_caches, v_caches):
+                if fp8:
+                    k, v = k.view(torch.uint8), v.view(torch.uint8)
+                    v[tb, :, :, t % KV_BLOCK] = v[fb, :, :, f % KV_BLOCK]
+                else:
+                    v[tb, :, t % KV_BLOCK] = v[fb, :, f % KV_BLOCK]
+                k[tb, :, t % KV_BLOCK] = k[fb, :, f % KV_BLOCK]
+
+
+def commit_tree(k_caches, v_caches, path: torch.Tensor, accepted: torch.Tensor, q_start: torch.Tensor,
+                kv_len: torch.Tensor, block_table: torch.Tensor) -> None:
+    """Move the accepted nodes' K / V behind the context, in place: of every sequence and layer slot
+    context + path[j] to slot context + j, j = 1 .. accepted (``path`` and ``accepted`` of a
+    :class:`TreeVerdict`; ``q_start``, ``kv_len``, ``block_table`` those of the step).
+
+    k_caches / v_caches: one cache per layer, of one shape (layers of other head counts take a
+    call of their own), as sequences of tensors or as one tensor with the layers in front; bf16
+    or fp8 (V transposed inside each block).  A path must rise (a parent lies below its
+    children); entries that do not, or that lie outside the tree or the cache, move nothing."""
+    L = len(k_caches)
+    _need(L == len(v_caches) and L > 0, "commit_tree takes as many K as V caches")
+    k0, v0 = k_caches[0], v_caches[0]
+    _need(k0.dim() == 4 and v0.dim() == 4, "caches are [blocks, Hkv, 64, D] per layer")
+    dev = k0.device
+    nb, Hk, bs, D = k0.shape
+    fp8 = k0.dtype == _FP8
+    Dv = v0.shape[2] if fp8 else v0.shape[3]
+    _need(tuple(v0.shape) == ((nb, Hk, Dv, bs) if fp8 else (nb, Hk, bs, Dv)) and v0.dtype == k0.dtype
+          and v0.device == dev, "K and V caches do not match")
+    _need(bs == KV_BLOCK, f"KV blocks hold {KV_BLOCK} tokens, not {bs}")
+    B, P = path.shape
+    _ints("path", path, (B, P), dev)
+    _ints("accepted", accepted, (B,), dev)
+    _ints("q_start", q_start, (B + 1,), dev)
+    _ints("kv_len", kv_len, (B,), dev)
+    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= B
+          and block_table.stride(1) == 1 and block_table.device == dev,
+          "block_table must be int32 [B, blocks] with contiguous rows")
+    stacked = isinstance(k_caches, torch.Tensor) and isinstance(v_caches, torch.Tensor)
+    for k, v in ((k0, v0),) if stacked else zip(k_caches, v_caches):
+        _need(k.shape == k0.shape and v.shape == v0.shape and k.dtype == k0.dtype and v.dtype == k0.dtype
+              and k.device == dev and v.device == dev, "the layers' caches must be alike")
+        _need(k.is_contiguous() and v.is_contiguous(), "the caches must be contiguous")
+    if not k0.is_cuda:
+        commit_tree_ref(k_caches, v_caches, path, accepted, q_start, kv_len, block_table)
+        return
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return commit_tree(k_caches, v_caches, path, accepted, q_start, kv_len, block_table)
+    es = k0.element_size()
+    _need(D * es % 16 == 0 and (fp8 or Dv * es % 16 == 0), "head rows must be multiples of 16 bytes")
+    if stacked:
+        kp = vp = None
+        kb, ks, vb, vs = k0.data_ptr(), k_caches.stride(0) * es, v0.data_ptr(), v_caches.stride(0) * es
+    else:
+        kp, vp = (N.c_longlong * L)(*[k.data_ptr() for k in k_caches]), (N.c_longlong * L)(*[v.data_ptr() for v in v_caches])
+        kb = ks = vb = vs = 0
+    _need(all(x % 16 == 0 for x in ((kb, ks, vb, vs) if stacked else (*kp, *vp))), "caches start on 16-byte boundaries")
+    N.call("xtu_tree_commit", kp, vp, kb, ks, vb, vs, L, path.data_ptr(), P, accepted.data_ptr(), q_start.data_ptr(),
+           kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], B, nb, Hk, D * es,
+           Dv * es, int(fp8), Dv, N.stream_ptr(dev))
