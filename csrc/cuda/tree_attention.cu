@@ -615,6 +615,479 @@ __global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mm
 }
 
 // ---------------------------------------------------------------------------------------
+// tensor-memory kernel: 128-row tiles
+// ---------------------------------------------------------------------------------------
+// One CTA = ROWT row tiles of 128 query rows of one (sequence, kv head, kv split, DV columns).
+// Two softmax units of 128 threads (one row each) keep the tensor core busy in turn:
+//   ROWT = 2  unit u owns row tile u; every K / V tile serves both
+//   ROWT = 1  both units own the same rows; unit u takes the key tiles t = u (mod 2) with a
+//             maximum, sum and accumulator of its own, and they merge at the end
+//   warp 0       TMA producer: key tiles of BN keys into a K ring and a V ring
+//   warp 1       MMA issuer: S_u = Q K^T into TMEM, O_u += P_u V with P_u from TMEM
+//   warps 4-7    unit 0;  warps 8-11 unit 1: S_u -> registers, mask, online softmax, P_u (16 bit)
+//                over S_u's own columns
+// The issuer alternates PV_u(t), S_u(t + 1): S_u's completion (one commit) also tells unit u that
+// PV_u(t) is done, so P and O need no barriers of their own and S and P share columns.
+template <int D, int DVT, int BN, int ROWT, int SK, int SV>
+struct TtCfg {
+  static constexpr int Q_BYTES = ROWT * 128 * D * 2;
+  static constexpr int K_BYTES = BN * D * 2, V_BYTES = BN * DVT * 2;
+  static constexpr int BARS = 2 * SK + 2 * SV + 8;
+  static constexpr int BYTES = 1024 + Q_BYTES + SK * K_BYTES + SV * V_BYTES + BARS * 8 + 64;
+  static constexpr int O_COL = 2 * BN;                 // S0 S1 | O0 O1
+  static constexpr int COLS = 2 * BN + 2 * DVT <= 256 ? 256 : 512;
+  static constexpr int MLD = DVT + 4;                  // ROWT = 1: unit 1's O in shared memory (floats)
+  static constexpr int THREADS = 384;
+  static_assert(2 * BN + 2 * DVT <= 512, "tensor memory");
+  static_assert(BYTES <= 232448, "shared memory");
+  static_assert(ROWT == 2 || 128 * MLD * 4 + 1024 <= SK * K_BYTES + SV * V_BYTES, "merge buffer");
+  static_assert(D % 64 == 0 && DVT % 64 == 0 && BN % 64 == 0 && SK >= 2 && SV >= 2, "tiles");
+};
+
+// 8 bf16 (16 bytes) at (row, col) of a K-major 128B-swizzled tile of [128 rows][64-column chunks]
+__device__ __forceinline__ void tt_st(uint8_t* tile, int row, int col, uint4 v) {
+  uint8_t* base = tile + (col >> 6) * (128 * 128) + row * 128;
+  *reinterpret_cast<uint4*>(base + ((((col & 63) >> 3) ^ (row & 7)) << 4)) = v;
+}
+
+__device__ __forceinline__ void tt_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]));
+}
+
+template <int D, int DVT, int BN, int ROWT, int SK, int SV>
+__global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tk,
+                                                              const __grid_constant__ CUtensorMap tv,
+                                                              const __grid_constant__ TaParams p, int DV) {
+  griddep_wait();
+  using C = TtCfg<D, DVT, BN, ROWT, SK, SV>;
+  constexpr int PPT = BN / TA_PAGE;                    // pages of a key tile
+  extern __shared__ uint8_t tt_smem[];
+  __shared__ int s_bad;                                // a masked tile held a non-finite value
+  const uint32_t sa = smem_u32(tt_smem);
+  uint8_t* base = tt_smem + (((sa + 1023u) & ~1023u) - sa);
+  uint8_t* sQ = base;
+  uint8_t* sK = sQ + C::Q_BYTES;
+  uint8_t* sV = sK + SK * C::K_BYTES;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(sV + SV * C::V_BYTES);
+  uint64_t* k_empty = k_full + SK;
+  uint64_t* v_full = k_empty + SK;
+  uint64_t* v_empty = v_full + SV;
+  uint64_t* q_ready = v_empty + SV;
+  uint64_t* s_full = q_ready + 1;                      // [2]
+  uint64_t* p_full = s_full + 2;                       // [2]
+  uint64_t* o_done = p_full + 2;                       // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 3);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z, halves = DV / DVT;
+  const int kh = blockIdx.y / halves, dv0 = (blockIdx.y - kh * halves) * DVT;
+  // row tiles of one split lie next to each other, so that they meet the same K / V in L2
+  const int rt = gridDim.x / p.splits;
+  const int sp = blockIdx.x / rt, tile = blockIdx.x - sp * rt;
+  const int q0 = __ldg(p.q_start + b), n = __ldg(p.q_start + b + 1) - q0;
+  const int L = __ldg(p.kv_len + b), ctx = L - n;
+  const int r0 = tile * (128 * ROWT);
+  const int rows_all = n * p.G;
+  if (r0 >= rows_all) {                                // uniform: no such row tile here
+    griddep_launch_dependents();
+    return;
+  }
+  const int npages = min((L + TA_PAGE - 1) / TA_PAGE, p.bt_cols);
+  const int ntile_all = (npages + PPT - 1) / PPT;
+  const int tfirst = p.window > 0 ? max(0, ctx - p.window + 1) / BN : 0;
+  const int per = (ntile_all - tfirst + p.splits - 1) / p.splits;
+  const int t0 = min(ntile_all, tfirst + sp * per), t1 = min(ntile_all, t0 + per);
+  const int nt = max(0, t1 - t0);
+  // tiles at or past `shut` or below `open` hide keys from some rows (see the masked pages above)
+  const int shut = ctx / BN;
+  const int open = p.window > 0 ? (max(0, ctx + n - p.window) + BN - 1) / BN : 0;
+  const bool two = ROWT == 2 ? r0 + 128 < rows_all : nt > 1;   // unit 1 has work
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+    s_bad = 0;
+    for (int i = 0; i < SK; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < SV; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
+    mbar_init(q_ready, 4 * ROWT);
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, C::COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // dependents may start only now: one that took this SM's tensor memory first, and waits for
+  // this grid, would never give it back
+  griddep_launch_dependents();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (elect_one() && nt > 0) {
+      const int* bt = p.block_table + (size_t)b * p.bt_stride;
+      // rows of the pages of tile t (the caches' zero fill where there is no page)
+      auto row_of = [&](int t, int sb) {
+        const int lp = (t0 + t) * PPT + sb;
+        int pg = lp < npages ? __ldg(bt + lp) : p.num_blocks;
+        if (lp < npages) (void)XTU_IN_BOUNDS(pg >= 0 && pg < p.num_blocks, p.status, 244, pg);
+        if (pg < 0 || pg > p.num_blocks) pg = p.num_blocks;
+        return (pg * p.Hkv + kh) * TA_PAGE;
+      };
+      int krow[PPT], vrow[PPT];
+#pragma unroll
+      for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(0, sb);
+      int kn = 0, vn = 0;
+      bool ok = true;
+      auto load_k = [&](int t) {
+        const int st = t % SK;
+        if (t >= SK && !mbar_wait(&k_empty[st], ((t / SK) - 1) & 1, p.status, 150)) return false;
+        mbar_arrive_expect_tx(&k_full[st], C::K_BYTES);
+#pragma unroll
+        for (int sb = 0; sb < PPT; ++sb)
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_2d(sK + st * C::K_BYTES + c * (BN * 128) + sb * (TA_PAGE * 128), &tk, &k_full[st], c * 64, krow[sb]);
+        ++kn;
+        return true;
+      };
+      auto load_v = [&](int t) {
+        const int st = t % SV;
+        if (t >= SV && !mbar_wait(&v_empty[st], ((t / SV) - 1) & 1, p.status, 151)) return false;
+        mbar_arrive_expect_tx(&v_full[st], C::V_BYTES);
+#pragma unroll
+        for (int sb = 0; sb < PPT; ++sb)
+#pragma unroll
+          for (int c = 0; c < DVT / 64; ++c)
+            tma_load_2d(sV + st * C::V_BYTES + c * (BN * 128) + sb * (TA_PAGE * 128), &tv, &v_full[st], dv0 + c * 64,
+                        vrow[sb]);
+        ++vn;
+        return true;
+      };
+      ok = load_k(0);
+      for (int t = 0; t < nt && ok; ++t) {
+#pragma unroll
+        for (int sb = 0; sb < PPT; ++sb) vrow[sb] = krow[sb];
+        if (t + 1 < nt) {
+#pragma unroll
+          for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(t + 1, sb);
+          ok = load_k(t + 1);
+        }
+        ok = ok && load_v(t);
+      }
+      if (!ok) {   // let the copies in flight land (bounded) before the CTA ends
+        for (int t = max(0, kn - SK); t < kn; ++t) mbar_wait(&k_full[t % SK], (t / SK) & 1, nullptr, 0, 50000000ull);
+        for (int t = max(0, vn - SV); t < vn; ++t) mbar_wait(&v_full[t % SV], (t / SV) & 1, nullptr, 0, 50000000ull);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one() && nt > 0) {
+      constexpr uint32_t id_s = idesc_bf16_f32(128, BN, 0, 0), id_o = idesc_bf16_f32(128, DVT, 0, 1);
+      bool ok = mbar_wait(q_ready, 0, p.status, 152);
+      tc_fence_after();
+      auto mma_s = [&](int u, int t) {
+        const uint32_t qa = smem_u32(sQ) + (ROWT == 2 ? u * (128 * D * 2) : 0);
+        const uint32_t ka = smem_u32(sK + (t % SK) * C::K_BYTES);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_f16_ss(tmem + u * BN, sdesc_kmajor_sw128(qa + (k >> 2) * (128 * 128) + (k & 3) * 32),
+                     sdesc_kmajor_sw128(ka + (k >> 2) * (BN * 128) + (k & 3) * 32), id_s, k > 0);
+        mma_commit(&s_full[u]);
+      };
+      auto mma_o = [&](int u, int t, bool first) {
+        const uint32_t va = smem_u32(sV + (t % SV) * C::V_BYTES);
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)
+          mma_f16_ts(tmem + C::O_COL + u * DVT, tmem + u * BN + k * 8,
+                     sdesc_mnmajor_sw128(va + k * 16 * 128, BN * 128, 1024), id_o, !(first && k == 0));
+      };
+      auto wait_k = [&](int t) { return mbar_wait(&k_full[t % SK], (t / SK) & 1, p.status, 153); };
+      auto wait_v = [&](int t) { return mbar_wait(&v_full[t % SV], (t / SV) & 1, p.status, 154); };
+      // a slot that no later tile takes is not given back: nothing arrives behind the CTA's end
+      auto free_k = [&](int t) { if (t + SK < nt) mma_commit(&k_empty[t % SK]); };
+      auto free_v = [&](int t) { if (t + SV < nt) mma_commit(&v_empty[t % SV]); };
+      if (ROWT == 2) {
+        ok = ok && wait_k(0);
+        if (ok) {
+          tc_fence_after();
+          mma_s(0, 0);
+          if (two) mma_s(1, 0);
+          free_k(0);
+        }
+        for (int t = 0; t < nt && ok; ++t) {
+          for (int u = 0; u < (two ? 2 : 1); ++u) {
+            ok = (u > 0 || wait_v(t)) && mbar_wait(&p_full[u], t & 1, p.status, 155);
+            if (!ok) break;
+            tc_fence_after();
+            mma_o(u, t, t == 0);
+            if (t + 1 < nt) {
+              if (u == 0) {
+                ok = wait_k(t + 1);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              mma_s(u, t + 1);
+            } else {
+              mma_commit(&o_done[u]);
+            }
+          }
+          free_v(t);
+          if (t + 1 < nt) free_k(t + 1);
+        }
+      } else {
+        for (int t = 0; t < min(nt, 2) && ok; ++t) {
+          ok = wait_k(t);
+          if (!ok) break;
+          tc_fence_after();
+          mma_s(t, t);
+          free_k(t);
+        }
+        for (int t = 0; t < nt && ok; ++t) {
+          const int u = t & 1;
+          ok = wait_v(t) && mbar_wait(&p_full[u], (t >> 1) & 1, p.status, 155);
+          if (!ok) break;
+          tc_fence_after();
+          mma_o(u, t, t < 2);
+          free_v(t);
+          if (t + 2 < nt) {
+            ok = wait_k(t + 2);
+            if (!ok) break;
+            tc_fence_after();
+            mma_s(u, t + 2);
+            free_k(t + 2);
+          } else {
+            mma_commit(&o_done[u]);
+          }
+        }
+      }
+      if (!ok) {   // the MMAs in flight end before the CTA gives its tensor memory back
+        uint64_t* drained = o_done + 2;
+        mbar_init(drained, 1);
+        fence_barrier_init();
+        mma_commit(drained);
+        mbar_wait(drained, 0, nullptr, 0, 50000000ull);
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax units
+    const int u = (warp - 4) >> 2, qd = warp & 3;
+    const int r = qd * 32 + lane;                      // row of the tile = TMEM lane
+    const int rr = r0 + (ROWT == 2 ? u * 128 : 0) + r;
+    const bool valid = rr < rows_all;
+    const int node = valid ? rr / p.G : 0, hh = valid ? rr - node * p.G : 0;
+    const int tok = q0 + node, head = kh * p.G + hh;
+    if (ROWT == 2 || u == 0) {
+      const __nv_bfloat16* src = p.q + (long long)tok * p.q_ts + (long long)head * p.q_hs;
+      uint8_t* dst = sQ + (ROWT == 2 ? u * (128 * D * 2) : 0);
+#pragma unroll 8
+      for (int c = 0; c < D; c += 8)
+        tt_st(dst, r, c, valid ? __ldg(reinterpret_cast<const uint4*>(src + c)) : make_uint4(0u, 0u, 0u, 0u));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+    }
+    const TaRow row = ta_row(p, q0, n, ctx, node, valid);
+    const uint32_t lanes = (uint32_t)(qd * 32) << 16;
+    const uint32_t s_t = tmem + lanes + u * BN, o_t = tmem + lanes + C::O_COL + u * DVT;
+    float m = -FLT_MAX, l = 0.f;                       // running maximum (log2 units) and sum
+    bool ok = true;
+    const int mine = ROWT == 2 ? ((u == 0 || two) ? nt : 0) : (nt - u + 1) / 2;   // this unit's tiles
+    for (int i = 0; i < mine && ok; ++i) {
+      const int t = ROWT == 2 ? i : 2 * i + u;
+      const int at = t0 + t;                           // key tile
+      const bool msk = at >= shut || at < open;
+      if (msk) {
+        // V's non-finite values become zero (0 * p must stay 0 for keys that a row does not
+        // see) and join the rows that do see them at the end
+        ok = mbar_wait(&v_full[t % SV], (t / SV) & 1, p.status, 156);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint4* vw = reinterpret_cast<uint4*>(sV + (t % SV) * C::V_BYTES);
+        for (int w = r; w < C::V_BYTES / 16; w += 128) {
+          uint4 x = vw[w];
+          const uint4 bad = make_uint4(bad_bf16x2(x.x), bad_bf16x2(x.y), bad_bf16x2(x.z), bad_bf16x2(x.w));
+          if (bad.x | bad.y | bad.z | bad.w) {
+            s_bad = 1;
+            __threadfence_block();                     // the flag before the zeros: the other unit may find only those
+            vw[w] = make_uint4(x.x & ~bad.x, x.y & ~bad.y, x.z & ~bad.z, x.w & ~bad.w);
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      ok = mbar_wait(&s_full[u], i & 1, p.status, 157);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t sv[BN];
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) tmem_ld32p(s_t + c * 32, sv + c * 32);
+      tmem_wait_ld();
+      if (msk) {
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          const uint32_t see = ta_see32(p, row, q0, at * BN + c * 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((see >> e) & 1u)) sv[c * 32 + e] = 0xFF800000u;   // -inf
+        }
+      }
+      float mx4[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};
+#pragma unroll
+      for (int e = 0; e < BN; e += 2)
+        mx4[(e >> 1) & 3] = fmax3(mx4[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+      float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      if (mx != -FLT_MAX) mx *= p.scale_log2;
+      // the maximum moves only when it grows by more than 2^8: P stays below 2^8, O is rarely rescaled
+      const bool raise = mx > m + 8.f;
+      const float m_new = raise ? mx : m;
+      const bool rescale = raise && m != -FLT_MAX && i > 0;
+      if (__any_sync(0xffffffffu, rescale)) {
+        const float f = rescale ? ta_ex2(m - m_new) : 1.f;
+        l *= f;
+#pragma unroll 1
+        for (int c = 0; c < DVT; c += 16) {
+          uint32_t x[16];
+          tmem_ld16(o_t + c, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+          tmem_st16(o_t + c, x);
+        }
+      }
+      m = m_new;
+      const float neg = m == -FLT_MAX ? 0.f : -m;
+      float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < BN / 64; ++c) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          const float a = ta_ex2(fmaf(__uint_as_float(sv[c * 64 + e]), p.scale_log2, neg));
+          const float d = ta_ex2(fmaf(__uint_as_float(sv[c * 64 + e + 1]), p.scale_log2, neg));
+          l4[(e >> 1) & 3] += a + d;
+          pk[e >> 1] = pack_bf16x2(a, d);              // P: bf16 (half a step of 2^-8); l keeps the 32-bit sum
+        }
+        tt_st32(s_t + c * 32, pk);
+      }
+      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[u]);
+    }
+    // ---- end: O / l
+    bool have = mine > 0 && ok;
+    if (have) {
+      have = mbar_wait(&o_done[u], 0, p.status, 158);
+      have = __all_sync(0xffffffffu, have);
+      tc_fence_after();
+    }
+    float M = m, scale_own = 1.f;
+    float* oth = nullptr;
+    if (ROWT == 1) {
+      // unit 1's rows meet unit 0's in shared memory (both units' MMAs and copies are done)
+      float* mo = reinterpret_cast<float*>(sK);                       // [128][MLD]
+      float* ml = mo + 128 * C::MLD;                                  // [128][2]
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (u == 1) {
+        ml[2 * r] = have ? m : -FLT_MAX;
+        ml[2 * r + 1] = have ? l : 0.f;
+        if (have) {
+#pragma unroll 1
+          for (int c = 0; c < DVT; c += 32) {
+            uint32_t x[32];
+            tmem_ld32(o_t + c, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(mo + r * C::MLD + c + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+          }
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (u == 0 && two) {
+        const float m1 = ml[2 * r], l1 = ml[2 * r + 1];
+        M = fmaxf(m, m1);
+        scale_own = m == -FLT_MAX ? (l != l ? l : 0.f) : ta_ex2(m - M);
+        const float f1 = m1 == -FLT_MAX ? (l1 != l1 ? l1 : 0.f) : ta_ex2(m1 - M);
+        l = l * scale_own + l1 * f1;
+        oth = mo + r * C::MLD;
+        ml[2 * r] = f1;
+      }
+    }
+    if (ROWT == 2 ? (u == 0 || two) : u == 0) {
+      if (p.sinks != nullptr && p.splits == 1 && M != -FLT_MAX && valid) l += ta_ex2(__ldg(p.sinks + head) * LOG2E - M);
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const float f1 = oth != nullptr ? reinterpret_cast<float*>(sK)[128 * C::MLD + 2 * r] : 0.f;
+      const bool bad = s_bad != 0;
+      const size_t at = ((size_t)tok * p.Hq + head) * DV + dv0;
+#pragma unroll 1
+      for (int c = 0; c < DVT; c += 32) {
+        uint32_t x[32];
+        if (have) {
+          tmem_ld32(o_t + c, x);
+          tmem_wait_ld();
+        }
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = have ? __uint_as_float(x[e]) * scale_own : 0.f;
+        if (oth != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] += oth[c + e] * f1;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] *= inv;
+        if (bad && valid) {   // rare: non-finite values of masked tiles, for the rows that see them
+          for (int tl = t0; tl < t1; ++tl) {
+            if (tl < shut && tl >= open) continue;
+            for (int k2 = 0; k2 < BN; ++k2) {
+              const int key = tl * BN + k2;
+              if (key / TA_PAGE >= npages || !ta_sees(p, row, q0, key)) continue;
+              const int page = __ldg(p.block_table + (size_t)b * p.bt_stride + key / TA_PAGE);
+              if (page < 0 || page >= p.num_blocks) continue;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float y = ta_v_at(p, false, DV, page, kh, key % TA_PAGE, dv0 + c + e);
+                if (!isfinite(y)) v[e] += y;
+              }
+            }
+          }
+        }
+        if (!valid) continue;
+        if (p.splits == 1) {
+          uint4* d4 = reinterpret_cast<uint4*>(p.o + at + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            d4[e] = make_uint4(pack_bf16x2(v[8 * e], v[8 * e + 1]), pack_bf16x2(v[8 * e + 2], v[8 * e + 3]),
+                               pack_bf16x2(v[8 * e + 4], v[8 * e + 5]), pack_bf16x2(v[8 * e + 6], v[8 * e + 7]));
+        } else {
+          float4* d4 = reinterpret_cast<float4*>(p.ws_o + (size_t)sp * p.T * p.Hq * DV + at + c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d4[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+        }
+      }
+      if (p.splits > 1 && valid && dv0 == 0)
+        p.ws_lse[((size_t)sp * p.T + tok) * p.Hq + head] =
+            l > 0.f || l != l ? (M == -FLT_MAX ? 0.f : M) + __log2f(l) : -FLT_MAX;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::COLS);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
 // the splits' normalised partials by their log-sum-exp: one warp per (token, head)
 // ---------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) tree_attn_merge_kernel(const float* __restrict__ ws_o,
@@ -728,6 +1201,26 @@ int tm_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int
   return tm_launch<D, DV, F8, 4>(tk, tv, p, (rows + 63) / 64, B, s);
 }
 
+template <int D, int DVT, int BN, int ROWT, int SK, int SV>
+int tt_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int tiles, int DV, int B,
+              cudaStream_t s) {
+  using C = TtCfg<D, DVT, BN, ROWT, SK, SV>;
+  static bool done[64] = {};
+  const auto kern = tree_attn_tc_kernel<D, DVT, BN, ROWT, SK, SV>;
+  if (const int rc = ta_allow(kern, C::BYTES, done)) return rc;
+  const cudaError_t e = launch_pdl(kern, dim3(tiles * p.splits, p.Hkv * (DV / DVT), B), dim3(C::THREADS), C::BYTES, s,
+                                   tk, tv, p, DV);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? 1 : -(int)e;
+}
+
+// rows: of the largest tree; one row tile, or two that share their K / V tiles
+template <int D, int DVT, int BN1, int SK1, int SV1, int BN2, int SK2, int SV2>
+int tt_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int DV, int B, cudaStream_t s) {
+  if (rows <= 128) return tt_launch<D, DVT, BN1, 1, SK1, SV1>(tk, tv, p, 1, DV, B, s);
+  return tt_launch<D, DVT, BN2, 2, SK2, SV2>(tk, tv, p, (rows + 255) / 256, DV, B, s);
+}
+
 }  // namespace
 }  // namespace xtu
 
@@ -795,10 +1288,10 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   if (fp8 && D == 64 && DV == 64) r = tm_rows<64, 64, true>(tk, tv, p, rows, B, s);
   else if (fp8 && D == 128 && DV == 128) r = tm_rows<128, 128, true>(tk, tv, p, rows, B, s);
   else if (fp8) return -6;
-  else if (D == 64 && DV == 64) r = tm_rows<64, 64, false>(tk, tv, p, rows, B, s);
-  else if (D == 128 && DV == 128) r = tm_rows<128, 128, false>(tk, tv, p, rows, B, s);
-  else if (D == 192 && DV == 128) r = tm_rows<192, 128, false>(tk, tv, p, rows, B, s);
-  else if (D == 256 && DV == 256) r = tm_rows<256, 256, false>(tk, tv, p, rows, B, s);
+  else if (D == 64 && DV == 64) r = tt_rows<64, 64, 128, 6, 6, 128, 5, 5>(tk, tv, p, rows, DV, B, s);
+  else if (D == 128 && DV == 128) r = tt_rows<128, 128, 128, 3, 3, 128, 3, 2>(tk, tv, p, rows, DV, B, s);
+  else if (D == 192 && DV == 128) r = tt_rows<192, 128, 64, 4, 4, 64, 3, 3>(tk, tv, p, rows, DV, B, s);
+  else if (D == 256 && DV == 256) r = tt_rows<256, 128, 64, 3, 3, 64, 2, 2>(tk, tv, p, rows, DV, B, s);
   if (r < 0 || splits == 1) return r;
   const int heads = T * Hq;
   const cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((heads + 7) / 8), dim3(256), 0, s,

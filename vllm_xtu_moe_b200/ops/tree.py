@@ -166,10 +166,13 @@ def tree_attention_ref(q, k_cache, v_cache, meta: TreeMetadata, scale: float, ou
     return out
 
 
-def tree_splits(num_seqs: int, num_kv_heads: int, rows: int, seen: int, num_sms: int = 148) -> int:
-    """KV splits of a step: as many CTAs (row tiles of 64 x KV heads x sequences x splits, one per
-    SM) as one wave holds, each with 4 pages of keys or more."""
-    ctas = max(1, -(-rows // 64) * num_kv_heads * num_seqs)
+def tree_splits(num_seqs: int, num_kv_heads: int, rows: int, seen: int, fp8: bool = False, dv: int = 128,
+                num_sms: int = 148) -> int:
+    """KV splits of a step: as many CTAs (row tiles x KV heads x sequences x splits, one per SM) as
+    one wave holds, each with 4 pages of keys or more.  ``rows``: query rows of the largest tree
+    per KV head, ``seen``: keys that a sequence attends to."""
+    tiles = -(-rows // 64) if fp8 else 1 if rows <= 128 else -(-rows // 256)
+    ctas = max(1, tiles * num_kv_heads * num_seqs * (2 if dv == 256 else 1))
     pages = -(-seen // KV_BLOCK)
     return max(1, min(num_sms // ctas, pages // 4, MAX_SPLITS))
 
@@ -220,6 +223,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
               f"sinks must be fp32 [{Hq}]")
     if scale is None:
         scale = 1.0 / math.sqrt(D)
+    _need(scale > 0 and k_scale > 0, "scales must be positive")
     if out is None:
         out = torch.empty(T, Hq, Dv, dtype=q.dtype, device=dev)
     _need(tuple(out.shape) == (T, Hq, Dv) and out.dtype == q.dtype and out.is_contiguous() and out.device == dev,
@@ -239,7 +243,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
           "q rows must be contiguous and start on 16-byte boundaries")
     rows = meta.max_nodes * (Hq // Hk)
     seen = min(meta.max_kv_len, window + meta.max_nodes + KV_BLOCK) if window > 0 else meta.max_kv_len
-    splits = meta.num_splits if meta.num_splits > 0 else tree_splits(B, Hk, rows, seen)
+    splits = meta.num_splits if meta.num_splits > 0 else tree_splits(B, Hk, rows, seen, fp8, Dv)
     _need(splits <= MAX_SPLITS, f"at most {MAX_SPLITS} splits")
     ws = None
     if splits > 1:
