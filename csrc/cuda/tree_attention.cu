@@ -42,6 +42,7 @@ struct TaParams {
   const int* depth;         // [T] (window > 0 only)
   int window;
   int Hq, Hkv, G, T;
+  uint32_t g_inv;           // ceil(2^32 / G): x / G for x < 2^25 (G = 1: unused)
   float scale_log2;         // softmax scale * log2(e) (fp8: times the K scale)
   float out_scale;          // fp8: the V scale, else 1
   const float* sinks;       // [Hq] or null
@@ -53,10 +54,30 @@ struct TaParams {
   XtuStatus* status;
 };
 
+// query row -> node
+__device__ __forceinline__ int ta_node(const TaParams& p, int row) {
+  return p.G == 1 ? row : (int)__umulhi((uint32_t)row, p.g_inv);
+}
+
 __device__ __forceinline__ float ta_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __noinline__ bool ta_wait_on(uint64_t* bar, uint32_t parity, XtuStatus* st, uint32_t where,
+                                        uint64_t limit_ns) {
+  return mbar_wait(bar, parity, st, where, limit_ns);
+}
+
+// mbar_wait behind a few tries of its own: it reads the global timer after one failed try, and
+// the read (hundreds of cycles) sat on the critical path of waits that were over sooner
+__device__ __forceinline__ bool ta_wait(uint64_t* bar, uint32_t parity, XtuStatus* st, uint32_t where,
+                                        uint64_t limit_ns = kIntraCtaWaitNs) {
+#pragma unroll 1
+  for (int it = 0; it < 64; ++it)
+    if (mbar_try_wait(bar, parity)) return true;
+  return ta_wait_on(bar, parity, st, where, limit_ns);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -85,7 +106,8 @@ __device__ __forceinline__ TaRow ta_row(const TaParams& p, int q0, int n, int ct
 }
 
 // bits of keys key0 .. key0 + 31 that the row sees
-__device__ __forceinline__ uint32_t ta_see32(const TaParams& p, const TaRow& r, int q0, int key0) {
+// (not inlined: rare, and code that is never run costs fetches of the code that is)
+__device__ __noinline__ uint32_t ta_see32(const TaParams& p, const TaRow& r, int q0, int key0) {
   if (r.words == nullptr) return 0u;
   const int off = key0 - r.ctx;              // node index of key0
   uint32_t bits = 0u;
@@ -125,6 +147,25 @@ __device__ __forceinline__ float ta_v_at(const TaParams& p, bool f8, int DV, int
     return __half2float(__half(h));
   }
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p.v_raw)[(((size_t)page * p.Hkv + kh) * TA_PAGE + off) * DV + d]);
+}
+
+// a row's output (32-bit partial or bf16 result, columns d0 .. d0 + cols - 1 of V) plus the non-finite
+// values of the keys of logical page pg that it sees
+__device__ __noinline__ void ta_add_bad(const TaParams& p, const TaRow& r, int q0, int b, int kh, int pg, int DV,
+                                        int d0, int cols, float* wo, __nv_bfloat16* o) {
+  const int page = __ldg(p.block_table + (size_t)b * p.bt_stride + pg);
+  if (page < 0 || page >= p.num_blocks) return;
+#pragma unroll 1
+  for (int k = 0; k < TA_PAGE; ++k) {
+    if (!ta_sees(p, r, q0, pg * TA_PAGE + k)) continue;
+#pragma unroll 1
+    for (int d = 0; d < cols; ++d) {
+      const float y = ta_v_at(p, false, DV, page, kh, k, d0 + d);
+      if (isfinite(y)) continue;
+      if (wo != nullptr) wo[d] += y;
+      else o[d] = __float2bfloat16(__bfloat162float(o[d]) + y);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -297,7 +338,7 @@ __global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mm
         if (lane == 0) (void)XTU_IN_BOUNDS(pg >= 0 && pg < p.num_blocks, p.status, 243, pg);
         if (lane == 0) {
           const int i = c0 + k, slot = i % STAGES;
-          if (i >= STAGES && !mbar_wait(&empty[slot], ((i / STAGES) - 1) & 1, p.status, 140)) {
+          if (i >= STAGES && !ta_wait(&empty[slot], ((i / STAGES) - 1) & 1, p.status, 140)) {
             ok = false;
           } else {
             ++issued;
@@ -323,7 +364,7 @@ __global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mm
     }
     if (!ok && lane == 0) {   // let the copies in flight land (bounded) before the CTA exits
       for (int j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j)
-        mbar_wait(&full[j % STAGES], (j / STAGES) & 1, nullptr, 0, 50000000ull);
+        ta_wait(&full[j % STAGES], (j / STAGES) & 1, nullptr, 0, 50000000ull);
     }
     return;
   }
@@ -337,7 +378,7 @@ __global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mm
   for (int h2 = 0; h2 < 2; ++h2) {
     const int r = mt * 16 + g4 + h2 * 8;
     const bool valid = r < nrows;
-    const int node = valid ? (r0 + r) / p.G : 0, hh = valid ? (r0 + r) - node * p.G : 0;
+    const int node = valid ? ta_node(p, r0 + r) : 0, hh = valid ? (r0 + r) - node * p.G : 0;
     row[h2] = ta_row(p, q0, n, ctx, node, valid);
     const __nv_bfloat16* qrow = p.q + (long long)(q0 + node) * p.q_ts + (long long)(kh * p.G + hh) * p.q_hs;
     if constexpr (F8) {
@@ -363,7 +404,7 @@ __global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mm
       const int r = i / (D / 8), c = (i - r * (D / 8)) * 8;
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (r < nrows) {
-        const int node = (r0 + r) / p.G, hh = (r0 + r) - node * p.G;
+        const int node = ta_node(p, r0 + r), hh = (r0 + r) - node * p.G;
         v = __ldg(reinterpret_cast<const uint4*>(p.q + (long long)(q0 + node) * p.q_ts +
                                                  (long long)(kh * p.G + hh) * p.q_hs + c));
       }
@@ -380,7 +421,7 @@ __global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mm
   bool ok = true;
   for (int i = 0; i < nj; ++i) {
     const int slot = i % STAGES;
-    if (ok && !mbar_wait(&full[slot], (i / STAGES) & 1, p.status, 141)) ok = false;
+    if (ok && !ta_wait(&full[slot], (i / STAGES) & 1, p.status, 141)) ok = false;
     const bool msk = masked(j0 + i);
     const uint32_t kb = smem_u32(ring + slot * C::STAGE), vb = kb + C::K_BYTES;
     if (msk) {
@@ -578,7 +619,7 @@ __global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mm
       acc[2] += wgt * v.z;
       acc[3] += wgt * v.w;
     }
-    const int node = (r0 + r) / p.G, hh = (r0 + r) - node * p.G;
+    const int node = ta_node(p, r0 + r), hh = (r0 + r) - node * p.G;
     const int tok = q0 + node, head = kh * p.G + hh;
     // the sink joins the denominator only (once: here, or in the merge of the splits)
     if (p.sinks != nullptr && p.splits == 1 && M != -INFINITY) Ls += ta_ex2(__ldg(p.sinks + head) * LOG2E - M);
@@ -618,72 +659,90 @@ __global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mm
 // tensor-memory kernel: 128-row tiles
 // ---------------------------------------------------------------------------------------
 // One CTA = ROWT row tiles of 128 query rows of one (sequence, kv head, kv split, DV columns).
-// Two softmax units of 128 threads (one row each) keep the tensor core busy in turn:
+// Two softmax units of 128 threads keep the tensor core busy in turn:
 //   ROWT = 2  unit u owns row tile u; every K / V tile serves both
 //   ROWT = 1  both units own the same rows; unit u takes the key tiles t = u (mod 2) with a
 //             maximum, sum and accumulator of its own, and they merge at the end
 //   warp 0       TMA producer: key tiles of BN keys into a K ring and a V ring
-//   warp 1       MMA issuer: S_u = Q K^T into TMEM, O_u += P_u V with P_u from TMEM
+//   warp 1       MMA issuer: S_u = Q K^T into TMEM, O_u += P_u V with P_u from TMEM, the units in turn
+//   warp 2       gives the ring's slots back
 //   warps 4-7    unit 0;  warps 8-11 unit 1: S_u -> registers, mask, online softmax, P_u (16 bit)
-//                over S_u's own columns
+//                over S_u's own columns, a thread a row
 // The issuer alternates PV_u(t), S_u(t + 1): S_u's completion (one commit) also tells unit u that
 // PV_u(t) is done, so P and O need no barriers of their own and S and P share columns.
-template <int D, int DVT, int BN, int ROWT, int SK, int SV>
+template <int D_, int DVT_, int BN_, int ROWT_, int SK, int SV>
 struct TtCfg {
+  static constexpr int D = D_, DVT = DVT_, BN = BN_, ROWT = ROWT_;
   static constexpr int Q_BYTES = ROWT * 128 * D * 2;
   static constexpr int K_BYTES = BN * D * 2, V_BYTES = BN * DVT * 2;
-  static constexpr int BARS = 2 * SK + 2 * SV + 8;
-  static constexpr int BYTES = 1024 + Q_BYTES + SK * K_BYTES + SV * V_BYTES + BARS * 8 + 64;
+  // one ring of SK + SV slots where a K and a V tile are the same size (K0 V0 K1 V1 ..: an odd count
+  // halves no lookahead), else a ring each
+  static constexpr bool ONE = K_BYTES == V_BYTES;
+  static constexpr int NS = SK + SV, RING = SK * K_BYTES + SV * V_BYTES;
+  __device__ static int k_slot(int t) { return ONE ? 2 * t % NS : t % SK; }
+  __device__ static int v_slot(int t) { return ONE ? (2 * t + 1) % NS : SK + t % SV; }
+  __device__ static int k_turn(int t) { return ONE ? 2 * t / NS : t / SK; }          // how often the slot was filled before
+  __device__ static int v_turn(int t) { return ONE ? (2 * t + 1) / NS : t / SV; }
+  __device__ static int slot_at(int s) { return ONE || s < SK ? s * K_BYTES : SK * K_BYTES + (s - SK) * V_BYTES; }
+  // tile t's K (V) slot is filled again before the last of nt tiles
+  __device__ static bool k_again(int t, int nt) { return ONE ? 2 * t + NS < 2 * nt : t + SK < nt; }
+  __device__ static bool v_again(int t, int nt) { return ONE ? 2 * t + 1 + NS < 2 * nt : t + SV < nt; }
+  static constexpr int BARS = 2 * NS + 10;
+  static constexpr int BYTES = Q_BYTES + RING + BARS * 8 + 16;
   static constexpr int O_COL = 2 * BN;                 // S0 S1 | O0 O1
   static constexpr int COLS = 2 * BN + 2 * DVT <= 256 ? 256 : 512;
   static constexpr int MLD = DVT + 4;                  // ROWT = 1: unit 1's O in shared memory (floats)
-  static constexpr int THREADS = 384;
+    static constexpr int THREADS = 384;
   static_assert(2 * BN + 2 * DVT <= 512, "tensor memory");
+  // V(t)'s slot is given back once S of the tile AHEAD of it stands, whose K the producer must have loaded
+  // before it comes to wait for that slot
+  static constexpr int AHEAD = ROWT == 2 ? 1 : 2;
+  static_assert(AHEAD <= (ONE ? NS / 2 : SV), "the ring would wait for itself");
   static_assert(BYTES <= 232448, "shared memory");
-  static_assert(ROWT == 2 || 128 * MLD * 4 + 1024 <= SK * K_BYTES + SV * V_BYTES, "merge buffer");
+  static_assert(ROWT == 2 || 128 * MLD * 4 + 1024 <= RING, "merge buffer");
   static_assert(D % 64 == 0 && DVT % 64 == 0 && BN % 64 == 0 && SK >= 2 && SV >= 2, "tiles");
 };
 
-// 8 bf16 (16 bytes) at (row, col) of a K-major 128B-swizzled tile of [128 rows][64-column chunks]
-__device__ __forceinline__ void tt_st(uint8_t* tile, int row, int col, uint4 v) {
-  uint8_t* base = tile + (col >> 6) * (128 * 128) + row * 128;
-  *reinterpret_cast<uint4*>(base + ((((col & 63) >> 3) ^ (row & 7)) << 4)) = v;
+// 16 bytes to shared memory without a register stop; zeros when `there` is false
+__device__ __forceinline__ void tt_copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-__device__ __forceinline__ void tt_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]));
+// pairs of floats in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
-
-template <int D, int DVT, int BN, int ROWT, int SK, int SV>
-__global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tk,
-                                                              const __grid_constant__ CUtensorMap tv,
-                                                              const __grid_constant__ TaParams p, int DV) {
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tk,
+                                                                     const __grid_constant__ CUtensorMap tv,
+                                                                     const __grid_constant__ TaParams p, int DV) {
   griddep_wait();
-  using C = TtCfg<D, DVT, BN, ROWT, SK, SV>;
+  constexpr int D = C::D, DVT = C::DVT, BN = C::BN, ROWT = C::ROWT;
   constexpr int PPT = BN / TA_PAGE;                    // pages of a key tile
-  extern __shared__ uint8_t tt_smem[];
-  __shared__ int s_bad;                                // a masked tile held a non-finite value
-  const uint32_t sa = smem_u32(tt_smem);
-  uint8_t* base = tt_smem + (((sa + 1023u) & ~1023u) - sa);
-  uint8_t* sQ = base;
-  uint8_t* sK = sQ + C::Q_BYTES;
-  uint8_t* sV = sK + SK * C::K_BYTES;
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(sV + SV * C::V_BYTES);
-  uint64_t* k_empty = k_full + SK;
-  uint64_t* v_full = k_empty + SK;
-  uint64_t* v_empty = v_full + SV;
-  uint64_t* q_ready = v_empty + SV;
+  extern __shared__ __align__(1024) uint8_t tt_smem[];   // (the swizzle atoms' alignment)
+  uint8_t* sQ = tt_smem;
+  uint8_t* sK = sQ + C::Q_BYTES;                       // the ring
+  uint64_t* full = reinterpret_cast<uint64_t*>(sK + C::RING);
+  uint64_t* empty = full + C::NS;
+  uint64_t* q_ready = empty + C::NS;
   uint64_t* s_full = q_ready + 1;                      // [2]
-  uint64_t* p_full = s_full + 2;                       // [2]
-  uint64_t* o_done = p_full + 2;                       // [2]
+  uint64_t* p_full = s_full + 2;                       // [2][2] halves of P
+  uint64_t* o_done = p_full + 4;                       // [2], and one for an issuer that gives up
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 3);
+  int& s_bad = *reinterpret_cast<int*>(tmem_slot + 1);   // a masked tile held a non-finite value
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, halves = DV / DVT;
@@ -714,10 +773,10 @@ __global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_const
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
     s_bad = 0;
-    for (int i = 0; i < SK; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
-    for (int i = 0; i < SV; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
-    mbar_init(q_ready, 4 * ROWT);
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+    for (int i = 0; i < C::NS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    mbar_init(q_ready, 8);
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&o_done[i], 1); }
+    for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc(tmem_slot, C::COLS);
@@ -745,127 +804,88 @@ __global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_const
 #pragma unroll
       for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(0, sb);
       int kn = 0, vn = 0;
+      auto load = [&](int slot, int turn, int bytes, const CUtensorMap* map, int c0, int cols, const int (&rows)[PPT],
+                      int site) {
+        if (turn > 0 && !ta_wait(&empty[slot], (turn - 1) & 1, p.status, site)) return false;
+        mbar_arrive_expect_tx(&full[slot], bytes);
+        uint8_t* dst = sK + C::slot_at(slot);
+#pragma unroll
+        for (int sb = 0; sb < PPT; ++sb)
+#pragma unroll
+          for (int c = 0; c < cols / 64; ++c)
+            tma_load_2d(dst + c * (BN * 128) + sb * (TA_PAGE * 128), map, &full[slot], c0 + c * 64, rows[sb]);
+        return true;
+      };
       bool ok = true;
-      auto load_k = [&](int t) {
-        const int st = t % SK;
-        if (t >= SK && !mbar_wait(&k_empty[st], ((t / SK) - 1) & 1, p.status, 150)) return false;
-        mbar_arrive_expect_tx(&k_full[st], C::K_BYTES);
-#pragma unroll
-        for (int sb = 0; sb < PPT; ++sb)
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_2d(sK + st * C::K_BYTES + c * (BN * 128) + sb * (TA_PAGE * 128), &tk, &k_full[st], c * 64, krow[sb]);
-        ++kn;
-        return true;
-      };
-      auto load_v = [&](int t) {
-        const int st = t % SV;
-        if (t >= SV && !mbar_wait(&v_empty[st], ((t / SV) - 1) & 1, p.status, 151)) return false;
-        mbar_arrive_expect_tx(&v_full[st], C::V_BYTES);
-#pragma unroll
-        for (int sb = 0; sb < PPT; ++sb)
-#pragma unroll
-          for (int c = 0; c < DVT / 64; ++c)
-            tma_load_2d(sV + st * C::V_BYTES + c * (BN * 128) + sb * (TA_PAGE * 128), &tv, &v_full[st], dv0 + c * 64,
-                        vrow[sb]);
-        ++vn;
-        return true;
-      };
-      ok = load_k(0);
       for (int t = 0; t < nt && ok; ++t) {
+        ok = load(C::k_slot(t), C::k_turn(t), C::K_BYTES, &tk, 0, D, krow, 150);
+        kn += ok;
 #pragma unroll
         for (int sb = 0; sb < PPT; ++sb) vrow[sb] = krow[sb];
         if (t + 1 < nt) {
 #pragma unroll
-          for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(t + 1, sb);
-          ok = load_k(t + 1);
+          for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(t + 1, sb);   // under way while V's slot gets free
         }
-        ok = ok && load_v(t);
+        ok = ok && load(C::v_slot(t), C::v_turn(t), C::V_BYTES, &tv, dv0, DVT, vrow, 151);
+        vn += ok;
       }
       if (!ok) {   // let the copies in flight land (bounded) before the CTA ends
-        for (int t = max(0, kn - SK); t < kn; ++t) mbar_wait(&k_full[t % SK], (t / SK) & 1, nullptr, 0, 50000000ull);
-        for (int t = max(0, vn - SV); t < vn; ++t) mbar_wait(&v_full[t % SV], (t / SV) & 1, nullptr, 0, 50000000ull);
+        for (int t = max(0, kn - C::NS); t < kn; ++t) ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, nullptr, 0, 50000000ull);
+        for (int t = max(0, vn - C::NS); t < vn; ++t) ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, nullptr, 0, 50000000ull);
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (elect_one() && nt > 0) {
       constexpr uint32_t id_s = idesc_bf16_f32(128, BN, 0, 0), id_o = idesc_bf16_f32(128, DVT, 0, 1);
-      bool ok = mbar_wait(q_ready, 0, p.status, 152);
-      tc_fence_after();
-      auto mma_s = [&](int u, int t) {
-        const uint32_t qa = smem_u32(sQ) + (ROWT == 2 ? u * (128 * D * 2) : 0);
-        const uint32_t ka = smem_u32(sK + (t % SK) * C::K_BYTES);
+      bool ok = ta_wait(q_ready, 0, p.status, 152);
+      auto tile_of = [&](int u, int i) { return ROWT == 2 ? i : 2 * i + u; };   // unit u's i-th tile
+      auto wait_k = [&](int t) { return ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, p.status, 153); };
+      auto wait_v = [&](int t) { return ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, p.status, 154); };
+      // S_u = Q_u K^T of the unit's i-th tile
+      auto mma_s = [&](int u, int i) {
+        const uint64_t qd = sdesc_kmajor_sw128(smem_u32(sQ) + (ROWT == 2 ? u * (128 * D * 2) : 0));
+        const uint64_t kd = sdesc_kmajor_sw128(smem_u32(sK + C::slot_at(C::k_slot(tile_of(u, i)))));
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_f16_ss(tmem + u * BN, sdesc_kmajor_sw128(qa + (k >> 2) * (128 * 128) + (k & 3) * 32),
-                     sdesc_kmajor_sw128(ka + (k >> 2) * (BN * 128) + (k & 3) * 32), id_s, k > 0);
+        for (int k = 0; k < D / 16; ++k)   // (descriptors count 16 bytes)
+          mma_f16_ss(tmem + u * BN, qd + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16,
+                     kd + ((k >> 2) * (BN * 128) + (k & 3) * 32) / 16, id_s, k > 0);
         mma_commit(&s_full[u]);
       };
-      auto mma_o = [&](int u, int t, bool first) {
-        const uint32_t va = smem_u32(sV + (t % SV) * C::V_BYTES);
+      // O_u += P_u V of its i-th tile, the two halves of the keys as P_u gets ready
+      auto mma_o = [&](int u, int i) {
+        const uint64_t vd = sdesc_mnmajor_sw128(smem_u32(sK + C::slot_at(C::v_slot(tile_of(u, i)))), BN * 128, 1024);
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          mma_f16_ts(tmem + C::O_COL + u * DVT, tmem + u * BN + k * 8,
-                     sdesc_mnmajor_sw128(va + k * 16 * 128, BN * 128, 1024), id_o, !(first && k == 0));
+        for (int h = 0; h < 2; ++h) {
+          if (!ta_wait(&p_full[2 * u + h], i & 1, p.status, 155)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int k = h * (BN / 32); k < (h + 1) * (BN / 32); ++k)
+            mma_f16_ts(tmem + C::O_COL + u * DVT, tmem + u * BN + k * 8, vd + k * 128, id_o, !(i == 0 && k == 0));
+        }
+        return true;
       };
-      auto wait_k = [&](int t) { return mbar_wait(&k_full[t % SK], (t / SK) & 1, p.status, 153); };
-      auto wait_v = [&](int t) { return mbar_wait(&v_full[t % SV], (t / SV) & 1, p.status, 154); };
-      // a slot that no later tile takes is not given back: nothing arrives behind the CTA's end
-      auto free_k = [&](int t) { if (t + SK < nt) mma_commit(&k_empty[t % SK]); };
-      auto free_v = [&](int t) { if (t + SV < nt) mma_commit(&v_empty[t % SV]); };
-      if (ROWT == 2) {
-        ok = ok && wait_k(0);
-        if (ok) {
-          tc_fence_after();
-          mma_s(0, 0);
-          if (two) mma_s(1, 0);
-          free_k(0);
-        }
-        for (int t = 0; t < nt && ok; ++t) {
-          for (int u = 0; u < (two ? 2 : 1); ++u) {
-            ok = (u > 0 || wait_v(t)) && mbar_wait(&p_full[u], t & 1, p.status, 155);
-            if (!ok) break;
-            tc_fence_after();
-            mma_o(u, t, t == 0);
-            if (t + 1 < nt) {
-              if (u == 0) {
-                ok = wait_k(t + 1);
-                if (!ok) break;
-                tc_fence_after();
-              }
-              mma_s(u, t + 1);
-            } else {
-              mma_commit(&o_done[u]);
-            }
-          }
-          free_v(t);
-          if (t + 1 < nt) free_k(t + 1);
-        }
-      } else {
-        for (int t = 0; t < min(nt, 2) && ok; ++t) {
-          ok = wait_k(t);
+      // the units in turn: PV of the unit's i-th tile, then S of its next
+      const int n0 = ROWT == 2 ? nt : (nt + 1) / 2, n1 = !two ? 0 : ROWT == 2 ? nt : nt / 2;   // the units' tiles
+      for (int u = 0; u < 2 && ok; ++u) {
+        if (u == 1 && n1 == 0) break;
+        ok = (ROWT == 2 && u == 1) || wait_k(tile_of(u, 0));
+        tc_fence_after();
+        if (ok) mma_s(u, 0);
+      }
+      // (a wait costs the issuer 100 cycles or more even when it is over, and the issuer's way from P to the
+      // next S is on every unit's path: the waits for K and V come before P's, and once for both
+      // units where they share the tiles)
+      for (int i = 0; i < n0 && ok; ++i) {
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+          const int nu = u == 0 ? n0 : n1;
+          if (i >= nu) continue;
+          if (ROWT == 1 || u == 0) ok = wait_v(tile_of(u, i)) && (i + 1 >= nu || wait_k(tile_of(u, i + 1)));
+          ok = ok && mma_o(u, i);
           if (!ok) break;
-          tc_fence_after();
-          mma_s(t, t);
-          free_k(t);
-        }
-        for (int t = 0; t < nt && ok; ++t) {
-          const int u = t & 1;
-          ok = wait_v(t) && mbar_wait(&p_full[u], (t >> 1) & 1, p.status, 155);
-          if (!ok) break;
-          tc_fence_after();
-          mma_o(u, t, t < 2);
-          free_v(t);
-          if (t + 2 < nt) {
-            ok = wait_k(t + 2);
-            if (!ok) break;
-            tc_fence_after();
-            mma_s(u, t + 2);
-            free_k(t + 2);
-          } else {
-            mma_commit(&o_done[u]);
-          }
+          if (i + 1 < nu) mma_s(u, i + 1);
+          else mma_commit(&o_done[u]);
         }
       }
       if (!ok) {   // the MMAs in flight end before the CTA gives its tensor memory back
@@ -873,7 +893,25 @@ __global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_const
         mbar_init(drained, 1);
         fence_barrier_init();
         mma_commit(drained);
-        mbar_wait(drained, 0, nullptr, 0, 50000000ull);
+        ta_wait(drained, 0, nullptr, 0, 50000000ull);
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ slots back to the producer
+    // A unit's S of a tile stands (s_full): K of that tile is done with, and V of the tile whose PV the
+    // issuer put before it.  With two units on the same tiles the one that is served last
+    // speaks for both.  (Commits of the issuer would do, but a third one under way stops it until
+    // the products are done; a softmax thread's arrivals cost its warp 350 cycles a tile.)
+    if (elect_one()) {
+      constexpr int ahead = C::AHEAD;
+      bool ok = true;
+      for (int t = 0; t < nt && ok; ++t) {
+        const int u = ROWT == 2 ? (two ? 1 : 0) : t & 1;
+        if (!C::k_again(t, nt) && !(t >= ahead && C::v_again(t - ahead, nt))) continue;
+        ok = ta_wait(&s_full[u], (ROWT == 2 ? t : t >> 1) & 1, p.status, 159);
+        if (!ok) break;
+        if (C::k_again(t, nt)) mbar_arrive(&empty[C::k_slot(t)]);
+        if (t >= ahead && C::v_again(t - ahead, nt)) mbar_arrive(&empty[C::v_slot(t - ahead)]);
       }
     }
   } else if (warp >= 4) {
@@ -882,37 +920,48 @@ __global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_const
     const int r = qd * 32 + lane;                      // row of the tile = TMEM lane
     const int rr = r0 + (ROWT == 2 ? u * 128 : 0) + r;
     const bool valid = rr < rows_all;
-    const int node = valid ? rr / p.G : 0, hh = valid ? rr - node * p.G : 0;
+    const int node = valid ? ta_node(p, rr) : 0, hh = valid ? rr - node * p.G : 0;
     const int tok = q0 + node, head = kh * p.G + hh;
-    if (ROWT == 2 || u == 0) {
-      const __nv_bfloat16* src = p.q + (long long)tok * p.q_ts + (long long)head * p.q_hs;
+    {
+      // Q, whole rows at a time: D / 8 lanes a row (a thread a row touched 32 lines a load: 5 us).
+      // 128B-swizzled K-major chunks of [128 rows][64 columns]
+      constexpr int PR = D / 8, TH = ROWT == 2 ? 128 : 256;     // pieces of a row, threads of this tile
       uint8_t* dst = sQ + (ROWT == 2 ? u * (128 * D * 2) : 0);
-#pragma unroll 8
-      for (int c = 0; c < D; c += 8)
-        tt_st(dst, r, c, valid ? __ldg(reinterpret_cast<const uint4*>(src + c)) : make_uint4(0u, 0u, 0u, 0u));
+      const int base = r0 + (ROWT == 2 ? u * 128 : 0);
+#pragma unroll 4
+      for (int i = ROWT == 2 ? r : u * 128 + r; i < 128 * PR; i += TH) {
+        const int row = i / PR, pc = i - row * PR, gr = base + row;
+        const bool there = gr < rows_all;
+        const int nd = there ? ta_node(p, gr) : 0;
+        const int hd = there ? gr - nd * p.G : 0;
+        tt_copy16(smem_u32(dst + (pc >> 3) * (128 * 128) + row * 128 + (((pc & 7) ^ (row & 7)) << 4)),
+                  p.q + (long long)(q0 + nd) * p.q_ts + (long long)(kh * p.G + hd) * p.q_hs + pc * 8, there);
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
     }
-    const TaRow row = ta_row(p, q0, n, ctx, node, valid);
     const uint32_t lanes = (uint32_t)(qd * 32) << 16;
     const uint32_t s_t = tmem + lanes + u * BN, o_t = tmem + lanes + C::O_COL + u * DVT;
     float m = -FLT_MAX, l = 0.f;                       // running maximum (log2 units) and sum
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     const int mine = ROWT == 2 ? ((u == 0 || two) ? nt : 0) : (nt - u + 1) / 2;   // this unit's tiles
-    for (int i = 0; i < mine && ok; ++i) {
+    for (int i = 0; i < mine; ++i) {
       const int t = ROWT == 2 ? i : 2 * i + u;
       const int at = t0 + t;                           // key tile
       const bool msk = at >= shut || at < open;
       if (msk) {
         // V's non-finite values become zero (0 * p must stay 0 for keys that a row does not
         // see) and join the rows that do see them at the end
-        ok = mbar_wait(&v_full[t % SV], (t / SV) & 1, p.status, 156);
+        ok = ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, p.status, 156);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint4* vw = reinterpret_cast<uint4*>(sV + (t % SV) * C::V_BYTES);
+        uint4* vw = reinterpret_cast<uint4*>(sK + C::slot_at(C::v_slot(t)));
+#pragma unroll 2
         for (int w = r; w < C::V_BYTES / 16; w += 128) {
-          uint4 x = vw[w];
+          const uint4 x = vw[w];
           const uint4 bad = make_uint4(bad_bf16x2(x.x), bad_bf16x2(x.y), bad_bf16x2(x.z), bad_bf16x2(x.w));
           if (bad.x | bad.y | bad.z | bad.w) {
             s_bad = 1;
@@ -922,21 +971,22 @@ __global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_const
         }
         fence_proxy_async_smem();
       }
-      ok = mbar_wait(&s_full[u], i & 1, p.status, 157);
+      ok = ta_wait(&s_full[u], i & 1, p.status, 157);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       uint32_t sv[BN];
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c) tmem_ld32p(s_t + c * 32, sv + c * 32);
+      for (int c = 0; c < BN; c += 32) tmem_ld32p(s_t + c, sv + c);
       tmem_wait_ld();
       if (msk) {
+        const TaRow row = ta_row(p, q0, n, ctx, node, valid);
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-          const uint32_t see = ta_see32(p, row, q0, at * BN + c * 32);
+        for (int c = 0; c < BN; c += 32) {
+          const uint32_t see = ta_see32(p, row, q0, at * BN + c);
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (!((see >> e) & 1u)) sv[c * 32 + e] = 0xFF800000u;   // -inf
+            if (!((see >> e) & 1u)) sv[c + e] = 0xFF800000u;   // -inf
         }
       }
       float mx4[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};
@@ -964,42 +1014,45 @@ __global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_const
       }
       m = m_new;
       const float neg = m == -FLT_MAX ? 0.f : -m;
-      float l4[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 ng2 = make_float2(neg, neg);
+      float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < BN / 64; ++c) {
-        uint32_t pk[32];
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 64; e += 2) {
-          const float a = ta_ex2(fmaf(__uint_as_float(sv[c * 64 + e]), p.scale_log2, neg));
-          const float d = ta_ex2(fmaf(__uint_as_float(sv[c * 64 + e + 1]), p.scale_log2, neg));
-          l4[(e >> 1) & 3] += a + d;
-          pk[e >> 1] = pack_bf16x2(a, d);              // P: bf16 (half a step of 2^-8); l keeps the 32-bit sum
+        for (int e = 0; e < 32; e += 2) {
+          const float2 x = fma2(make_float2(__uint_as_float(sv[c + e]), __uint_as_float(sv[c + e + 1])), sc2, ng2);
+          const float2 y = make_float2(ta_ex2(x.x), ta_ex2(x.y));
+          l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], y);
+          pk[e >> 1] = pack_bf16x2(y.x, y.y);          // P: bf16 (half a step of 2^-8); l keeps the 32-bit sum
         }
-        tt_st32(s_t + c * 32, pk);
+        tmem_st16(s_t + c / 2, pk);
+        if ((c + 32) % (BN / 2) == 0) {                // half of P is ready: its product may start
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * u + c / (BN / 2)]);
+        }
       }
-      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[u]);
+      l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
     }
     // ---- end: O / l
     bool have = mine > 0 && ok;
     if (have) {
-      have = mbar_wait(&o_done[u], 0, p.status, 158);
+      have = ta_wait(&o_done[u], 0, p.status, 158);
       have = __all_sync(0xffffffffu, have);
       tc_fence_after();
     }
-    float M = m, scale_own = 1.f;
-    float* oth = nullptr;
+    float M = m, scale_own = 1.f, f1 = 0.f;
+    const float* oth = nullptr;
     if (ROWT == 1) {
-      // unit 1's rows meet unit 0's in shared memory (both units' MMAs and copies are done)
+      // unit 1's rows meet unit 0's in shared memory: with both units done the ring is free
       float* mo = reinterpret_cast<float*>(sK);                       // [128][MLD]
-      float* ml = mo + 128 * C::MLD;                                  // [128][2]
+      float* ml = mo + 128 * C::MLD;                                  // [2][128]
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (u == 1) {
-        ml[2 * r] = have ? m : -FLT_MAX;
-        ml[2 * r + 1] = have ? l : 0.f;
+        ml[r] = have ? m : -FLT_MAX;
+        ml[128 + r] = have ? l : 0.f;
         if (have) {
 #pragma unroll 1
           for (int c = 0; c < DVT; c += 32) {
@@ -1014,21 +1067,20 @@ __global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_const
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (u == 0 && two) {
-        const float m1 = ml[2 * r], l1 = ml[2 * r + 1];
+        const float m1 = ml[r], l1 = ml[128 + r];
         M = fmaxf(m, m1);
         scale_own = m == -FLT_MAX ? (l != l ? l : 0.f) : ta_ex2(m - M);
-        const float f1 = m1 == -FLT_MAX ? (l1 != l1 ? l1 : 0.f) : ta_ex2(m1 - M);
+        f1 = m1 == -FLT_MAX ? (l1 != l1 ? l1 : 0.f) : ta_ex2(m1 - M);
         l = l * scale_own + l1 * f1;
         oth = mo + r * C::MLD;
-        ml[2 * r] = f1;
       }
     }
     if (ROWT == 2 ? (u == 0 || two) : u == 0) {
       if (p.sinks != nullptr && p.splits == 1 && M != -FLT_MAX && valid) l += ta_ex2(__ldg(p.sinks + head) * LOG2E - M);
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-      const float f1 = oth != nullptr ? reinterpret_cast<float*>(sK)[128 * C::MLD + 2 * r] : 0.f;
-      const bool bad = s_bad != 0;
       const size_t at = ((size_t)tok * p.Hq + head) * DV + dv0;
+      float* wo = p.splits > 1 ? p.ws_o + (size_t)sp * p.T * p.Hq * DV + at : nullptr;
+      const float sc0 = scale_own * inv, sc1 = f1 * inv;
 #pragma unroll 1
       for (int c = 0; c < DVT; c += 32) {
         uint32_t x[32];
@@ -1036,47 +1088,41 @@ __global__ void __launch_bounds__(384, 1) tree_attn_tc_kernel(const __grid_const
           tmem_ld32(o_t + c, x);
           tmem_wait_ld();
         }
+        if (!valid) continue;
         float v[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = have ? __uint_as_float(x[e]) * scale_own : 0.f;
+        for (int e = 0; e < 32; ++e) v[e] = have ? __uint_as_float(x[e]) * sc0 : 0.f;
         if (oth != nullptr) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] += oth[c + e] * f1;
-        }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] *= inv;
-        if (bad && valid) {   // rare: non-finite values of masked tiles, for the rows that see them
-          for (int tl = t0; tl < t1; ++tl) {
-            if (tl < shut && tl >= open) continue;
-            for (int k2 = 0; k2 < BN; ++k2) {
-              const int key = tl * BN + k2;
-              if (key / TA_PAGE >= npages || !ta_sees(p, row, q0, key)) continue;
-              const int page = __ldg(p.block_table + (size_t)b * p.bt_stride + key / TA_PAGE);
-              if (page < 0 || page >= p.num_blocks) continue;
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float y = ta_v_at(p, false, DV, page, kh, key % TA_PAGE, dv0 + c + e);
-                if (!isfinite(y)) v[e] += y;
-              }
-            }
+          for (int e = 0; e < 32; e += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(oth + c + e);
+            v[e] += y.x * sc1;
+            v[e + 1] += y.y * sc1;
+            v[e + 2] += y.z * sc1;
+            v[e + 3] += y.w * sc1;
           }
         }
-        if (!valid) continue;
-        if (p.splits == 1) {
+        if (wo == nullptr) {
           uint4* d4 = reinterpret_cast<uint4*>(p.o + at + c);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             d4[e] = make_uint4(pack_bf16x2(v[8 * e], v[8 * e + 1]), pack_bf16x2(v[8 * e + 2], v[8 * e + 3]),
                                pack_bf16x2(v[8 * e + 4], v[8 * e + 5]), pack_bf16x2(v[8 * e + 6], v[8 * e + 7]));
         } else {
-          float4* d4 = reinterpret_cast<float4*>(p.ws_o + (size_t)sp * p.T * p.Hq * DV + at + c);
+          float4* d4 = reinterpret_cast<float4*>(wo + c);
 #pragma unroll
           for (int e = 0; e < 8; ++e) d4[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
         }
       }
-      if (p.splits > 1 && valid && dv0 == 0)
+      if (wo != nullptr && valid && dv0 == 0)
         p.ws_lse[((size_t)sp * p.T + tok) * p.Hq + head] =
             l > 0.f || l != l ? (M == -FLT_MAX ? 0.f : M) + __log2f(l) : -FLT_MAX;
+      if (s_bad && valid) {   // rare: non-finite values of masked tiles, for the rows that see them
+        const TaRow row = ta_row(p, q0, n, ctx, node, valid);
+        for (int pg = t0 * PPT; pg < min(t1 * PPT, npages); ++pg)
+          if (pg / PPT >= shut || pg / PPT < open)
+            ta_add_bad(p, row, q0, b, kh, pg, DV, dv0, DVT, wo, wo == nullptr ? p.o + at : nullptr);
+      }
     }
   }
   tc_fence_before();
@@ -1118,15 +1164,26 @@ __global__ void __launch_bounds__(256) tree_attn_merge_kernel(const float* __res
   for (int d0 = 0; d0 < DV; d0 += 128) {
     const int d = d0 + lane * 4;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, s < 32 ? wa : wc, s & 31);
-      const float ls = __shfl_sync(0xffffffffu, s < 32 ? a : c, s & 31);
-      if (ls == -FLT_MAX || d >= DV) continue;   // empty: nothing was written
-      const float4 v = __ldg(reinterpret_cast<const float4*>(ws_o + ((size_t)s * rows + w) * DV + d));
-      acc[0] += ws * v.x;
-      acc[1] += ws * v.y;
-      acc[2] += ws * v.z;
-      acc[3] += ws * v.w;
+    for (int s0 = 0; s0 < splits; s0 += 4) {   // four splits' loads under way at a time
+      float4 v[4];
+      float ws[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int s = s0 + k;
+        const float ls = __shfl_sync(0xffffffffu, s < 32 ? a : c, s & 31);
+        ws[k] = __shfl_sync(0xffffffffu, s < 32 ? wa : wc, s & 31);
+        const bool there = s < splits && ls != -FLT_MAX && d < DV;   // (an empty split wrote nothing)
+        v[k] = there ? __ldg(reinterpret_cast<const float4*>(ws_o + ((size_t)s * rows + w) * DV + d))
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!there) ws[k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        acc[0] += ws[k] * v[k].x;
+        acc[1] += ws[k] * v[k].y;
+        acc[2] += ws[k] * v[k].z;
+        acc[3] += ws[k] * v[k].w;
+      }
     }
     if (d >= DV) continue;
     uint2 pk;
@@ -1201,24 +1258,22 @@ int tm_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int
   return tm_launch<D, DV, F8, 4>(tk, tv, p, (rows + 63) / 64, B, s);
 }
 
-template <int D, int DVT, int BN, int ROWT, int SK, int SV>
+template <class C>
 int tt_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int tiles, int DV, int B,
               cudaStream_t s) {
-  using C = TtCfg<D, DVT, BN, ROWT, SK, SV>;
   static bool done[64] = {};
-  const auto kern = tree_attn_tc_kernel<D, DVT, BN, ROWT, SK, SV>;
-  if (const int rc = ta_allow(kern, C::BYTES, done)) return rc;
-  const cudaError_t e = launch_pdl(kern, dim3(tiles * p.splits, p.Hkv * (DV / DVT), B), dim3(C::THREADS), C::BYTES, s,
-                                   tk, tv, p, DV);
+  if (const int rc = ta_allow(tree_attn_tc_kernel<C>, C::BYTES, done)) return rc;
+  const cudaError_t e = launch_pdl(tree_attn_tc_kernel<C>, dim3(tiles * p.splits, p.Hkv * (DV / C::DVT), B),
+                                   dim3(C::THREADS), C::BYTES, s, tk, tv, p, DV);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? 1 : -(int)e;
 }
 
 // rows: of the largest tree; one row tile, or two that share their K / V tiles
-template <int D, int DVT, int BN1, int SK1, int SV1, int BN2, int SK2, int SV2>
+template <class ONE, class TWO>
 int tt_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int DV, int B, cudaStream_t s) {
-  if (rows <= 128) return tt_launch<D, DVT, BN1, 1, SK1, SV1>(tk, tv, p, 1, DV, B, s);
-  return tt_launch<D, DVT, BN2, 2, SK2, SV2>(tk, tv, p, (rows + 255) / 256, DV, B, s);
+  if (rows <= 128) return tt_launch<ONE>(tk, tv, p, 1, DV, B, s);
+  return tt_launch<TWO>(tk, tv, p, (rows + 255) / 256, DV, B, s);
 }
 
 }  // namespace
@@ -1258,6 +1313,7 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   p.Hkv = Hkv;
   p.G = Hq / Hkv;
   p.T = T;
+  p.g_inv = p.G > 1 ? (uint32_t)(((1ull << 32) + p.G - 1) / p.G) : 0u;
   p.scale_log2 = scale * LOG2E * (fp8 ? k_scale : 1.f);
   p.out_scale = fp8 ? v_scale : 1.f;
   p.sinks = sinks;
@@ -1288,10 +1344,14 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   if (fp8 && D == 64 && DV == 64) r = tm_rows<64, 64, true>(tk, tv, p, rows, B, s);
   else if (fp8 && D == 128 && DV == 128) r = tm_rows<128, 128, true>(tk, tv, p, rows, B, s);
   else if (fp8) return -6;
-  else if (D == 64 && DV == 64) r = tt_rows<64, 64, 128, 6, 6, 128, 5, 5>(tk, tv, p, rows, DV, B, s);
-  else if (D == 128 && DV == 128) r = tt_rows<128, 128, 128, 3, 3, 128, 3, 2>(tk, tv, p, rows, DV, B, s);
-  else if (D == 192 && DV == 128) r = tt_rows<192, 128, 64, 4, 4, 64, 3, 3>(tk, tv, p, rows, DV, B, s);
-  else if (D == 256 && DV == 256) r = tt_rows<256, 128, 64, 3, 3, 64, 2, 2>(tk, tv, p, rows, DV, B, s);
+  else if (D == 64 && DV == 64)
+    r = tt_rows<TtCfg<64, 64, 128, 1, 6, 6>, TtCfg<64, 64, 128, 2, 5, 5>>(tk, tv, p, rows, DV, B, s);
+  else if (D == 128 && DV == 128)
+    r = tt_rows<TtCfg<128, 128, 128, 1, 3, 3>, TtCfg<128, 128, 128, 2, 3, 2>>(tk, tv, p, rows, DV, B, s);
+  else if (D == 192 && DV == 128)
+    r = tt_rows<TtCfg<192, 128, 64, 1, 4, 4>, TtCfg<192, 128, 64, 2, 3, 3>>(tk, tv, p, rows, DV, B, s);
+  else if (D == 256 && DV == 256)
+    r = tt_rows<TtCfg<256, 128, 64, 1, 3, 4>, TtCfg<256, 128, 64, 2, 2, 2>>(tk, tv, p, rows, DV, B, s);
   if (r < 0 || splits == 1) return r;
   const int heads = T * Hq;
   const cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((heads + 7) / 8), dim3(256), 0, s,
