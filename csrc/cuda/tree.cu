@@ -8,6 +8,7 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <climits>
 #include <cstdint>
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -154,8 +155,16 @@ struct TvCmd {
   double target; // draw: target less the slices before the owner's
 };
 
-constexpr int TV_THREADS = 512;
-constexpr int TV_WARPS = TV_THREADS / 32;
+// Drawn children: a pass for every rejection, so 1024 threads whose registers hold their slices of p and
+// q (20 weights each: a vocabulary of 163840 over 8 CTAs) from pass to pass; measured (32
+// sequences of 26 nodes, V = 151552): 512 threads that read them again 72 us, 1024 that read
+// again 64.  Drafts chosen outright: one pass, 512 threads start sooner (18.4 us against 20.5).
+template <bool DRAFT>
+struct TvCfg {
+  static constexpr int THREADS = DRAFT ? 1024 : 512, WARPS = THREADS / 32;
+  static constexpr int HELD = DRAFT ? 20 : 16;   // weights of a thread in flight (bf16: whole 16-byte loads of them)
+};
+constexpr int TV_MAX_WARPS = 32;
 constexpr int TV_MAX_C = 8;
 
 __device__ __forceinline__ float tv_load1(const float* p) { return __ldg(p); }
@@ -172,51 +181,98 @@ __device__ __forceinline__ void tv_loadv(const __nv_bfloat16* p, float (&v)[8]) 
   v[4] = bf16_lo(x.z); v[5] = bf16_hi(x.z); v[6] = bf16_lo(x.w); v[7] = bf16_hi(x.w);
 }
 
-template <typename E>
 struct TvShared {
   int par[TREE_MAX_NODES];
   int tok[TREE_MAX_NODES];
   float u[TREE_MAX_NODES], pt[TREE_MAX_NODES], qt[TREE_MAX_NODES];
   int rejected[TREE_MAX_NODES];       // tokens of the rejected children of the current node
-  double z[TREE_MAX_NODES];           // z[r]: sum of the weights after r rejections (z[0] = 1)
+  double zi[TREE_MAX_NODES];          // zi[r]: 1 / (sum of the weights after r rejections)
   double slice[TV_MAX_C];             // rank 0: the CTAs' sums
-  double warp_sum[TV_WARPS];
+  double warp_sum[TV_MAX_WARPS];
+  int found, best;                    // the draw: the first weight past the target, the last positive one
   TvCmd cmd;
 };
 
 // weight of an element after `rej` rejections (drawn children), from its p and q
-__device__ __forceinline__ double tv_weight(float p, float q, const double* z, int rej) {
+__device__ __forceinline__ double tv_weight(float p, float q, const double* zi, int rej) {
   double w = p > 0.f ? (double)p : 0.0;      // NaN and negative entries weigh nothing
+  if (rej == 0) return w;
   const double qd = q > 0.f ? (double)q : 0.0;
-  for (int r = 0; r < rej; ++r) {
-    const double x = (r == 0 ? w : w / z[r]) - qd;
-    w = x > 0.0 ? x : 0.0;
-  }
+  w = fmax(w - qd, 0.0);
+  for (int r = 1; r < rej; ++r) w = fmax(w * zi[r] - qd, 0.0);
   return w;
 }
 
+// One warp's view of a row: `weights(i, w)` gives the VE weights from element i on (0 past the row).
+// 16-byte loads where the rows allow them; where they do not (an odd vocabulary or stride) element
+// loads of the same elements by the same lane: the order of the sums does not depend on it.
 template <typename E, bool DRAFT>
-__global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
+struct TvRow {
+  static constexpr int VE = 16 / sizeof(E);
+  const E* p;
+  const E* q;          // draft row (DRAFT and rej > 0)
+  int hi, vec, rej;
+  const double* zi;
+  const int* rejected;
+
+  __device__ __forceinline__ void load(int i, float (&x)[VE], float (&y)[VE]) const {
+    if (vec && i < hi) {
+      tv_loadv(p + i, x);
+      if (DRAFT && rej > 0) tv_loadv(q + i, y);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        x[e] = i + e < hi ? tv_load1(p + i + e) : 0.f;
+        if (DRAFT && rej > 0) y[e] = i + e < hi ? tv_load1(q + i + e) : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void weigh(int i, const float (&x)[VE], const float (&y)[VE], double (&w)[VE]) const {
+    unsigned gone = 0;                       // point mass: rejected tokens among these
+    for (int r = 0; !DRAFT && r < rej; ++r) {
+      const unsigned d = (unsigned)(rejected[r] - i);
+      if (d < (unsigned)VE) gone |= 1u << d;
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      w[e] = DRAFT ? tv_weight(x[e], y[e], zi, rej) : x[e] > 0.f && !((gone >> e) & 1u) ? (double)x[e] : 0.0;
+  }
+};
+
+__device__ __forceinline__ double tv_warp_sum(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+template <typename E, bool DRAFT>
+__global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
     const E* __restrict__ probs, long long ldp, const E* __restrict__ draft, long long ldq, int V, int vec,
     const int* __restrict__ tokens, const int* __restrict__ parents, const int* __restrict__ q_start,
     const float* __restrict__ u_accept, const float* __restrict__ u_draw, int P, int* __restrict__ accepted,
     int* __restrict__ path, int* __restrict__ out, int* __restrict__ last_row, XtuStatus* st) {
   griddep_wait();
   griddep_launch_dependents();
-  __shared__ TvShared<E> s;
+  __shared__ TvShared s;
   cg::cluster_group cl = cg::this_cluster();
   const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int VE = 16 / sizeof(E);
+  constexpr int VE = 16 / sizeof(E), TV_THREADS = TvCfg<DRAFT>::THREADS, TV_WARPS = TvCfg<DRAFT>::WARPS;
   // this warp's slice of the vocabulary: whole 32 x VE steps
   const int step = 32 * VE;
+  constexpr int TV_BATCH = (TvCfg<DRAFT>::HELD + VE - 1) / VE;   // 16-byte loads of a lane under way at a time
   const int per = (((V + C * TV_WARPS - 1) / (C * TV_WARPS)) + step - 1) / step * step;
+  const bool whole = per <= TV_BATCH * step;                     // the slice is one batch: it stays
+  float x[TV_BATCH][VE], y[TV_BATCH][VE];
+  int held = -1;                                                 // row whose slice x (and y, when held_q) holds
+  bool held_q = false;
   const long long first = (long long)(rank * TV_WARPS + warp) * per;
   const int lo = (int)(first < V ? first : V), hi = (int)(first + per < V ? first + per : V);
 
   int n = 0, q0 = 0;
   int cur = 0, from = 1, a = 0, rej = 0;     // rank 0, warp 0: the walk
   double gone = 0.0;                         // point mass: probability of the rejected tokens
+  double z = 1.0;                            // drawn children: sum of the weights at hand
   bool plain = false;                        // nothing was left: draw from p itself
   int* pb = path + (size_t)b * P;
   int* ob = out + (size_t)b * P;
@@ -244,7 +300,8 @@ __global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
         if (have_sum) {                       // the sum that was asked for
           double tot = 0.0;
           for (int r = 0; r < C; ++r) tot += s.slice[r];
-          s.z[rej] = tot > 0.0 ? tot : 1.0;
+          if (lane == 0) s.zi[rej] = tot > 0.0 ? 1.0 / tot : 1.0;
+          z = tot > 0.0 ? tot : 1.0;
           __syncwarp();
           c.op = -1;
         }
@@ -257,10 +314,9 @@ __global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
           const int x = s.tok[next];
           bool take;
           if (DRAFT) {
-            double w = tv_weight(s.pt[next], s.qt[next], s.z, rej);
+            const double w = tv_weight(s.pt[next], s.qt[next], s.zi, rej);
             const double q = s.qt[next] > 0.f ? (double)s.qt[next] : 0.0;
-            const double z = rej > 0 ? s.z[rej] : 1.0;
-            take = s.pt[next] >= 0.f && (double)s.u[next] * q * z < w;
+            take = s.pt[next] >= 0.f && (double)s.u[next] * q * (rej > 0 ? z : 1.0) < w;
           } else {
             bool dup = false;
             for (int r = lane; r < rej; r += 32) dup |= s.rejected[r] == x;
@@ -326,7 +382,7 @@ __global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
         for (int r = 1; r < C; ++r)
           for (int i = lane; i < c.rej; i += 32) {
             if (DRAFT) {
-              cl.map_shared_rank(s.z, r)[i] = s.z[i];
+              cl.map_shared_rank(s.zi, r)[i] = s.zi[i];
             } else {
               cl.map_shared_rank(s.rejected, r)[i] = s.rejected[i];
             }
@@ -335,33 +391,34 @@ __global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
     cl.sync();
     const TvCmd c = s.cmd;
     if (c.op == 2) break;
-    const E* pr = probs + (long long)c.row * ldp;
-    const E* qr = DRAFT ? draft + (long long)c.row * ldq : nullptr;
-    auto weight = [&](int i, float p, float q) -> double {
-      if constexpr (DRAFT) {
-        return tv_weight(p, q, s.z, c.rej);
-      } else {
-        for (int r = 0; r < c.rej; ++r)
-          if (s.rejected[r] == i) return 0.0;
-        return p > 0.f ? (double)p : 0.0;
-      }
-    };
+    TvRow<E, DRAFT> row;
+    row.p = probs + (long long)c.row * ldp;
+    row.q = DRAFT ? draft + (long long)c.row * ldq : nullptr;
+    row.hi = hi;
+    row.vec = vec;
+    row.rej = c.rej;
+    row.zi = s.zi;
+    row.rejected = s.rejected;
     if (c.op == 0) {
       double sum = 0.0;
-      if (vec) {
-        for (int i = lo + lane * VE; i < hi; i += step) {
-          float p[VE], q[VE];
-          tv_loadv(pr + i, p);
-          if (DRAFT && c.rej > 0) tv_loadv(qr + i, q);
+      for (int base = lo; base < hi; base += TV_BATCH * step) {
+        if (held != c.row || (DRAFT && c.rej > 0 && !held_q)) {
 #pragma unroll
-          for (int e = 0; e < VE; ++e) sum += weight(i + e, p[e], DRAFT && c.rej > 0 ? q[e] : 0.f);
+          for (int k = 0; k < TV_BATCH; ++k) row.load(base + k * step + lane * VE, x[k], y[k]);
         }
-      } else {
-        for (int i = lo + lane; i < hi; i += 32)
-          sum += weight(i, tv_load1(pr + i), DRAFT && c.rej > 0 ? tv_load1(qr + i) : 0.f);
-      }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int k = 0; k < TV_BATCH; ++k) {
+          double w[VE];
+          row.weigh(base + k * step + lane * VE, x[k], y[k], w);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) sum += w[e];
+        }
+      }
+      if (whole) {
+        held_q = c.rej > 0 || (held == c.row && held_q);
+        held = c.row;
+      }
+      sum = tv_warp_sum(sum);
       if (lane == 0) s.warp_sum[warp] = sum;
       __syncthreads();
       if (tid == 0) {
@@ -386,27 +443,55 @@ __global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
         if (x > 0.0) last = w;
         before += x;
       }
+      // that slice again, VE neighbouring weights a thread and a turn of the block (one load latency
+      // instead of one warp's chain of them): prefix sums over the lanes, then over the warps
       const bool any = mine < 0;
-      if (warp == (any ? last : mine)) {
-        double run = 0.0;
-        int found = -1, best = 0;
-        for (int base = lo; base < hi && found < 0; base += 32) {
-          const int i = base + lane;
-          const double w = i < hi ? weight(i, tv_load1(pr + i), DRAFT && c.rej > 0 ? tv_load1(qr + i) : 0.f) : 0.0;
-          double cum = w;
+      const int wsel = any ? last : mine;
+      const long long sf = (long long)(rank * TV_WARPS + wsel) * per;
+      const int slo = (int)(sf < V ? sf : V), shi = (int)(sf + per < V ? sf + per : V);
+      row.hi = shi;
+      double run = 0.0;
+      for (int base = slo; base < shi; base += TV_THREADS * VE) {
+        float x1[VE], y1[VE];
+        double w[VE], own = 0.0;
+        const int i = base + tid * VE;
+        row.load(i, x1, y1);
+        row.weigh(i, x1, y1, w);
+        int last_pos = -1;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double up = __shfl_up_sync(0xffffffffu, cum, o);
-            if (lane >= o) cum += up;
-          }
-          const unsigned pos = __ballot_sync(0xffffffffu, w > 0.0);
-          const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && run + cum > at);
-          if (pos) best = base + 31 - __clz(pos);
-          if (hit && !any) found = base + __ffs(hit) - 1;
-          run += __shfl_sync(0xffffffffu, cum, 31);
+        for (int e = 0; e < VE; ++e) {
+          own += w[e];
+          if (w[e] > 0.0) last_pos = i + e;
         }
-        if (lane == 0) ob[c.slot] = found >= 0 ? found : best;
+        double cum = own;                                // lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double up = __shfl_up_sync(0xffffffffu, cum, o);
+          if (lane >= o) cum += up;
+        }
+        __syncthreads();                                 // (warp_sum was read above, or in the turn before)
+        if (lane == 31) s.warp_sum[warp] = cum;
+        if (tid == 0) s.found = INT_MAX;
+        if (tid == 0 && base == slo) s.best = 0;
+        __syncthreads();
+        double c2 = run;
+        for (int k = 0; k < TV_WARPS; ++k) {
+          if (k < warp) c2 += s.warp_sum[k];
+          run += s.warp_sum[k];
+        }
+        c2 += cum - own;
+        int first_pos = INT_MAX;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          c2 += w[e];
+          if (first_pos == INT_MAX && w[e] > 0.0 && c2 > at) first_pos = i + e;
+        }
+        if (!any && first_pos != INT_MAX) atomicMin(&s.found, first_pos);
+        if (last_pos >= 0) atomicMax(&s.best, last_pos);
+        __syncthreads();
+        if (s.found != INT_MAX) break;
       }
+      if (tid == 0) ob[c.slot] = slo < shi ? (s.found != INT_MAX ? s.found : s.best) : 0;
     }
     break;
   }
@@ -423,11 +508,19 @@ __global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
 
 // ---------------------------------------------------------------------------------------
 // the accepted path's rows behind the committed context: slot ctx + path[j] -> ctx + j
-// (j = 1 .. accepted) in every layer.  One CTA per (sequence, layer); a thread owns 16 bytes of
-// the row (fp8 V, transposed inside its block: one value column) and moves them for every
-// j in order.  A path rises (path[j] >= j), so no later source lies at an earlier
-// destination, and reading four rows ahead of writing them is safe.
+// (j = 1 .. accepted) in every layer.  A path rises (path[j] >= j), so no later source lies at
+// an earlier destination: moves in the order of j, reading ahead of writing.
+//
+// Grid (sequence, layer, part).  Rows that lie whole in a page (K, bf16 V): a thread owns 16
+// bytes of the row.  fp8 V lies transposed in its page, [column][64 keys]: parts 1 .. take 256
+// columns each; the two pages around the tree come in whole (16-byte pieces, 128 bytes a
+// column), a thread permutes its column in shared memory, and the pieces that a destination
+// lies in go back: byte moves in global memory fetched the same sectors one dependent
+// byte at a time (61 us for 46 layers x 16 sequences of 61 nodes).  A tree that reaches over a
+// third page moves bytes.
 constexpr int TC_LAYERS = 64;   // layers of one launch (their pointers travel as parameters)
+constexpr int TC_MOVES = 256;   // moves of one turn
+constexpr int TC_LD = 132;      // a column's two pages in shared memory (33 words: no bank conflicts)
 struct TcLayers {
   void* k[TC_LAYERS];
   void* v[TC_LAYERS];
@@ -442,28 +535,35 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
                                                           int num_blocks, int Hkv, int kb, int vb, int fp8_v, int Dv) {
   griddep_wait();
   griddep_launch_dependents();
-  __shared__ int src[256], dst[256];   // flat cache rows (page * 64 + offset), -1: nothing to move
+  __shared__ int src[TC_MOVES], dst[TC_MOVES];   // flat cache rows (page * 64 + offset), -1: nothing to move
+  __shared__ __align__(16) uint8_t cols[256 * TC_LD];
+  __shared__ int reach;                          // the furthest source
   const int b = blockIdx.x, tid = threadIdx.x;
   const int n = q_start[b + 1] - q_start[b];
   const int ctx = kv_len[b] - n;
   const int acc = min(min(accepted[b], P - 1), n - 1);
-  if (ctx < 0) return;
+  if (ctx < 0 || acc < 1) return;
   uint8_t* kc = static_cast<uint8_t*>(layers.k[blockIdx.y]);
   uint8_t* vc = static_cast<uint8_t*>(layers.v[blockIdx.y]);
-  const int kch = kb >> 4, vch = vb >> 4;   // 16-byte pieces of one head's K and V row
-  for (int j0 = 1; j0 <= acc; j0 += 256) {
+  const int kch = kb >> 4, vch = vb >> 4;        // 16-byte pieces of one head's K and V row
+  const int pg0 = (ctx + 1) >> 6;                // the two pages (fp8 V)
+  const int part = blockIdx.z;
+  for (int j0 = 1; j0 <= acc; j0 += TC_MOVES) {
+    __syncthreads();
+    if (tid == 0) reach = 0;
     __syncthreads();
     const int j = j0 + tid;
     int f = -1, t = -1;
     if (j <= acc) {
       const int node = path[(size_t)b * P + j];
-      if (node > j && node < n) {           // node == j: already in place
+      if (node > j && node < n) {                // node == j: already in place
         const int fs = ctx + node, ts = ctx + j;
         if ((fs >> 6) < bt_cols) {
           const int fp = bt[(size_t)b * bt_stride + (fs >> 6)], tp = bt[(size_t)b * bt_stride + (ts >> 6)];
           if (fp >= 0 && fp < num_blocks && tp >= 0 && tp < num_blocks) {
             f = fp * 64 + (fs & 63);
             t = tp * 64 + (ts & 63);
+            if (part > 0) atomicMax(&reach, fs);
           }
         }
       }
@@ -471,35 +571,70 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
     src[tid] = f;
     dst[tid] = t;
     __syncthreads();
-    const int cnt = min(256, acc - j0 + 1);
-    const int kw = Hkv * kch, all = kw + (fp8_v ? Hkv * Dv : Hkv * vch);
-    for (int c = tid; c < all; c += 256) {
-      if (c >= kw && fp8_v) {               // column d of head h: byte (page, h, d, offset)
-        const int col = c - kw;
-        for (int i = 0; i < cnt; ++i) {
-          const int f1 = src[i], t1 = dst[i];
-          if (f1 < 0) continue;
-          const size_t hd = (size_t)Hkv * Dv;
-          vc[((t1 >> 6) * hd + col) * 64 + (t1 & 63)] = vc[((f1 >> 6) * hd + col) * 64 + (f1 & 63)];
+    const int cnt = min(TC_MOVES, acc - j0 + 1);
+    if (part == 0) {
+      const int kw = Hkv * kch, all = kw + (fp8_v ? 0 : Hkv * vch);
+      for (int c = tid; c < all; c += 256) {
+        uint8_t* base = c < kw ? kc : vc;
+        const int ch = c < kw ? kch : vch, cc = c < kw ? c : c - kw;
+        const int h = cc / ch, o = cc - h * ch;
+        const size_t rb = (size_t)ch << 4;
+        auto at = [&](int row) {
+          return reinterpret_cast<uint4*>(base + (((size_t)(row >> 6) * Hkv + h) * 64 + (row & 63)) * rb) + o;
+        };
+        for (int i = 0; i < cnt; i += 4) {
+          uint4 x[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (i + u < cnt && src[i + u] >= 0) x[u] = *at(src[i + u]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (i + u < cnt && src[i + u] >= 0) *at(dst[i + u]) = x[u];
         }
-        continue;
       }
-      uint8_t* base = c < kw ? kc : vc;
-      const int ch = c < kw ? kch : vch, cc = c < kw ? c : c - kw;
-      const int h = cc / ch, o = cc - h * ch;
-      const size_t rb = (size_t)ch << 4;
-      auto at = [&](int row) {
-        return reinterpret_cast<uint4*>(base + (((size_t)(row >> 6) * Hkv + h) * 64 + (row & 63)) * rb) + o;
-      };
-      for (int i = 0; i < cnt; i += 4) {
-        uint4 x[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (i + u < cnt && src[i + u] >= 0) x[u] = *at(src[i + u]);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (i + u < cnt && src[i + u] >= 0) *at(dst[i + u]) = x[u];
+      continue;
+    }
+    const int c0 = (part - 1) * 256, nc = min(256, Hkv * Dv - c0);
+    const size_t page_b = (size_t)Hkv * Dv * 64;
+    if ((reach >> 6) > pg0 + 1) {
+      for (int i = 0; tid < nc && i < cnt; ++i) {
+        const int f1 = src[i], t1 = dst[i];
+        if (f1 < 0) continue;
+        uint8_t* col = vc + (size_t)(c0 + tid) * 64;
+        col[(t1 >> 6) * page_b + (t1 & 63)] = col[(f1 >> 6) * page_b + (f1 & 63)];
       }
+      continue;
+    }
+    int pages[2];
+    for (int g = 0; g < 2; ++g) pages[g] = pg0 + g < bt_cols ? bt[(size_t)b * bt_stride + pg0 + g] : -1;
+    if (reach == 0 || pages[0] < 0 || pages[0] >= num_blocks) continue;   // (without the first page no source lies in one)
+    const bool second = (reach >> 6) > pg0;                               // (its id was checked with the move)
+    const int pieces = second ? 8 : 4;
+    for (int i = tid; i < nc * pieces; i += 256) {
+      const int c = i / pieces, o = i - c * pieces;
+      const uint4 x = *reinterpret_cast<const uint4*>(vc + pages[o >> 2] * page_b + (size_t)(c0 + c) * 64 + (o & 3) * 16);
+      uint32_t* d = reinterpret_cast<uint32_t*>(cols + c * TC_LD + o * 16);
+      d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w;
+    }
+    __syncthreads();
+    if (tid < nc) {
+      uint8_t* col = cols + tid * TC_LD;
+      for (int i = 0; i < cnt; ++i) {
+        const int f1 = src[i], t1 = dst[i];
+        if (f1 < 0) continue;
+        // (the same page twice in a table would be the caller's own two names of one slot)
+        const int fo = ((f1 >> 6) == pages[0] ? 0 : 64) + (f1 & 63), to = ((t1 >> 6) == pages[0] ? 0 : 64) + (t1 & 63);
+        col[to] = col[fo];
+      }
+    }
+    __syncthreads();
+    const int a0 = (ctx + j0) - pg0 * 64, a1 = (ctx + j0 + cnt - 1) - pg0 * 64;   // destinations
+    for (int i = tid; i < nc * pieces; i += 256) {
+      const int c = i / pieces, o = i - c * pieces;
+      if (o * 16 > a1 || o * 16 + 15 < a0) continue;
+      const uint32_t* d = reinterpret_cast<const uint32_t*>(cols + c * TC_LD + o * 16);
+      *reinterpret_cast<uint4*>(vc + pages[o >> 2] * page_b + (size_t)(c0 + c) * 64 + (o & 3) * 16) =
+          make_uint4(d[0], d[1], d[2], d[3]);
     }
   }
 }
@@ -515,7 +650,7 @@ int tv_launch(const void* probs, long long ldp, const void* draft, long long ldq
                    (!DRAFT || (ldq % VE == 0 && (reinterpret_cast<uintptr_t>(draft) & 15) == 0));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C, B);
-  cfg.blockDim = dim3(TV_THREADS);
+  cfg.blockDim = dim3(TvCfg<DRAFT>::THREADS);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -594,6 +729,7 @@ int xtu_tree_commit(const long long* k_ptrs, const long long* v_ptrs, long long 
                     int num_blocks, int Hkv, int kb, int vb, int fp8_v, int Dv, cudaStream_t s) {
   if (B <= 0 || L <= 0 || P <= 1) return 0;
   if (kb % 16 != 0 || (!fp8_v && vb % 16 != 0)) return -2;
+  const int parts = fp8_v ? 1 + (Hkv * Dv + 255) / 256 : 1;
   int launches = 0;
   for (int l0 = 0; l0 < L; l0 += TC_LAYERS) {
     const int m = L - l0 < TC_LAYERS ? L - l0 : TC_LAYERS;
@@ -602,7 +738,7 @@ int xtu_tree_commit(const long long* k_ptrs, const long long* v_ptrs, long long 
       t.k[l] = reinterpret_cast<void*>(k_ptrs ? k_ptrs[l0 + l] : k_base + (l0 + l) * k_step);
       t.v[l] = reinterpret_cast<void*>(v_ptrs ? v_ptrs[l0 + l] : v_base + (l0 + l) * v_step);
     }
-    const cudaError_t e = launch_pdl(tree_commit_kernel, dim3(B, m), dim3(256), 0, s, t, path, P, accepted, q_start,
+    const cudaError_t e = launch_pdl(tree_commit_kernel, dim3(B, m, parts), dim3(256), 0, s, t, path, P, accepted, q_start,
                                      kv_len, bt, bt_stride, bt_cols, num_blocks, Hkv, kb, vb, fp8_v, Dv);
     if (e != cudaSuccess) {
       (void)cudaGetLastError();

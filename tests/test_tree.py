@@ -599,19 +599,36 @@ def test_commit(device, fp8, L, Hk, D, Dv, lens, ctx):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-def test_commit_moves_nothing_outside_the_tree(device):
+@pytest.mark.parametrize("fp8", [False, True])
+def test_commit_moves_nothing_outside_the_tree(device, fp8):
     """accepted beyond the path, entries that do not rise, lie outside the tree or name no page."""
-    k, v, path, acc, qs, kl, bt = commit_inputs(2, 2, 64, 64, [6, 6, 6], [60, 61, 3], False, 32)
+    k, v, path, acc, qs, kl, bt = commit_inputs(2, 2, 64, 64, [6, 6, 6], [60, 61, 3], fp8, 32)
     path[0] = i32([0, 1, 0, 9, -1, -1])
     path[1] = i32([0, 1, 2, 3, 4, 5])
     path[2] = i32([0, 2, 1, 2 ** 30, -5, 6])
     acc[:] = i32([5, 100, 5])
     k1, v1 = k.clone(), v.clone()
     p = int(bt[2, 0])
-    k1[:, p, :, 4], v1[:, p, :, 4] = k[:, p, :, 5], v[:, p, :, 5]     # the one good entry: node 2 to slot 1
+    if fp8:
+        k, v, k1, v1 = (x.view(torch.uint8) for x in (k, v, k1, v1))
+        v1[:, p, :, :, 4] = v[:, p, :, :, 5]
+    else:
+        v1[:, p, :, 4] = v[:, p, :, 5]
+    k1[:, p, :, 4] = k[:, p, :, 5]                     # the one good entry: node 2 to slot 1
     kd, vd = k.to(device), v.to(device)
-    tree.commit_tree(kd, vd, *[t.to(device) for t in (path, acc, qs, kl, bt)])
+    t = FP8 if fp8 else torch.bfloat16
+    tree.commit_tree(kd.view(t), vd.view(t), *[x.to(device) for x in (path, acc, qs, kl, bt)])
     assert torch.equal(kd.cpu(), k1) and torch.equal(vd.cpu(), v1)
+    # a path that falls back after reaching the second page: the first move is good, the second is none
+    k, v, path, acc, qs, kl, bt = commit_inputs(1, 2, 64, 64, [50], [40], fp8, 33)
+    path[0, :3] = i32([0, 45, 2])
+    acc[:] = 2
+    path[0, 3:] = -1
+    one = acc.clone().fill_(1)
+    k1, v1 = commit_oracle(k, v, path, one, qs, kl, bt)
+    kd, vd = k.to(device), v.to(device)
+    tree.commit_tree(kd, vd, *[x.to(device) for x in (path, acc, qs, kl, bt)])
+    assert torch.equal(kd.cpu().double(), k1) and torch.equal(vd.cpu().double(), v1)
 
 
 # ---------------------------------------------------------------- together

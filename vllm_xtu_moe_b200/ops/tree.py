@@ -59,15 +59,17 @@ class TreeVerdict:
     last_row: torch.Tensor       # int32 [B] row of the last accepted node (-1: a sequence without nodes)
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
+# A step makes these calls once per layer and their kernels take a few microseconds, so the checks are
+# written to cost little where they pass: messages are put together only for a refusal.
 def _ints(name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}, not "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _table(bt: torch.Tensor, B: int, device: torch.device) -> None:
+    if bt.dtype is not torch.int32 or bt.dim() != 2 or bt.shape[0] < B or bt.stride(1) != 1 or bt.device != device:
+        raise ValueError(f"block_table must be int32 [{B}, blocks] with contiguous rows on {device}")
 
 
 def _max_nodes(n: int) -> None:
@@ -76,7 +78,12 @@ def _max_nodes(n: int) -> None:
 
 
 def _elsewhere(device: torch.device) -> bool:
-    return device.type == "cuda" and device.index != torch.cuda.current_device()
+    return device.index != torch.cuda.current_device()
+
+
+def _status(device: torch.device) -> int:
+    st = N._status.get(device.index)
+    return (st if st is not None else N.status_buffer(device)).data_ptr()
 
 
 # ---------------------------------------------------------------------------
@@ -108,8 +115,8 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, max_nodes: int, mask
     _ints("parents", parents, (T,), dev)
     _ints("q_start", q_start, (B + 1,), dev)
     W = (max_nodes + 31) // 32
-    mask = mask if mask is not None else torch.empty(T, W, dtype=torch.int32, device=dev)
-    depth = depth if depth is not None else torch.empty(T, dtype=torch.int32, device=dev)
+    mask = mask if mask is not None else parents.new_empty((T, W))
+    depth = depth if depth is not None else parents.new_empty(T)
     _ints("mask", mask, (T, W), dev)
     _ints("depth", depth, (T,), dev)
     if not parents.is_cuda:
@@ -119,7 +126,7 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, max_nodes: int, mask
         with torch.cuda.device(dev):
             return tree_mask(parents, q_start, max_nodes, mask, depth)
     N.call("xtu_tree_mask", parents.data_ptr(), q_start.data_ptr(), B, max_nodes, W, mask.data_ptr(),
-           depth.data_ptr(), N.status_buffer(dev).data_ptr(), N.stream_ptr(dev))
+           depth.data_ptr(), _status(dev), N.stream_ptr(dev))
     return mask, depth
 
 
@@ -203,82 +210,93 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     latent caches are not served.  ``workspace``: fp32, ``splits * T * Hq * (Dv + 2)`` elements when
     the KV range is split; allocated when None or too small.  One that is passed in belongs to
     the call until its work is done: calls that may overlap take one each."""
-    _need(q.dim() == 3 and q.dtype == torch.bfloat16 or not q.is_cuda, "q must be [T, Hq, D] bfloat16")
+    if q.dim() != 3 or (q.is_cuda and q.dtype is not torch.bfloat16):
+        raise ValueError("q must be [T, Hq, D] bfloat16")
     T, Hq, D = q.shape
     dev = q.device
-    _need(k_cache.dim() == 4 and v_cache is not None and v_cache.dim() == 4, "tree attention takes a K and a V cache")
+    if k_cache.dim() != 4 or v_cache is None or v_cache.dim() != 4:
+        raise ValueError("tree attention takes a K and a V cache [blocks, Hkv, 64, D]")
     nb, Hk, bs, Dk = k_cache.shape
-    fp8 = k_cache.dtype == _FP8
+    fp8 = k_cache.dtype is _FP8
     Dv = v_cache.shape[2] if fp8 else v_cache.shape[3]
-    _need(tuple(v_cache.shape) == ((nb, Hk, Dv, bs) if fp8 else (nb, Hk, bs, Dv)) and Dk == D
-          and v_cache.dtype == k_cache.dtype, "K and V caches do not match each other or q")
-    _need(Hq % Hk == 0, f"{Hq} query heads do not divide over {Hk} KV heads")
+    if v_cache.shape != ((nb, Hk, Dv, bs) if fp8 else (nb, Hk, bs, Dv)) or Dk != D or v_cache.dtype != k_cache.dtype:
+        raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} do not match each other or q")
+    if Hq % Hk:
+        raise ValueError(f"{Hq} query heads do not divide over {Hk} KV heads")
+    if k_cache.device != dev or v_cache.device != dev:
+        raise ValueError(f"the caches must be on {dev}")
     B = meta.num_seqs
+    bt, mask = meta.block_table, meta.mask
     _max_nodes(meta.max_nodes)
-    _need(k_cache.device == dev and v_cache.device == dev, f"the caches must be on {dev}")
     _ints("q_start", meta.q_start, (B + 1,), dev)
     _ints("kv_len", meta.kv_len, (B,), dev)
-    bt = meta.block_table
-    _need(bt.dtype == torch.int32 and bt.dim() == 2 and bt.shape[0] >= B and bt.stride(1) == 1 and bt.device == dev,
-          "block_table must be int32 [B, blocks] with contiguous rows")
-    W = meta.mask.shape[1]
-    _ints("mask", meta.mask, (T, W), dev)
-    _need(32 * W >= meta.max_nodes, f"a mask of {W} words is too narrow for {meta.max_nodes} nodes")
+    _table(bt, B, dev)
+    W = mask.shape[-1]
+    _ints("mask", mask, (T, W), dev)
+    if 32 * W < meta.max_nodes:
+        raise ValueError(f"a mask of {W} words is too narrow for {meta.max_nodes} nodes")
     if window > 0:
-        _need(meta.depth is not None, "a sliding window needs the nodes' depths")
+        if meta.depth is None:
+            raise ValueError("a sliding window needs the nodes' depths")
         _ints("depth", meta.depth, (T,), dev)
-    if sinks is not None:
-        _need(sinks.dtype == torch.float32 and sinks.is_contiguous() and sinks.numel() == Hq and sinks.device == dev,
-              f"sinks must be fp32 [{Hq}]")
+    if sinks is not None and (sinks.dtype is not torch.float32 or not sinks.is_contiguous() or sinks.numel() != Hq
+                              or sinks.device != dev):
+        raise ValueError(f"sinks must be contiguous fp32 [{Hq}] on {dev}")
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    _need(scale > 0 and k_scale > 0, "scales must be positive")
+    if not (scale > 0 and k_scale > 0):
+        raise ValueError("scales must be positive")
     if out is None:
-        out = torch.empty(T, Hq, Dv, dtype=q.dtype, device=dev)
-    _need(tuple(out.shape) == (T, Hq, Dv) and out.dtype == q.dtype and out.is_contiguous() and out.device == dev,
-          f"out must be contiguous {q.dtype} [{T}, {Hq}, {Dv}]")
+        out = q.new_empty((T, Hq, Dv))
+    elif out.shape != (T, Hq, Dv) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be contiguous {q.dtype} [{T}, {Hq}, {Dv}] on {dev}")
     if not q.is_cuda:
         return tree_attention_ref(q, k_cache, v_cache, meta, scale, out, window, sinks, k_scale, v_scale)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return tree_attention(q, k_cache, v_cache, meta, scale, out, workspace, window, sinks, k_scale, v_scale)
-    _need(fp8 or k_cache.dtype == torch.bfloat16, "the cache must be bfloat16 or float8_e4m3fn")
-    _need((D, Dv) in (FP8_HEAD_DIMS if fp8 else HEAD_DIMS),
-          f"{'fp8 ' if fp8 else ''}head sizes {D} / {Dv} are not served ({FP8_HEAD_DIMS if fp8 else HEAD_DIMS})")
-    _need(bs == KV_BLOCK, f"the GPU kernels read KV blocks of {KV_BLOCK} tokens, not {bs}")
-    _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "the caches must be contiguous")
-    _need(nb > 0 and (nb + 1) * Hk * max(bs, Dv) < 2 ** 31, "the cache has more rows than 31 bits count")
-    _need(q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0 and q.data_ptr() % 16 == 0,
-          "q rows must be contiguous and start on 16-byte boundaries")
+    if not fp8 and k_cache.dtype is not torch.bfloat16:
+        raise ValueError(f"the cache must be bfloat16 or float8_e4m3fn, not {k_cache.dtype}")
+    if (D, Dv) not in (FP8_HEAD_DIMS if fp8 else HEAD_DIMS):
+        raise ValueError(f"{'fp8 ' if fp8 else ''}head sizes {D} / {Dv} are not served "
+                         f"({FP8_HEAD_DIMS if fp8 else HEAD_DIMS})")
+    if bs != KV_BLOCK:
+        raise ValueError(f"the GPU kernels read KV blocks of {KV_BLOCK} tokens, not {bs}")
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous() or (k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+        raise ValueError("the caches must be contiguous and start on 16-byte boundaries")
+    if not 0 < (nb + 1) * Hk * max(bs, Dv) < 2 ** 31:
+        raise ValueError("the cache is empty or has more rows than 31 bits count")
+    q_ts, q_hs, q1 = q.stride()
+    if q1 != 1 or (q_ts | q_hs) & 7 or q.data_ptr() & 15:
+        raise ValueError("q rows must be contiguous and start on 16-byte boundaries")
     rows = meta.max_nodes * (Hq // Hk)
     seen = min(meta.max_kv_len, window + meta.max_nodes + KV_BLOCK) if window > 0 else meta.max_kv_len
     splits = meta.num_splits if meta.num_splits > 0 else tree_splits(B, Hk, rows, seen, fp8, D, Dv)
-    _need(splits <= MAX_SPLITS, f"at most {MAX_SPLITS} splits")
+    if splits > MAX_SPLITS:
+        raise ValueError(f"at most {MAX_SPLITS} splits")
     ws = None
     if splits > 1:
         need = splits * T * Hq * (Dv + 2)
         ws = workspace
-        if ws is not None:
-            _need(ws.dtype == torch.float32 and ws.is_contiguous() and ws.device == dev and ws.data_ptr() % 16 == 0,
-                  "workspace must be contiguous fp32 on q's device")
+        if ws is not None and (ws.dtype is not torch.float32 or not ws.is_contiguous() or ws.device != dev
+                               or ws.data_ptr() & 15):
+            raise ValueError(f"workspace must be contiguous fp32 on {dev}, on a 16-byte boundary")
         if ws is None or ws.numel() < need:
             ws = torch.empty(need, dtype=torch.float32, device=dev)
-    N.call("xtu_tree_attention", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
+    N.call("xtu_tree_attention", q.data_ptr(), q_ts, q_hs, k_cache.data_ptr(), v_cache.data_ptr(),
            int(fp8), out.data_ptr(), meta.q_start.data_ptr(), meta.kv_len.data_ptr(), bt.data_ptr(), bt.stride(0),
            bt.shape[1], meta.mask.data_ptr(), W, N.ptr(meta.depth), int(window), B, meta.max_nodes, T, Hq, Hk, D, Dv,
            nb, float(scale), float(k_scale), float(v_scale), N.ptr(sinks), splits, N.ptr(ws),
-           N.status_buffer(dev).data_ptr(), N.stream_ptr(dev))
+           _status(dev), N.stream_ptr(dev))
     return out
 
 
 # ---------------------------------------------------------------------------
 # verification
 # ---------------------------------------------------------------------------
-def _verdict(B: int, max_nodes: int, device) -> TreeVerdict:
-    buf = torch.empty(2 * B * (max_nodes + 1), dtype=torch.int32, device=device)
-    n = B * max_nodes
-    return TreeVerdict(accepted=buf[2 * n:2 * n + B], path=buf[:n].view(B, max_nodes),
-                       tokens=buf[n:2 * n].view(B, max_nodes), last_row=buf[2 * n + B:])
+def _verdict(B: int, max_nodes: int, like: torch.Tensor) -> TreeVerdict:
+    return TreeVerdict(like.new_empty(B), like.new_empty((B, max_nodes)), like.new_empty((B, max_nodes)),
+                       like.new_empty(B))
 
 
 def _children(parents: list, n: int, at: int) -> list:
@@ -289,7 +307,7 @@ def _walk(tokens, parents, q_start, max_nodes, choose, final) -> TreeVerdict:
     """The verification of every sequence on the host: ``choose(row, children)`` -> the accepted
     child or None, ``final(row, children, b)`` -> the token after the path."""
     qs, par, tok = q_start.tolist(), parents.tolist(), tokens.tolist()
-    v = _verdict(len(qs) - 1, max_nodes, tokens.device)
+    v = _verdict(len(qs) - 1, max_nodes, tokens)
     for t in (v.path, v.tokens, v.last_row):
         t.fill_(-1)
     v.accepted.zero_()
@@ -340,10 +358,10 @@ def verify_tree_greedy(target: torch.Tensor, tokens: torch.Tensor, parents: torc
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return verify_tree_greedy(target, tokens, parents, q_start, max_nodes)
-    v = _verdict(B, max_nodes, dev)
+    v = _verdict(B, max_nodes, tokens)
     N.call("xtu_tree_verify_greedy", target.data_ptr(), tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), B,
            max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
-           N.status_buffer(dev).data_ptr(), N.stream_ptr(dev))
+           _status(dev), N.stream_ptr(dev))
     return v
 
 
@@ -419,26 +437,26 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     distribution.  NaN and negative entries weigh nothing, and a draft outside the vocabulary is
     never accepted."""
     T, B, dev = _tree_args(tokens, parents, q_start, max_nodes)
-    _need(probs.dim() == 2 and probs.shape[0] == T and probs.shape[1] > 0 and probs.device == dev
-          and probs.stride(1) == 1 and probs.dtype in (torch.float32, torch.bfloat16),
-          f"probs must be fp32 or bf16 [{T}, V] with contiguous rows on {dev}")
-    if draft_probs is not None:
-        _need(draft_probs.shape == probs.shape and draft_probs.dtype == probs.dtype and draft_probs.device == dev
-              and draft_probs.stride(1) == 1, "draft_probs must match probs")
+    if (probs.dim() != 2 or probs.shape[0] != T or probs.shape[1] < 1 or probs.device != dev or probs.stride(1) != 1
+            or probs.dtype not in (torch.float32, torch.bfloat16)):
+        raise ValueError(f"probs must be fp32 or bf16 [{T}, V] with contiguous rows on {dev}")
+    if draft_probs is not None and (draft_probs.shape != probs.shape or draft_probs.dtype != probs.dtype
+                                    or draft_probs.device != dev or draft_probs.stride(1) != 1):
+        raise ValueError("draft_probs must match probs in shape and type, with contiguous rows")
     for name, u, n in (("u_accept", u_accept, T), ("u_draw", u_draw, B)):
-        _need(u.dtype == torch.float32 and tuple(u.shape) == (n,) and u.is_contiguous() and u.device == dev,
-              f"{name} must be contiguous fp32 [{n}] on {dev}")
+        if u.dtype is not torch.float32 or u.shape != (n,) or not u.is_contiguous() or u.device != dev:
+            raise ValueError(f"{name} must be contiguous fp32 [{n}] on {dev}")
     if not tokens.is_cuda:
         return verify_tree_ref(probs, tokens, parents, q_start, max_nodes, u_accept, u_draw, draft_probs)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return verify_tree(probs, tokens, parents, q_start, max_nodes, u_accept, u_draw, draft_probs)
-    v = _verdict(B, max_nodes, dev)
+    v = _verdict(B, max_nodes, tokens)
     N.call("xtu_tree_verify", probs.data_ptr(), probs.stride(0), N.ptr(draft_probs),
            0 if draft_probs is None else draft_probs.stride(0), int(probs.dtype == torch.bfloat16), probs.shape[1],
            tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(), B,
            max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
-           N.status_buffer(dev).data_ptr(), N.stream_ptr(dev))
+           _status(dev), N.stream_ptr(dev))
     return v
 
 
@@ -475,30 +493,44 @@ def commit_tree(k_caches, v_caches, path: torch.Tensor, accepted: torch.Tensor, 
     call of their own), as sequences of tensors or as one tensor with the layers in front; bf16
     or fp8 (V transposed inside each block).  A path must rise (a parent lies below its
     children); entries that do not, or that lie outside the tree or the cache, move nothing."""
-    L = len(k_caches)
-    _need(L == len(v_caches) and L > 0, "commit_tree takes as many K as V caches")
-    k0, v0 = k_caches[0], v_caches[0]
-    _need(k0.dim() == 4 and v0.dim() == 4, "caches are [blocks, Hkv, 64, D] per layer")
+    stacked = isinstance(k_caches, torch.Tensor) and isinstance(v_caches, torch.Tensor)
+    if stacked:
+        if k_caches.dim() != 5 or v_caches.dim() != 5:
+            raise ValueError("stacked caches are [layers, blocks, Hkv, 64, D]")
+        k0, v0, kshape, vshape, L, Lv = k_caches, v_caches, k_caches.shape[1:], v_caches.shape[1:], \
+            k_caches.shape[0], v_caches.shape[0]
+    else:
+        L, Lv = len(k_caches), len(v_caches)
+        if L == 0 or L != Lv:
+            raise ValueError("commit_tree takes as many K as V caches")
+        k0, v0 = k_caches[0], v_caches[0]
+        kshape, vshape = k0.shape, v0.shape
+        if len(kshape) != 4 or len(vshape) != 4:
+            raise ValueError("caches are [blocks, Hkv, 64, D] per layer")
+    if L == 0 or L != Lv:
+        raise ValueError("commit_tree takes as many K as V caches")
     dev = k0.device
-    nb, Hk, bs, D = k0.shape
-    fp8 = k0.dtype == _FP8
-    Dv = v0.shape[2] if fp8 else v0.shape[3]
-    _need(tuple(v0.shape) == ((nb, Hk, Dv, bs) if fp8 else (nb, Hk, bs, Dv)) and v0.dtype == k0.dtype
-          and v0.device == dev, "K and V caches do not match")
-    _need(bs == KV_BLOCK, f"KV blocks hold {KV_BLOCK} tokens, not {bs}")
+    nb, Hk, bs, D = kshape
+    fp8 = k0.dtype is _FP8
+    Dv = vshape[2] if fp8 else vshape[3]
+    if vshape != ((nb, Hk, Dv, bs) if fp8 else (nb, Hk, bs, Dv)):
+        raise ValueError(f"K and V caches {tuple(kshape)} and {tuple(vshape)} do not match")
+    if bs != KV_BLOCK:
+        raise ValueError(f"KV blocks hold 64 tokens, not {bs}")
+    if not fp8 and k0.dtype is not torch.bfloat16 and k0.is_cuda:
+        raise ValueError(f"the caches must be bfloat16 or float8_e4m3fn, not {k0.dtype}")
     B, P = path.shape
     _ints("path", path, (B, P), dev)
     _ints("accepted", accepted, (B,), dev)
     _ints("q_start", q_start, (B + 1,), dev)
     _ints("kv_len", kv_len, (B,), dev)
-    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= B
-          and block_table.stride(1) == 1 and block_table.device == dev,
-          "block_table must be int32 [B, blocks] with contiguous rows")
-    stacked = isinstance(k_caches, torch.Tensor) and isinstance(v_caches, torch.Tensor)
+    _table(block_table, B, dev)
     for k, v in ((k0, v0),) if stacked else zip(k_caches, v_caches):
-        _need(k.shape == k0.shape and v.shape == v0.shape and k.dtype == k0.dtype and v.dtype == k0.dtype
-              and k.device == dev and v.device == dev, "the layers' caches must be alike")
-        _need(k.is_contiguous() and v.is_contiguous(), "the caches must be contiguous")
+        if (k.shape != k0.shape or v.shape != v0.shape or k.dtype != k0.dtype or v.dtype != k0.dtype or k.device != dev
+                or v.device != dev):
+            raise ValueError("the layers' caches must be alike")
+        if not k.is_contiguous() or not v.is_contiguous():
+            raise ValueError("the caches must be contiguous")
     if not k0.is_cuda:
         commit_tree_ref(k_caches, v_caches, path, accepted, q_start, kv_len, block_table)
         return
@@ -506,14 +538,19 @@ def commit_tree(k_caches, v_caches, path: torch.Tensor, accepted: torch.Tensor, 
         with torch.cuda.device(dev):
             return commit_tree(k_caches, v_caches, path, accepted, q_start, kv_len, block_table)
     es = k0.element_size()
-    _need(D * es % 16 == 0 and (fp8 or Dv * es % 16 == 0), "head rows must be multiples of 16 bytes")
+    if D * es % 16 or (not fp8 and Dv * es % 16):
+        raise ValueError("head rows must be multiples of 16 bytes")
+    kp = vp = None
+    kb = ks = vb = vs = 0
     if stacked:
-        kp = vp = None
         kb, ks, vb, vs = k0.data_ptr(), k_caches.stride(0) * es, v0.data_ptr(), v_caches.stride(0) * es
+        odd = (kb | ks | vb | vs) & 15
     else:
-        kp, vp = (N.c_longlong * L)(*[k.data_ptr() for k in k_caches]), (N.c_longlong * L)(*[v.data_ptr() for v in v_caches])
-        kb = ks = vb = vs = 0
-    _need(all(x % 16 == 0 for x in ((kb, ks, vb, vs) if stacked else (*kp, *vp))), "caches start on 16-byte boundaries")
+        kl, vl = [k.data_ptr() for k in k_caches], [v.data_ptr() for v in v_caches]
+        kp, vp = (N.c_longlong * L)(*kl), (N.c_longlong * L)(*vl)
+        odd = any(x & 15 for x in kl) or any(x & 15 for x in vl)
+    if odd:
+        raise ValueError("the caches must start on 16-byte boundaries")
     N.call("xtu_tree_commit", kp, vp, kb, ks, vb, vs, L, path.data_ptr(), P, accepted.data_ptr(), q_start.data_ptr(),
            kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], B, nb, Hk, D * es,
            Dv * es, int(fp8), Dv, N.stream_ptr(dev))
