@@ -151,7 +151,7 @@ __device__ __forceinline__ float ta_v_at(const TaParams& p, bool f8, int DV, int
 
 // a row's output (32-bit partial or bf16 result, columns d0 .. d0 + cols - 1 of V) plus the non-finite
 // values of the keys of logical page pg that it sees
-__device__ __noinline__ void ta_add_bad(const TaParams& p, const TaRow& r, int q0, int b, int kh, int pg, int DV,
+__device__ __noinline__ void ta_add_bad(const TaParams& p, const TaRow& r, bool f8, int q0, int b, int kh, int pg, int DV,
                                         int d0, int cols, float* wo, __nv_bfloat16* o) {
   const int page = __ldg(p.block_table + (size_t)b * p.bt_stride + pg);
   if (page < 0 || page >= p.num_blocks) return;
@@ -160,54 +160,12 @@ __device__ __noinline__ void ta_add_bad(const TaParams& p, const TaRow& r, int q
     if (!ta_sees(p, r, q0, pg * TA_PAGE + k)) continue;
 #pragma unroll 1
     for (int d = 0; d < cols; ++d) {
-      const float y = ta_v_at(p, false, DV, page, kh, k, d0 + d);
+      const float y = ta_v_at(p, f8, DV, page, kh, k, d0 + d);
       if (isfinite(y)) continue;
       if (wo != nullptr) wo[d] += y;
       else o[d] = __float2bfloat16(__bfloat162float(o[d]) + y);
     }
   }
-}
-
-// ---------------------------------------------------------------------------------------
-// warp-level kernel: up to 64 query rows per CTA
-// ---------------------------------------------------------------------------------------
-// One CTA = one (row tile of 16 MT rows, kv split, kv head, sequence).  Warp 0 streams 64-key
-// pages of K and V through a shared-memory ring with TMA; CW consumer warps take m-tile
-// w % MT and key subset w / MT of every page: S = Q K^T (mma.sync m16n8k16), online softmax
-// in the exp2 domain with a lazily raised maximum, O += P V.  The key subsets meet in
-// shared memory at the end.
-template <int D, int DV, bool F8, int MT>
-struct TmCfg {
-  static constexpr int CW = MT == 1 ? 4 : 8;                     // consumer warps
-  static constexpr int ESZ = F8 ? 1 : 2;
-  static constexpr int K_BYTES = TA_PAGE * D * ESZ, V_BYTES = TA_PAGE * DV * ESZ;
-  static constexpr int STAGE = K_BYTES + V_BYTES;
-  static constexpr bool QSM = D > 128;                           // Q fragments from shared memory
-  static constexpr int QLD = D + 8;
-  static constexpr int Q_BYTES = QSM ? (MT * 16 * QLD * 2 + 1023) / 1024 * 1024 : 0;
-  static constexpr int BUDGET = 220 * 1024 - Q_BYTES;
-  static constexpr int STAGES = BUDGET / STAGE > 8 ? 8 : BUDGET / STAGE;
-  static constexpr int THREADS = 32 * (1 + CW);
-  static constexpr int BYTES = 1024 + Q_BYTES + STAGES * STAGE + 2 * STAGES * 8 + 64;
-  static_assert(STAGES >= 2, "ring");
-  static_assert(CW * 16 * DV * 4 <= STAGES * STAGE, "merge buffer");
-  static_assert(D % 64 == 0 && DV % 64 == 0 && (!F8 || (D <= 128 && DV <= 128)), "head sizes");
-};
-
-__device__ __forceinline__ void tm_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void tm_mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ void tm_e4m3(uint32_t w, uint32_t& lo, uint32_t& hi) {   // exact
@@ -223,436 +181,9 @@ __device__ __forceinline__ uint32_t tm_f16x2(float lo, float hi) {
   return r;
 }
 
-__device__ __forceinline__ void tm_ldsm4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-
-__device__ __forceinline__ void tm_ldsm4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-
-// 16-byte piece `ch` of key row `r` in a bf16 page ([64 keys][128 bytes] boxes, 128B swizzle)
-__device__ __forceinline__ uint32_t tm_piece(uint32_t base, int r, int ch) {
-  return base + (ch >> 3) * 8192 + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-}
-
-// fp8 pages: byte b of row r (rows of 128 bytes: 128B swizzle, of 64 bytes: 64B swizzle)
-template <int ROWB>
-__device__ __forceinline__ uint32_t tm_f8_off(int r, int b) {
-  if (ROWB == 128) return r * 128 + ((((b >> 4) ^ (r & 7)) << 4) | (b & 15));
-  return r * 64 + ((((b >> 4) ^ ((r >> 1) & 3)) << 4) | (b & 15));
-}
-
-__device__ __forceinline__ uint32_t tm_lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
-
-__device__ __forceinline__ uint4 tm_lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-
 // non-finite bf16 values of a packed pair as a mask of the halves to clear
 __device__ __forceinline__ uint32_t bad_bf16x2(uint32_t w) {
   return ((w & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((w & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
-}
-__device__ __forceinline__ uint32_t bad_e4m3x4(uint32_t w) {   // NaN is 0x7F / 0xFF
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (((w >> (8 * i)) & 0x7Fu) == 0x7Fu) m |= 0xFFu << (8 * i);
-  return m;
-}
-
-template <int D, int DV, bool F8, int MT>
-__global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mma_kernel(
-    const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-    const __grid_constant__ TaParams p) {
-  griddep_wait();
-  griddep_launch_dependents();
-  using C = TmCfg<D, DV, F8, MT>;
-  constexpr int CW = C::CW, STAGES = C::STAGES;
-  constexpr int NS = CW / MT;            // key subsets of a page
-  constexpr int KW = TA_PAGE / NS;       // keys of a warp per page
-  constexpr int NKT = KW / 8, DK = D / 16, DN = DV / 8;
-  extern __shared__ uint8_t tm_smem[];
-  const uint32_t sa = smem_u32(tm_smem);
-  uint8_t* base = tm_smem + (((sa + 1023u) & ~1023u) - sa);
-  __nv_bfloat16* sq = reinterpret_cast<__nv_bfloat16*>(base);
-  uint8_t* ring = base + C::Q_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + STAGES * C::STAGE);
-  uint64_t* empty = full + STAGES;
-  __shared__ int s_bad;                  // a masked page held a non-finite value
-  __shared__ float cm[CW * 16], cl[CW * 16];   // maximum and sum of each warp's rows
-  const int b = blockIdx.z, kh = blockIdx.y;
-  const int tile = blockIdx.x / p.splits, sp = blockIdx.x - tile * p.splits;
-  const int q0 = __ldg(p.q_start + b), n = __ldg(p.q_start + b + 1) - q0;
-  const int L = __ldg(p.kv_len + b), ctx = L - n;
-  const int r0 = tile * 16 * MT;
-  if (r0 >= n * p.G) return;             // uniform: no such row tile here
-  const int nrows = min(16 * MT, n * p.G - r0);
-  if (threadIdx.x == 0) {
-    s_bad = 0;
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], CW);
-    }
-    fence_barrier_init();
-  }
-  __syncthreads();
-  // pages of this split; with a window none below the first key that the tile's rows can see
-  // (the root's window reaches furthest back)
-  const int npages = min((L + TA_PAGE - 1) / TA_PAGE, p.bt_cols);
-  const int jfirst = p.window > 0 ? max(0, ctx - p.window + 1) / TA_PAGE : 0;
-  const int per = (npages - jfirst + p.splits - 1) / p.splits;
-  const int j0 = min(npages, jfirst + sp * per), j1 = min(npages, j0 + per);
-  const int nj = max(0, j1 - j0);
-  // pages below `open` and at or past `shut` are seen whole by every row; the others
-  // ("masked pages": the tree's own, the last, and with a window those it cuts) are not
-  const int shut = ctx / TA_PAGE;
-  const int open = p.window > 0 ? (max(0, ctx + n - p.window) + TA_PAGE - 1) / TA_PAGE : 0;   // depth < n
-  auto masked = [&](int page) { return page >= shut || page < open; };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) {
-    // ---------------- producer
-    if (lane == 0) {
-      prefetch_tmap(&tk);
-      prefetch_tmap(&tv);
-    }
-    bool ok = true;
-    int issued = 0;
-    const int* bt = p.block_table + (size_t)b * p.bt_stride + j0;
-    for (int c0 = 0; c0 < nj && ok; c0 += 32) {
-      const int page = c0 + lane < nj ? __ldg(bt + c0 + lane) : 0;
-      const int cnt = min(32, nj - c0);
-      for (int k = 0; k < cnt; ++k) {
-        const int pg = __shfl_sync(0xffffffffu, page, k);
-        // a page id outside the cache reads zero fill (TMA bounds); the bounds-check build reports it
-        if (lane == 0) (void)XTU_IN_BOUNDS(pg >= 0 && pg < p.num_blocks, p.status, 243, pg);
-        if (lane == 0) {
-          const int i = c0 + k, slot = i % STAGES;
-          if (i >= STAGES && !ta_wait(&empty[slot], ((i / STAGES) - 1) & 1, p.status, 140)) {
-            ok = false;
-          } else {
-            ++issued;
-            mbar_arrive_expect_tx(&full[slot], C::STAGE);
-            uint8_t* dst = ring + slot * C::STAGE;
-            const int pr = pg >= 0 && pg < p.num_blocks ? pg : p.num_blocks;   // past the end: zero fill
-            const int row = (pr * p.Hkv + kh) * TA_PAGE;
-            if constexpr (F8) {   // K [64 keys][D bytes]; V^T [DV rows][64 bytes]
-              tma_load_2d(dst, &tk, &full[slot], 0, row);
-              tma_load_2d(dst + C::K_BYTES, &tv, &full[slot], 0, (pr * p.Hkv + kh) * DV);
-            } else {
-#pragma unroll
-              for (int x = 0; x < D / 64; ++x) tma_load_2d(dst + x * 8192, &tk, &full[slot], x * 64, row);
-#pragma unroll
-              for (int x = 0; x < DV / 64; ++x)
-                tma_load_2d(dst + C::K_BYTES + x * 8192, &tv, &full[slot], x * 64, row);
-            }
-          }
-        }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        if (!ok) break;
-      }
-    }
-    if (!ok && lane == 0) {   // let the copies in flight land (bounded) before the CTA exits
-      for (int j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j)
-        ta_wait(&full[j % STAGES], (j / STAGES) & 1, nullptr, 0, 50000000ull);
-    }
-    return;
-  }
-  // ---------------- consumers
-  const int cw = warp - 1, ctid = threadIdx.x - 32;
-  const int mt = cw % MT, ks = cw / MT;
-  const int g4 = lane >> 2, tq = lane & 3;
-  TaRow row[2];
-  uint32_t qa[C::QSM ? 1 : DK][4];
-#pragma unroll
-  for (int h2 = 0; h2 < 2; ++h2) {
-    const int r = mt * 16 + g4 + h2 * 8;
-    const bool valid = r < nrows;
-    const int node = valid ? ta_node(p, r0 + r) : 0, hh = valid ? (r0 + r) - node * p.G : 0;
-    row[h2] = ta_row(p, q0, n, ctx, node, valid);
-    const __nv_bfloat16* qrow = p.q + (long long)(q0 + node) * p.q_ts + (long long)(kh * p.G + hh) * p.q_hs;
-    if constexpr (F8) {
-      // k-step s of lane tq covers d = tq * D/4 + 4 s + {0,1 | 2,3}: the order in which a lane
-      // reads K bytes, four at a time.  Q is rounded to f16 (11 bits of bf16's 8: exact
-      // within f16's range)
-#pragma unroll
-      for (int k = 0; k < DK; ++k) {
-        const uint2 v = valid ? __ldg(reinterpret_cast<const uint2*>(qrow + tq * (D / 4) + 4 * k)) : make_uint2(0u, 0u);
-        qa[k][h2] = tm_f16x2(bf16_lo(v.x), bf16_hi(v.x));
-        qa[k][2 + h2] = tm_f16x2(bf16_lo(v.y), bf16_hi(v.y));
-      }
-    } else if constexpr (!C::QSM) {
-#pragma unroll
-      for (int k = 0; k < DK; ++k) {
-        qa[k][h2] = valid ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * k + 2 * tq)) : 0u;
-        qa[k][2 + h2] = valid ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * k + 8 + 2 * tq)) : 0u;
-      }
-    }
-  }
-  if constexpr (C::QSM) {
-    for (int i = ctid; i < MT * 16 * (D / 8); i += 32 * CW) {
-      const int r = i / (D / 8), c = (i - r * (D / 8)) * 8;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (r < nrows) {
-        const int node = ta_node(p, r0 + r), hh = (r0 + r) - node * p.G;
-        v = __ldg(reinterpret_cast<const uint4*>(p.q + (long long)(q0 + node) * p.q_ts +
-                                                 (long long)(kh * p.G + hh) * p.q_hs + c));
-      }
-      *reinterpret_cast<uint4*>(sq + r * C::QLD + c) = v;
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory");
-  }
-  float o[DN][4];
-#pragma unroll
-  for (int i = 0; i < DN; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  bool ok = true;
-  for (int i = 0; i < nj; ++i) {
-    const int slot = i % STAGES;
-    if (ok && !ta_wait(&full[slot], (i / STAGES) & 1, p.status, 141)) ok = false;
-    const bool msk = masked(j0 + i);
-    const uint32_t kb = smem_u32(ring + slot * C::STAGE), vb = kb + C::K_BYTES;
-    if (msk) {
-      // masked pages: 0 * p must stay 0 for keys that a row does not see, so V's non-finite
-      // values become zero here and join the rows that do see them at the end.  Every
-      // consumer warp passes these two barriers, a timed-out one too.
-      if (ok) {
-        uint32_t* vw = reinterpret_cast<uint32_t*>(ring + slot * C::STAGE + C::K_BYTES);
-        bool any = false;
-        for (int w = ctid; w < C::V_BYTES / 4; w += 32 * CW) {
-          const uint32_t x = vw[w], bad = F8 ? bad_e4m3x4(x) : bad_bf16x2(x);
-          if (bad) {
-            vw[w] = x & ~bad;
-            any = true;
-          }
-        }
-        if (any) s_bad = 1;
-      }
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory");
-    }
-    if (!ok) continue;
-    const int key_lo = ks * KW;                              // this warp's first key in the page
-    const int kabs = (j0 + i) * TA_PAGE + key_lo;
-    // ---- S = Q K^T
-    float s[NKT][4];
-#pragma unroll
-    for (int nt = 0; nt < NKT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-    if constexpr (F8) {
-#pragma unroll
-      for (int nt = 0; nt < NKT; ++nt) {
-        // n-position g4 of tile nt is key 16 (nt/2) + 4 (g4/2) + 2 (nt%2) + g4%2 of the warp's keys,
-        // so that a lane's four P values below are four consecutive keys
-        const int r = key_lo + 16 * (nt >> 1) + 4 * (g4 >> 1) + 2 * (nt & 1) + (g4 & 1);
-        uint32_t w[D / 16];
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const uint4 v = tm_lds128(kb + tm_f8_off<D>(r, tq * (D / 4) + 16 * c));
-          w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
-        }
-#pragma unroll
-        for (int k = 0; k < DK; ++k) {
-          uint32_t b0, b1;
-          tm_e4m3(w[k], b0, b1);
-          tm_mma_f16(s[nt], qa[k], b0, b1);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int kc = 0; kc < DK / 2; ++kc) {
-        uint32_t a0[4], a1[4];
-        if constexpr (C::QSM) {
-          const uint32_t qb = smem_u32(sq + (mt * 16 + (lane & 15)) * C::QLD + kc * 32 + (lane >> 4) * 8);
-          tm_ldsm4(qb, a0[0], a0[1], a0[2], a0[3]);
-          tm_ldsm4(qb + 32, a1[0], a1[1], a1[2], a1[3]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NKT; ++nt) {
-          uint32_t b0, b1, b2, b3;
-          tm_ldsm4(tm_piece(kb, key_lo + nt * 8 + (lane & 7), kc * 4 + (lane >> 3)), b0, b1, b2, b3);
-          if constexpr (C::QSM) {
-            tm_mma(s[nt], a0, b0, b1);
-            tm_mma(s[nt], a1, b2, b3);
-          } else {
-            tm_mma(s[nt], qa[2 * kc], b0, b1);
-            tm_mma(s[nt], qa[2 * kc + 1], b2, b3);
-          }
-        }
-      }
-    }
-    // ---- scale, mask, online softmax (rows h2 = 0: g4, 1: g4 + 8)
-    uint32_t see[2] = {0xffffffffu, 0xffffffffu};
-    if (msk) {
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        see[h2] = ta_see32(p, row[h2], q0, kabs & ~31) >> (kabs & 31);
-        static_assert(KW <= 32, "a warp's keys lie in one aligned word");
-      }
-    }
-    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int nt = 0; nt < NKT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = F8 ? 16 * (nt >> 1) + 4 * tq + 2 * (nt & 1) + (e & 1) : nt * 8 + 2 * tq + (e & 1);
-        float v = s[nt][e] * p.scale_log2;
-        if (msk) v = (see[e >> 1] >> key) & 1u ? v : -INFINITY;
-        s[nt][e] = v;
-        mx[e >> 1] = fmaxf(mx[e >> 1], v);
-      }
-    bool need = false;
-    float mnew[2];
-#pragma unroll
-    for (int h2 = 0; h2 < 2; ++h2) {
-      mx[h2] = fmaxf(mx[h2], __shfl_xor_sync(0xffffffffu, mx[h2], 1));
-      mx[h2] = fmaxf(mx[h2], __shfl_xor_sync(0xffffffffu, mx[h2], 2));
-      mnew[h2] = fmaxf(m[h2], mx[h2]);
-      need |= mnew[h2] > m[h2] + 8.f;
-    }
-    // the maximum moves only when it grows by more than 2^8: P stays below 2^8, and O is rarely rescaled
-    if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        const bool up = mnew[h2] > m[h2] + 8.f;
-        const float f = up ? ta_ex2(m[h2] - mnew[h2]) : 1.f;
-        if (up) m[h2] = mnew[h2];
-        l[h2] *= f;
-#pragma unroll
-        for (int i2 = 0; i2 < DN; ++i2) {
-          o[i2][2 * h2] *= f;
-          o[i2][2 * h2 + 1] *= f;
-        }
-      }
-    }
-    const float mb[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-    uint32_t pa[NKT / 2][4];
-#pragma unroll
-    for (int nt = 0; nt < NKT; ++nt) {
-      float pv[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        pv[e] = ta_ex2(s[nt][e] - mb[e >> 1]);
-        l[e >> 1] += pv[e];
-      }
-      // P is rounded to the MMA's 16-bit type (bf16: half a step of 2^-8); l keeps the 32-bit sum
-      pa[nt >> 1][(nt & 1) * 2 + 0] = F8 ? tm_f16x2(pv[0], pv[1]) : pack_bf16x2(pv[0], pv[1]);
-      pa[nt >> 1][(nt & 1) * 2 + 1] = F8 ? tm_f16x2(pv[2], pv[3]) : pack_bf16x2(pv[2], pv[3]);
-    }
-    // ---- O += P V
-#pragma unroll
-    for (int kk = 0; kk < NKT / 2; ++kk) {
-      if constexpr (F8) {
-#pragma unroll
-        for (int dn = 0; dn < DN; ++dn) {
-          uint32_t b0, b1;
-          tm_e4m3(tm_lds32(vb + tm_f8_off<64>(dn * 8 + g4, key_lo + 16 * kk + 4 * tq)), b0, b1);
-          tm_mma_f16(o[dn], pa[kk], b0, b1);
-        }
-      } else {
-        const int r = key_lo + kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-#pragma unroll
-        for (int dn2 = 0; dn2 < DN / 2; ++dn2) {
-          uint32_t b0, b1, b2, b3;
-          tm_ldsm4_t(tm_piece(vb, r, 2 * dn2 + (lane >> 4)), b0, b1, b2, b3);
-          tm_mma(o[2 * dn2], pa[kk], b0, b1);
-          tm_mma(o[2 * dn2 + 1], pa[kk], b2, b3);
-        }
-      }
-    }
-    fence_proxy_async_smem();   // generic-proxy accesses of the slot before the TMA that refills it
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[slot]);
-  }
-  // ---- merge the key subsets of each m-tile (every copy has landed: the ring is free)
-#pragma unroll
-  for (int h2 = 0; h2 < 2; ++h2) {
-    l[h2] += __shfl_xor_sync(0xffffffffu, l[h2], 1);
-    l[h2] += __shfl_xor_sync(0xffffffffu, l[h2], 2);
-  }
-  asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory");
-  float* co = reinterpret_cast<float*>(ring);             // [CW][16][DV]
-  {
-    float* mine = co + cw * 16 * DV;
-#pragma unroll
-    for (int i = 0; i < DN; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mine[(g4 + (e >> 1) * 8) * DV + i * 8 + 2 * tq + (e & 1)] = o[i][e];
-    if (tq == 0) {
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        cm[cw * 16 + g4 + h2 * 8] = ok ? m[h2] : -INFINITY;
-        cl[cw * 16 + g4 + h2 * 8] = ok ? l[h2] : 0.f;
-      }
-    }
-  }
-  asm volatile("bar.sync 1, %0;" ::"n"(32 * CW) : "memory");
-  constexpr int C4 = DV / 4;
-  for (int idx = ctid; idx < nrows * C4; idx += 32 * CW) {
-    const int r = idx / C4, c = (idx - r * C4) * 4;
-    const int rm = r >> 4, rr = r & 15;
-    float M = -INFINITY;
-#pragma unroll
-    for (int s2 = 0; s2 < NS; ++s2) M = fmaxf(M, cm[(s2 * MT + rm) * 16 + rr]);
-    const float Mb = M == -INFINITY ? 0.f : M;
-    float Ls = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s2 = 0; s2 < NS; ++s2) {
-      const int w = s2 * MT + rm;
-      const float wgt = ta_ex2(cm[w * 16 + rr] - Mb);
-      Ls += wgt * cl[w * 16 + rr];
-      const float4 v = *reinterpret_cast<const float4*>(co + (w * 16 + rr) * DV + c);
-      acc[0] += wgt * v.x;
-      acc[1] += wgt * v.y;
-      acc[2] += wgt * v.z;
-      acc[3] += wgt * v.w;
-    }
-    const int node = ta_node(p, r0 + r), hh = (r0 + r) - node * p.G;
-    const int tok = q0 + node, head = kh * p.G + hh;
-    // the sink joins the denominator only (once: here, or in the merge of the splits)
-    if (p.sinks != nullptr && p.splits == 1 && M != -INFINITY) Ls += ta_ex2(__ldg(p.sinks + head) * LOG2E - M);
-    const float inv = Ls > 0.f || Ls != Ls ? p.out_scale / Ls : 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] *= inv;
-    if (s_bad) {   // rare: non-finite values of masked pages, for the rows that see them
-      const TaRow rw = ta_row(p, q0, n, ctx, node, true);
-      for (int pg = j0; pg < j1; ++pg) {
-        if (!masked(pg)) continue;
-        const int page = __ldg(p.block_table + (size_t)b * p.bt_stride + pg);
-        if (page < 0 || page >= p.num_blocks) continue;
-        for (int k2 = 0; k2 < TA_PAGE; ++k2) {
-          if (!ta_sees(p, rw, q0, pg * TA_PAGE + k2)) continue;
-          for (int e = 0; e < 4; ++e) {
-            const float v = ta_v_at(p, F8, DV, page, kh, k2, c + e);
-            if (!isfinite(v)) acc[e] += v;
-          }
-        }
-      }
-    }
-    if (p.splits == 1) {
-      uint2 pk;
-      pk.x = pack_bf16x2(acc[0], acc[1]);
-      pk.y = pack_bf16x2(acc[2], acc[3]);
-      *reinterpret_cast<uint2*>(p.o + ((size_t)tok * p.Hq + head) * DV + c) = pk;
-    } else {
-      *reinterpret_cast<float4*>(p.ws_o + (((size_t)sp * p.T + tok) * p.Hq + head) * DV + c) =
-          make_float4(acc[0], acc[1], acc[2], acc[3]);
-      if (c == 0)
-        p.ws_lse[((size_t)sp * p.T + tok) * p.Hq + head] = Ls > 0.f || Ls != Ls ? M + __log2f(Ls) : -FLT_MAX;
-    }
-  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -670,9 +201,12 @@ __global__ void __launch_bounds__(TmCfg<D, DV, F8, MT>::THREADS, 1) tree_attn_mm
 //                over S_u's own columns, a thread a row
 // The issuer alternates PV_u(t), S_u(t + 1): S_u's completion (one commit) also tells unit u that
 // PV_u(t) is done, so P and O need no barriers of their own and S and P share columns.
-template <int D_, int DVT_, int BN_, int ROWT_, int SK, int SV>
+template <int D_, int DVT_, int BN_, int ROWT_, int SK, int SV, int NR_ = 0>
 struct TtCfg {
   static constexpr int D = D_, DVT = DVT_, BN = BN_, ROWT = ROWT_;
+  static constexpr int NR = NR_;                       // slots of the raw ring (fp8 caches)
+  static constexpr bool F8 = NR > 0;
+  static constexpr int RAW = BN * D;                   // bytes of an fp8 tile
   static constexpr int Q_BYTES = ROWT * 128 * D * 2;
   static constexpr int K_BYTES = BN * D * 2, V_BYTES = BN * DVT * 2;
   // one ring of SK + SV slots where a K and a V tile are the same size (K0 V0 K1 V1 ..: an odd count
@@ -687,12 +221,13 @@ struct TtCfg {
   // tile t's K (V) slot is filled again before the last of nt tiles
   __device__ static bool k_again(int t, int nt) { return ONE ? 2 * t + NS < 2 * nt : t + SK < nt; }
   __device__ static bool v_again(int t, int nt) { return ONE ? 2 * t + 1 + NS < 2 * nt : t + SV < nt; }
-  static constexpr int BARS = 2 * NS + 10;
-  static constexpr int BYTES = Q_BYTES + RING + BARS * 8 + 16;
+  static constexpr int BARS = 2 * NS + 2 * NR + 10;
+  static constexpr int BYTES = Q_BYTES + RING + NR * RAW + BARS * 8 + 16;
   static constexpr int O_COL = 2 * BN;                 // S0 S1 | O0 O1
+  static constexpr int P_COL = F8 ? BN / 2 : 0;        // P's first column in S's
   static constexpr int COLS = 2 * BN + 2 * DVT <= 256 ? 256 : 512;
   static constexpr int MLD = DVT + 4;                  // ROWT = 1: unit 1's O in shared memory (floats)
-    static constexpr int THREADS = 384;
+  static constexpr int THREADS = F8 ? 512 : 384;
   static_assert(2 * BN + 2 * DVT <= 512, "tensor memory");
   // V(t)'s slot is given back once S of the tile AHEAD of it stands, whose K the producer must have loaded
   // before it comes to wait for that slot
@@ -700,7 +235,7 @@ struct TtCfg {
   static_assert(AHEAD <= (ONE ? NS / 2 : SV), "the ring would wait for itself");
   static_assert(BYTES <= 232448, "shared memory");
   static_assert(ROWT == 2 || 128 * MLD * 4 + 1024 <= RING, "merge buffer");
-  static_assert(D % 64 == 0 && DVT % 64 == 0 && BN % 64 == 0 && SK >= 2 && SV >= 2, "tiles");
+  static_assert(D % 64 == 0 && DVT % 64 == 0 && BN % 64 == 0 && NS >= 3 && (!F8 || (D == DVT && BN == 128 && NR >= 2)), "tiles");
 };
 
 // 16 bytes to shared memory without a register stop; zeros when `there` is false
@@ -725,6 +260,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+template <bool F8>
+__device__ __forceinline__ uint32_t tt_bad(uint32_t w) {   // the halves to clear of a pair in the operand tile
+  return F8 ? ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u)
+            : bad_bf16x2(w);
+}
+
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tk,
                                                                      const __grid_constant__ CUtensorMap tv,
@@ -735,9 +276,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
   extern __shared__ __align__(1024) uint8_t tt_smem[];   // (the swizzle atoms' alignment)
   uint8_t* sQ = tt_smem;
   uint8_t* sK = sQ + C::Q_BYTES;                       // the ring
-  uint64_t* full = reinterpret_cast<uint64_t*>(sK + C::RING);
+  uint8_t* raw = sK + C::RING;                         // fp8 tiles as they lie in the cache
+  uint64_t* full = reinterpret_cast<uint64_t*>(raw + C::NR * C::RAW);
   uint64_t* empty = full + C::NS;
-  uint64_t* q_ready = empty + C::NS;
+  uint64_t* r_full = empty + C::NS;                    // [NR]
+  uint64_t* r_empty = r_full + C::NR;                  // [NR]
+  uint64_t* q_ready = r_empty + C::NR;
   uint64_t* s_full = q_ready + 1;                      // [2]
   uint64_t* p_full = s_full + 2;                       // [2][2] halves of P
   uint64_t* o_done = p_full + 4;                       // [2], and one for an issuer that gives up
@@ -773,7 +317,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
     s_bad = 0;
-    for (int i = 0; i < C::NS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < C::NS; ++i) { mbar_init(&full[i], C::F8 ? 4 : 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < C::NR; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], 4); }
     mbar_init(q_ready, 8);
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&o_done[i], 1); }
     for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
@@ -800,9 +345,29 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         if (pg < 0 || pg > p.num_blocks) pg = p.num_blocks;
         return (pg * p.Hkv + kh) * TA_PAGE;
       };
+      bool ok = true;
       int krow[PPT], vrow[PPT];
 #pragma unroll
       for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(0, sb);
+      if constexpr (C::F8) {   // K0 V0 K1 V1 .. as they lie: K [64 keys][D bytes], V [DV columns][64 keys] a page
+        int in = 0;
+        for (; in < 2 * nt && ok; ++in) {
+          const int slot = in % C::NR, turn = in / C::NR;
+          if ((in & 1) == 0 && in > 0) {
+#pragma unroll
+            for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(in >> 1, sb);
+          }
+          ok = turn == 0 || ta_wait(&r_empty[slot], (turn - 1) & 1, p.status, 150);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&r_full[slot], C::RAW);
+#pragma unroll
+          for (int sb = 0; sb < PPT; ++sb)
+            tma_load_2d(raw + slot * C::RAW + sb * TA_PAGE * D, in & 1 ? &tv : &tk, &r_full[slot], 0,
+                        in & 1 ? krow[sb] / TA_PAGE * DVT : krow[sb]);
+        }
+        if (!ok)   // let the copies in flight land (bounded) before the CTA ends
+          for (int i = max(0, in - C::NR); i < in; ++i) ta_wait(&r_full[i % C::NR], (i / C::NR) & 1, nullptr, 0, 50000000ull);
+      } else {
       int kn = 0, vn = 0;
       auto load = [&](int slot, int turn, int bytes, const CUtensorMap* map, int c0, int cols, const int (&rows)[PPT],
                       int site) {
@@ -816,7 +381,6 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
             tma_load_2d(dst + c * (BN * 128) + sb * (TA_PAGE * 128), map, &full[slot], c0 + c * 64, rows[sb]);
         return true;
       };
-      bool ok = true;
       for (int t = 0; t < nt && ok; ++t) {
         ok = load(C::k_slot(t), C::k_turn(t), C::K_BYTES, &tk, 0, D, krow, 150);
         kn += ok;
@@ -833,11 +397,15 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         for (int t = max(0, kn - C::NS); t < kn; ++t) ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, nullptr, 0, 50000000ull);
         for (int t = max(0, vn - C::NS); t < vn; ++t) ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, nullptr, 0, 50000000ull);
       }
+      }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (elect_one() && nt > 0) {
-      constexpr uint32_t id_s = idesc_bf16_f32(128, BN, 0, 0), id_o = idesc_bf16_f32(128, DVT, 0, 1);
+      // (fp8: f16 operands, type bits 0; V lies [column][key] and is K-major)
+      constexpr uint32_t types = (1u << 7) | (1u << 10);
+      constexpr uint32_t id_s = C::F8 ? idesc_bf16_f32(128, BN, 0, 0) & ~types : idesc_bf16_f32(128, BN, 0, 0);
+      constexpr uint32_t id_o = C::F8 ? idesc_bf16_f32(128, DVT, 0, 0) & ~types : idesc_bf16_f32(128, DVT, 0, 1);
       bool ok = ta_wait(q_ready, 0, p.status, 152);
       auto tile_of = [&](int u, int i) { return ROWT == 2 ? i : 2 * i + u; };   // unit u's i-th tile
       auto wait_k = [&](int t) { return ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, p.status, 153); };
@@ -854,14 +422,19 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       };
       // O_u += P_u V of its i-th tile, the two halves of the keys as P_u gets ready
       auto mma_o = [&](int u, int i) {
-        const uint64_t vd = sdesc_mnmajor_sw128(smem_u32(sK + C::slot_at(C::v_slot(tile_of(u, i)))), BN * 128, 1024);
+        const uint32_t va = smem_u32(sK + C::slot_at(C::v_slot(tile_of(u, i))));
+        const uint64_t vd = C::F8 ? sdesc_kmajor_sw128(va) : sdesc_mnmajor_sw128(va, BN * 128, 1024);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (!ta_wait(&p_full[2 * u + h], i & 1, p.status, 155)) return false;
           tc_fence_after();
 #pragma unroll
-          for (int k = h * (BN / 32); k < (h + 1) * (BN / 32); ++k)
-            mma_f16_ts(tmem + C::O_COL + u * DVT, tmem + u * BN + k * 8, vd + k * 128, id_o, !(i == 0 && k == 0));
+          for (int e = 0; e < BN / 32; ++e) {
+            const int k = (h ^ C::F8) * (BN / 32) + e;                 // fp8: the second half of the keys first
+            mma_f16_ts(tmem + C::O_COL + u * DVT, tmem + u * BN + C::P_COL + k * 8,
+                       vd + (C::F8 ? ((k >> 2) * (DVT * 128) + (k & 3) * 32) / 16 : k * 128), id_o,
+                       !(i == 0 && h == 0 && e == 0));
+          }
         }
         return true;
       };
@@ -914,6 +487,44 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         if (t >= ahead && C::v_again(t - ahead, nt)) mbar_arrive(&empty[C::v_slot(t - ahead)]);
       }
     }
+  } else if (C::F8 && warp >= 12) {
+    // ------------------------------------------------------------ fp8 -> f16 (exact), swizzled operand tiles
+    if constexpr (C::F8) {
+      const int ct = threadIdx.x - 384;
+      bool ok = true;
+      for (int in = 0; in < 2 * nt && ok; ++in) {
+        const int rs = in % C::NR, t = in >> 1;
+        const bool isv = in & 1;
+        const int slot = isv ? C::v_slot(t) : C::k_slot(t), turn = isv ? C::v_turn(t) : C::k_turn(t);
+        ok = ta_wait(&r_full[rs], (in / C::NR) & 1, p.status, 162) &&
+             (turn == 0 || ta_wait(&empty[slot], (turn - 1) & 1, p.status, 163));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint4* from = reinterpret_cast<const uint4*>(raw + rs * C::RAW);
+        uint8_t* to = sK + C::slot_at(slot);
+#pragma unroll
+        for (int i = ct; i < C::RAW / 16; i += 128) {
+          const uint4 v = from[i];
+          uint4 a, c;
+          tm_e4m3(v.x, a.x, a.y);
+          tm_e4m3(v.y, a.z, a.w);
+          tm_e4m3(v.z, c.x, c.y);
+          tm_e4m3(v.w, c.z, c.w);
+          // K: row = key, 16 of its D values; V: row = column of page i / (DVT * 4), 16 of its 64 keys
+          const int row = isv ? (i >> 2) % DVT : i / (D / 16), chunk = isv ? i / (DVT * 4) : i % (D / 16) / 4;
+          uint8_t* line = to + chunk * ((isv ? DVT : BN) * 128) + row * 128;
+          const int pc = (i & 3) * 2;
+          *reinterpret_cast<uint4*>(line + ((pc ^ (row & 7)) << 4)) = a;
+          *reinterpret_cast<uint4*>(line + (((pc + 1) ^ (row & 7)) << 4)) = c;
+        }
+        fence_proxy_async_smem();      // the MMAs read this, and the TMA refills the raw slot
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&full[slot]);
+          mbar_arrive(&r_empty[rs]);
+        }
+      }
+    }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax units
     const int u = (warp - 4) >> 2, qd = warp & 3;
@@ -934,8 +545,18 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         const bool there = gr < rows_all;
         const int nd = there ? ta_node(p, gr) : 0;
         const int hd = there ? gr - nd * p.G : 0;
-        tt_copy16(smem_u32(dst + (pc >> 3) * (128 * 128) + row * 128 + (((pc & 7) ^ (row & 7)) << 4)),
-                  p.q + (long long)(q0 + nd) * p.q_ts + (long long)(kh * p.G + hd) * p.q_hs + pc * 8, there);
+        uint8_t* at = dst + (pc >> 3) * (128 * 128) + row * 128 + (((pc & 7) ^ (row & 7)) << 4);
+        const __nv_bfloat16* from = p.q + (long long)(q0 + nd) * p.q_ts + (long long)(kh * p.G + hd) * p.q_hs + pc * 8;
+        if constexpr (C::F8) {   // rounded to f16 (bf16's 8 bits fit its 11; beyond 65504 infinite)
+          uint4 v = there ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
+          v.x = tm_f16x2(bf16_lo(v.x), bf16_hi(v.x));
+          v.y = tm_f16x2(bf16_lo(v.y), bf16_hi(v.y));
+          v.z = tm_f16x2(bf16_lo(v.z), bf16_hi(v.z));
+          v.w = tm_f16x2(bf16_lo(v.w), bf16_hi(v.w));
+          *reinterpret_cast<uint4*>(at) = v;
+        } else {
+          tt_copy16(smem_u32(at), from, there);
+        }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
@@ -962,7 +583,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
 #pragma unroll 2
         for (int w = r; w < C::V_BYTES / 16; w += 128) {
           const uint4 x = vw[w];
-          const uint4 bad = make_uint4(bad_bf16x2(x.x), bad_bf16x2(x.y), bad_bf16x2(x.z), bad_bf16x2(x.w));
+          const uint4 bad = make_uint4(tt_bad<C::F8>(x.x), tt_bad<C::F8>(x.y), tt_bad<C::F8>(x.z), tt_bad<C::F8>(x.w));
           if (bad.x | bad.y | bad.z | bad.w) {
             s_bad = 1;
             __threadfence_block();                     // the flag before the zeros: the other unit may find only those
@@ -975,24 +596,31 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      uint32_t sv[BN];
+      // HW columns of S in registers at a time: all of them, or with 16 warps' share of the registers (fp8) a half
+      constexpr int HW = C::F8 ? BN / 2 : BN;
+      uint32_t sv[HW];
+      auto fetch = [&](int c0) {
 #pragma unroll
-      for (int c = 0; c < BN; c += 32) tmem_ld32p(s_t + c, sv + c);
-      tmem_wait_ld();
-      if (msk) {
+        for (int c = 0; c < HW; c += 32) tmem_ld32p(s_t + c0 + c, sv + c);
+        tmem_wait_ld();
+        if (!msk) return;
         const TaRow row = ta_row(p, q0, n, ctx, node, valid);
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          const uint32_t see = ta_see32(p, row, q0, at * BN + c);
+        for (int c = 0; c < HW; c += 32) {
+          const uint32_t see = ta_see32(p, row, q0, at * BN + c0 + c);
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (!((see >> e) & 1u)) sv[c + e] = 0xFF800000u;   // -inf
         }
-      }
+      };
       float mx4[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};
 #pragma unroll
-      for (int e = 0; e < BN; e += 2)
-        mx4[(e >> 1) & 3] = fmax3(mx4[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+      for (int c0 = 0; c0 < BN; c0 += HW) {
+        fetch(c0);
+#pragma unroll
+        for (int e = 0; e < HW; e += 2)
+          mx4[(e >> 1) & 3] = fmax3(mx4[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+      }
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       if (mx != -FLT_MAX) mx *= p.scale_log2;
       // the maximum moves only when it grows by more than 2^8: P stays below 2^8, O is rarely rescaled
@@ -1016,22 +644,37 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       const float neg = m == -FLT_MAX ? 0.f : -m;
       const float2 ng2 = make_float2(neg, neg);
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int c = 0; c < BN; c += 32) {
+      auto weigh = [&](int c, int col) {               // registers c .. c + 31 into P's columns col ..
         uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float2 x = fma2(make_float2(__uint_as_float(sv[c + e]), __uint_as_float(sv[c + e + 1])), sc2, ng2);
           const float2 y = make_float2(ta_ex2(x.x), ta_ex2(x.y));
           l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], y);
-          pk[e >> 1] = pack_bf16x2(y.x, y.y);          // P: bf16 (half a step of 2^-8); l keeps the 32-bit sum
+          // P in 16 bits (bf16: half a step of 2^-8, f16: 2^-11); l keeps the 32-bit sum
+          pk[e >> 1] = C::F8 ? tm_f16x2(y.x, y.y) : pack_bf16x2(y.x, y.y);
         }
-        tmem_st16(s_t + c / 2, pk);
-        if ((c + 32) % (BN / 2) == 0) {                // half of P is ready: its product may start
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * u + c / (BN / 2)]);
+        tmem_st16(s_t + C::P_COL + col, pk);
+      };
+      auto hand_over = [&](int h) {                    // half of P is ready: its product may start
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * u + h]);
+      };
+      if constexpr (C::F8) {   // the second half is at hand; P lies over its S, so the first half's still stands
+#pragma unroll
+        for (int c = 0; c < HW; c += 32) weigh(c, (HW + c) / 2);
+        hand_over(0);
+        fetch(0);
+#pragma unroll
+        for (int c = 0; c < HW; c += 32) weigh(c, c / 2);
+        hand_over(1);
+      } else {
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) {
+          weigh(c, c / 2);
+          if ((c + 32) % (BN / 2) == 0) hand_over(c / (BN / 2));
         }
       }
       l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
@@ -1077,7 +720,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     }
     if (ROWT == 2 ? (u == 0 || two) : u == 0) {
       if (p.sinks != nullptr && p.splits == 1 && M != -FLT_MAX && valid) l += ta_ex2(__ldg(p.sinks + head) * LOG2E - M);
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const float inv = l > 0.f || l != l ? p.out_scale / l : 0.f;
       const size_t at = ((size_t)tok * p.Hq + head) * DV + dv0;
       float* wo = p.splits > 1 ? p.ws_o + (size_t)sp * p.T * p.Hq * DV + at : nullptr;
       const float sc0 = scale_own * inv, sc1 = f1 * inv;
@@ -1121,7 +764,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         const TaRow row = ta_row(p, q0, n, ctx, node, valid);
         for (int pg = t0 * PPT; pg < min(t1 * PPT, npages); ++pg)
           if (pg / PPT >= shut || pg / PPT < open)
-            ta_add_bad(p, row, q0, b, kh, pg, DV, dv0, DVT, wo, wo == nullptr ? p.o + at : nullptr);
+            ta_add_bad(p, row, C::F8, q0, b, kh, pg, DV, dv0, DVT, wo, wo == nullptr ? p.o + at : nullptr);
       }
     }
   }
@@ -1240,24 +883,6 @@ int ta_allow(K kern, int bytes, bool (&done)[64]) {
   return 0;
 }
 
-template <int D, int DV, bool F8, int MT>
-int tm_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int tiles, int B, cudaStream_t s) {
-  using C = TmCfg<D, DV, F8, MT>;
-  static bool done[64] = {};
-  if (const int rc = ta_allow(tree_attn_mma_kernel<D, DV, F8, MT>, C::BYTES, done)) return rc;
-  const cudaError_t e = launch_pdl(tree_attn_mma_kernel<D, DV, F8, MT>, dim3(tiles * p.splits, p.Hkv, B),
-                                   dim3(C::THREADS), C::BYTES, s, tk, tv, p);
-  if (e != cudaSuccess) (void)cudaGetLastError();
-  return e == cudaSuccess ? 1 : -(int)e;
-}
-
-template <int D, int DV, bool F8>
-int tm_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int B, cudaStream_t s) {
-  if (rows <= 16) return tm_launch<D, DV, F8, 1>(tk, tv, p, 1, B, s);
-  if (rows <= 32) return tm_launch<D, DV, F8, 2>(tk, tv, p, 1, B, s);
-  return tm_launch<D, DV, F8, 4>(tk, tv, p, (rows + 63) / 64, B, s);
-}
-
 template <class C>
 int tt_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int tiles, int DV, int B,
               cudaStream_t s) {
@@ -1327,11 +952,10 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   CUtensorMap tk, tv;
   int rc;
   if (fp8) {
-    rc = ta_map(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, k_cache, krows, D, TA_PAGE, D,
-                D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    rc = ta_map(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, k_cache, krows, D, TA_PAGE, D, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (rc == 0)
       rc = ta_map(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, v_cache, (uint64_t)num_blocks * Hkv * DV, TA_PAGE, DV,
-                  TA_PAGE, CU_TENSOR_MAP_SWIZZLE_64B);
+                  TA_PAGE, CU_TENSOR_MAP_SWIZZLE_NONE);
   } else {
     rc = ta_map(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, k_cache, krows, D, TA_PAGE, 64, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == 0)
@@ -1341,8 +965,10 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   if (rc) return rc;
   const int rows = max_nodes * p.G;
   int r = -6;   // head sizes not served
-  if (fp8 && D == 64 && DV == 64) r = tm_rows<64, 64, true>(tk, tv, p, rows, B, s);
-  else if (fp8 && D == 128 && DV == 128) r = tm_rows<128, 128, true>(tk, tv, p, rows, B, s);
+  if (fp8 && D == 64 && DV == 64)
+    r = tt_rows<TtCfg<64, 64, 128, 1, 3, 3, 6>, TtCfg<64, 64, 128, 2, 3, 3, 6>>(tk, tv, p, rows, DV, B, s);
+  else if (fp8 && D == 128 && DV == 128)
+    r = tt_rows<TtCfg<128, 128, 128, 1, 2, 2, 4>, TtCfg<128, 128, 128, 2, 2, 1, 4>>(tk, tv, p, rows, DV, B, s);
   else if (fp8) return -6;
   else if (D == 64 && DV == 64)
     r = tt_rows<TtCfg<64, 64, 128, 1, 6, 6>, TtCfg<64, 64, 128, 2, 5, 5>>(tk, tv, p, rows, DV, B, s);

@@ -175,7 +175,7 @@ def tree_attention_ref(q, k_cache, v_cache, meta: TreeMetadata, scale: float, ou
 
 
 @functools.lru_cache(maxsize=4096)
-def tree_splits(num_seqs: int, num_kv_heads: int, rows: int, seen: int, fp8: bool = False, d: int = 128, dv: int = 128,
+def tree_splits(num_seqs: int, num_kv_heads: int, rows: int, seen: int, d: int = 128, dv: int = 128,
                 num_sms: int = 148) -> int:
     """KV splits of a step.  ``rows``: query rows of the largest tree per KV head, ``seen``: keys that a
     sequence attends to.
@@ -184,9 +184,9 @@ def tree_splits(num_seqs: int, num_kv_heads: int, rows: int, seen: int, fp8: boo
     waves * (key tiles per split + 5) + (4 for the merge of the splits), in key tiles: a CTA's start
     and end cost about 9 us and the merge 7, a key tile 1.8 us.  Measured (4 x 14.6K keys, 8 KV
     heads): 732 rows 211 / 172 us at 1 / 3 splits, 192 rows 78 / 84 us at 4 / 9."""
-    tiles = -(-rows // 64) if fp8 else 1 if rows <= 128 else -(-rows // 256)
+    tiles = 1 if rows <= 128 else -(-rows // 256)
     ctas = max(1, tiles * num_kv_heads * num_seqs * (2 if dv == 256 else 1))
-    keys = -(-seen // (128 if d <= 128 and not fp8 else 64))
+    keys = -(-seen // (128 if d <= 128 else 64))
 
     def cost(s):
         return -(-ctas * s // num_sms) * (-(-keys // s) + 5) + (4 if s > 1 else 0)
@@ -271,7 +271,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError("q rows must be contiguous and start on 16-byte boundaries")
     rows = meta.max_nodes * (Hq // Hk)
     seen = min(meta.max_kv_len, window + meta.max_nodes + KV_BLOCK) if window > 0 else meta.max_kv_len
-    splits = meta.num_splits if meta.num_splits > 0 else tree_splits(B, Hk, rows, seen, fp8, D, Dv)
+    splits = meta.num_splits if meta.num_splits > 0 else tree_splits(B, Hk, rows, seen, D, Dv)
     if splits > MAX_SPLITS:
         raise ValueError(f"at most {MAX_SPLITS} splits")
     ws = None
