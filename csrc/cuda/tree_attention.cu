@@ -149,18 +149,18 @@ __device__ __forceinline__ float ta_v_at(const TaParams& p, bool f8, int DV, int
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p.v_raw)[(((size_t)page * p.Hkv + kh) * TA_PAGE + off) * DV + d]);
 }
 
-// a row's output (32-bit partial or bf16 result, columns d0 .. d0 + cols - 1 of V) plus the non-finite
+// a row's output (32-bit partial or bf16 result from column dv0 on; its columns d0 .. d1 - 1) plus the non-finite
 // values of the keys of logical page pg that it sees
 __device__ __noinline__ void ta_add_bad(const TaParams& p, const TaRow& r, bool f8, int q0, int b, int kh, int pg, int DV,
-                                        int d0, int cols, float* wo, __nv_bfloat16* o) {
+                                        int dv0, int d0, int d1, float* wo, __nv_bfloat16* o) {
   const int page = __ldg(p.block_table + (size_t)b * p.bt_stride + pg);
   if (page < 0 || page >= p.num_blocks) return;
 #pragma unroll 1
   for (int k = 0; k < TA_PAGE; ++k) {
     if (!ta_sees(p, r, q0, pg * TA_PAGE + k)) continue;
 #pragma unroll 1
-    for (int d = 0; d < cols; ++d) {
-      const float y = ta_v_at(p, f8, DV, page, kh, k, d0 + d);
+    for (int d = d0; d < d1; ++d) {
+      const float y = ta_v_at(p, f8, DV, page, kh, k, dv0 + d);
       if (isfinite(y)) continue;
       if (wo != nullptr) wo[d] += y;
       else o[d] = __float2bfloat16(__bfloat162float(o[d]) + y);
@@ -206,6 +206,10 @@ struct TtCfg {
   static constexpr int D = D_, DVT = DVT_, BN = BN_, ROWT = ROWT_;
   static constexpr int NR = NR_;                       // slots of the raw ring (fp8 caches)
   static constexpr bool F8 = NR > 0;
+  // ROWT = 1: two accumulators fill the tensor memory at DVT = 128; wider heads share one, with one
+  // running maximum that goes from tile to tile (unit to unit)
+  static constexpr bool SHARE = ROWT == 1 && DVT > 128;
+  static constexpr int NO = SHARE ? 1 : 2;             // accumulators
   static constexpr int RAW = BN * D;                   // bytes of an fp8 tile
   static constexpr int Q_BYTES = ROWT * 128 * D * 2;
   static constexpr int K_BYTES = BN * D * 2, V_BYTES = BN * DVT * 2;
@@ -221,20 +225,20 @@ struct TtCfg {
   // tile t's K (V) slot is filled again before the last of nt tiles
   __device__ static bool k_again(int t, int nt) { return ONE ? 2 * t + NS < 2 * nt : t + SK < nt; }
   __device__ static bool v_again(int t, int nt) { return ONE ? 2 * t + 1 + NS < 2 * nt : t + SV < nt; }
-  static constexpr int BARS = 2 * NS + 2 * NR + 10;
-  static constexpr int BYTES = Q_BYTES + RING + NR * RAW + BARS * 8 + 16;
+  static constexpr int BARS = 2 * NS + 2 * NR + 12;
+  static constexpr int BYTES = Q_BYTES + RING + NR * RAW + BARS * 8 + 16 + (SHARE ? 512 : 0);
   static constexpr int O_COL = 2 * BN;                 // S0 S1 | O0 O1
   static constexpr int P_COL = F8 ? BN / 2 : 0;        // P's first column in S's
-  static constexpr int COLS = 2 * BN + 2 * DVT <= 256 ? 256 : 512;
+  static constexpr int COLS = 2 * BN + NO * DVT <= 256 ? 256 : 512;
   static constexpr int MLD = DVT + 4;                  // ROWT = 1: unit 1's O in shared memory (floats)
   static constexpr int THREADS = F8 ? 512 : 384;
-  static_assert(2 * BN + 2 * DVT <= 512, "tensor memory");
-  // V(t)'s slot is given back once S of the tile AHEAD of it stands, whose K the producer must have loaded
+  static_assert(2 * BN + NO * DVT <= 512, "tensor memory");
+  // ROWT = 2 gives V(t)'s slot back once S of tile t + 1 stands, whose K the producer must have loaded
   // before it comes to wait for that slot
-  static constexpr int AHEAD = ROWT == 2 ? 1 : 2;
-  static_assert(AHEAD <= (ONE ? NS / 2 : SV), "the ring would wait for itself");
+  static_assert(ROWT == 1 || (ONE ? NS / 2 : SV) >= 1, "the ring would wait for itself");
   static_assert(BYTES <= 232448, "shared memory");
-  static_assert(ROWT == 2 || 128 * MLD * 4 + 1024 <= RING, "merge buffer");
+  static_assert(ROWT == 2 || (SHARE ? 0 : 128 * MLD * 4) + 1024 <= RING, "merge buffer");
+  static_assert(!SHARE || !F8, "fp8 heads are 128 wide at most");
   static_assert(D % 64 == 0 && DVT % 64 == 0 && BN % 64 == 0 && NS >= 3 && (!F8 || (D == DVT && BN == 128 && NR >= 2)), "tiles");
 };
 
@@ -285,8 +289,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
   uint64_t* s_full = q_ready + 1;                      // [2]
   uint64_t* p_full = s_full + 2;                       // [2][2] halves of P
   uint64_t* o_done = p_full + 4;                       // [2], and one for an issuer that gives up
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 3);
+  uint64_t* checked = o_done + 3;                      // [2] SHARE: the unit's tile has its maximum in m_row
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(checked + 2);
   int& s_bad = *reinterpret_cast<int*>(tmem_slot + 1);   // a masked tile held a non-finite value
+  float* m_row = reinterpret_cast<float*>(tmem_slot + 2);  // [128] SHARE: the rows' running maximum
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, halves = DV / DVT;
@@ -320,7 +326,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     for (int i = 0; i < C::NS; ++i) { mbar_init(&full[i], C::F8 ? 4 : 1); mbar_init(&empty[i], 1); }
     for (int i = 0; i < C::NR; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], 4); }
     mbar_init(q_ready, 8);
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&o_done[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&o_done[i], 1); mbar_init(&checked[i], 4); }
     for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
     fence_barrier_init();
   }
@@ -431,9 +437,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
 #pragma unroll
           for (int e = 0; e < BN / 32; ++e) {
             const int k = (h ^ C::F8) * (BN / 32) + e;                 // fp8: the second half of the keys first
-            mma_f16_ts(tmem + C::O_COL + u * DVT, tmem + u * BN + C::P_COL + k * 8,
+            mma_f16_ts(tmem + C::O_COL + u % C::NO * DVT, tmem + u * BN + C::P_COL + k * 8,
                        vd + (C::F8 ? ((k >> 2) * (DVT * 128) + (k & 3) * 32) / 16 : k * 128), id_o,
-                       !(i == 0 && h == 0 && e == 0));
+                       !(i == 0 && h == 0 && e == 0 && (!C::SHARE || u == 0)));
           }
         }
         return true;
@@ -454,8 +460,17 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         for (int u = 0; u < 2; ++u) {
           const int nu = u == 0 ? n0 : n1;
           if (i >= nu) continue;
-          if (ROWT == 1 || u == 0) ok = wait_v(tile_of(u, i)) && (i + 1 >= nu || wait_k(tile_of(u, i + 1)));
-          ok = ok && mma_o(u, i);
+          const int t = tile_of(u, i);
+          if (ROWT == 1) {
+            // tiles of one row tile are half as long: PV must not wait for K of the tile after next, and V's
+            // slot goes back by a commit of its own, an S earlier than by the recycler
+            ok = wait_v(t) && mma_o(u, i);
+            if (ok && C::v_again(t, nt)) mma_commit(&empty[C::v_slot(t)]);
+            ok = ok && (i + 1 >= nu || wait_k(tile_of(u, i + 1)));
+          } else {
+            if (u == 0) ok = wait_v(t) && (i + 1 >= nu || wait_k(t + 1));
+            ok = ok && mma_o(u, i);
+          }
           if (!ok) break;
           if (i + 1 < nu) mma_s(u, i + 1);
           else mma_commit(&o_done[u]);
@@ -471,20 +486,19 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ slots back to the producer
-    // A unit's S of a tile stands (s_full): K of that tile is done with, and V of the tile whose PV the
-    // issuer put before it.  With two units on the same tiles the one that is served last
-    // speaks for both.  (Commits of the issuer would do, but a third one under way stops it until
-    // the products are done; a softmax thread's arrivals cost its warp 350 cycles a tile.)
+    // A unit's S of a tile stands (s_full): K of that tile is done with, and with two units on the same
+    // tiles (the one that is served last speaks for both) V of the tile before, whose PV the
+    // issuer put before that S.  (Softmax threads' arrivals cost their warp 350 cycles a tile.)
     if (elect_one()) {
-      constexpr int ahead = C::AHEAD;
       bool ok = true;
       for (int t = 0; t < nt && ok; ++t) {
         const int u = ROWT == 2 ? (two ? 1 : 0) : t & 1;
-        if (!C::k_again(t, nt) && !(t >= ahead && C::v_again(t - ahead, nt))) continue;
+        const bool k = C::k_again(t, nt), v = ROWT == 2 && t > 0 && C::v_again(t - 1, nt);
+        if (!k && !v) continue;
         ok = ta_wait(&s_full[u], (ROWT == 2 ? t : t >> 1) & 1, p.status, 159);
         if (!ok) break;
-        if (C::k_again(t, nt)) mbar_arrive(&empty[C::k_slot(t)]);
-        if (t >= ahead && C::v_again(t - ahead, nt)) mbar_arrive(&empty[C::v_slot(t - ahead)]);
+        if (k) mbar_arrive(&empty[C::k_slot(t)]);
+        if (v) mbar_arrive(&empty[C::v_slot(t - 1)]);
       }
     }
   } else if (C::F8 && warp >= 12) {
@@ -530,9 +544,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     const int u = (warp - 4) >> 2, qd = warp & 3;
     const int r = qd * 32 + lane;                      // row of the tile = TMEM lane
     const int rr = r0 + (ROWT == 2 ? u * 128 : 0) + r;
-    const bool valid = rr < rows_all;
-    const int node = valid ? ta_node(p, rr) : 0, hh = valid ? rr - node * p.G : 0;
-    const int tok = q0 + node, head = kh * p.G + hh;
+    // (worked out where it is needed: kept through the loop it costs registers that the scores need)
+    auto row_here = [&](int x) {
+      asm volatile("" : "+r"(x));
+      return ta_row(p, q0, n, ctx, x < rows_all ? ta_node(p, x) : 0, x < rows_all);
+    };
     {
       // Q, whole rows at a time: D / 8 lanes a row (a thread a row touched 32 lines a load: 5 us).
       // 128B-swizzled K-major chunks of [128 rows][64 columns]
@@ -564,7 +580,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       if (lane == 0) mbar_arrive(q_ready);
     }
     const uint32_t lanes = (uint32_t)(qd * 32) << 16;
-    const uint32_t s_t = tmem + lanes + u * BN, o_t = tmem + lanes + C::O_COL + u * DVT;
+    const uint32_t s_t = tmem + lanes + u * BN, o_t = tmem + lanes + C::O_COL + u % C::NO * DVT;
     float m = -FLT_MAX, l = 0.f;                       // running maximum (log2 units) and sum
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
@@ -604,7 +620,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         for (int c = 0; c < HW; c += 32) tmem_ld32p(s_t + c0 + c, sv + c);
         tmem_wait_ld();
         if (!msk) return;
-        const TaRow row = ta_row(p, q0, n, ctx, node, valid);
+        const TaRow row = row_here(rr);
 #pragma unroll
         for (int c = 0; c < HW; c += 32) {
           const uint32_t see = ta_see32(p, row, q0, at * BN + c0 + c);
@@ -623,13 +639,32 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       }
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       if (mx != -FLT_MAX) mx *= p.scale_log2;
+      if constexpr (C::SHARE) {
+        if (t > 0) {                                   // the maximum that the tile before (the other unit's) left
+          ok = ta_wait(&checked[u ^ 1], (u == 0 ? i - 1 : i) & 1, p.status, 164);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const float m_now = m_row[r];
+          if (m_now != m) {
+            if (m != -FLT_MAX) l *= ta_ex2(m - m_now);
+            m = m_now;
+          }
+        }
+      }
       // the maximum moves only when it grows by more than 2^8: P stays below 2^8, O is rarely rescaled
       const bool raise = mx > m + 8.f;
       const float m_new = raise ? mx : m;
-      const bool rescale = raise && m != -FLT_MAX && i > 0;
+      const bool rescale = raise && m != -FLT_MAX && (C::SHARE ? t : i) > 0;
       if (__any_sync(0xffffffffu, rescale)) {
         const float f = rescale ? ta_ex2(m - m_new) : 1.f;
         l *= f;
+        if constexpr (C::SHARE) {   // PV of the tile before is done once S of the tile after stands (the issuer's order)
+          ok = t + 1 < nt ? ta_wait(&s_full[u ^ 1], ((t + 1) >> 1) & 1, p.status, 165)
+                          : ta_wait(&o_done[u ^ 1], 0, p.status, 166);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+        }
 #pragma unroll 1
         for (int c = 0; c < DVT; c += 16) {
           uint32_t x[16];
@@ -641,6 +676,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         }
       }
       m = m_new;
+      if constexpr (C::SHARE) {
+        m_row[r] = m;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&checked[u]);
+      }
       const float neg = m == -FLT_MAX ? 0.f : -m;
       const float2 ng2 = make_float2(neg, neg);
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -686,9 +726,30 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       have = __all_sync(0xffffffffu, have);
       tc_fence_after();
     }
+    const bool valid = rr < rows_all;
+    const int node = valid ? ta_node(p, rr) : 0, head = kh * p.G + (valid ? rr - node * p.G : 0), tok = q0 + node;
     float M = m, scale_own = 1.f, f1 = 0.f;
     const float* oth = nullptr;
-    if (ROWT == 1) {
+    if constexpr (C::SHARE) {
+      // one accumulator, each unit's part of the sum in its own last maximum; a unit writes half of the columns.
+      // (O is complete once both units' last products are)
+      if (ok && nt > 0 && (two || u == 1)) {
+        have = ta_wait(&o_done[u ^ 1], 0, p.status, 167);
+        have = __all_sync(0xffffffffu, have);
+        tc_fence_after();
+      }
+      float* ml = reinterpret_cast<float*>(sK);                       // [2 units][m, l][128]
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      ml[u * 256 + r] = mine > 0 ? m : -FLT_MAX;
+      ml[u * 256 + 128 + r] = mine > 0 ? l : 0.f;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      M = fmaxf(ml[r], ml[256 + r]);
+      l = 0.f;
+      for (int w = 0; w < 2; ++w) {
+        const float mw = ml[w * 256 + r], lw = ml[w * 256 + 128 + r];
+        l += mw == -FLT_MAX ? (lw != lw ? lw : 0.f) : lw * ta_ex2(mw - M);
+      }
+    } else if (ROWT == 1) {
       // unit 1's rows meet unit 0's in shared memory: with both units done the ring is free
       float* mo = reinterpret_cast<float*>(sK);                       // [128][MLD]
       float* ml = mo + 128 * C::MLD;                                  // [2][128]
@@ -718,14 +779,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         oth = mo + r * C::MLD;
       }
     }
-    if (ROWT == 2 ? (u == 0 || two) : u == 0) {
+    if (ROWT == 2 ? (u == 0 || two) : C::SHARE || u == 0) {
       if (p.sinks != nullptr && p.splits == 1 && M != -FLT_MAX && valid) l += ta_ex2(__ldg(p.sinks + head) * LOG2E - M);
       const float inv = l > 0.f || l != l ? p.out_scale / l : 0.f;
       const size_t at = ((size_t)tok * p.Hq + head) * DV + dv0;
       float* wo = p.splits > 1 ? p.ws_o + (size_t)sp * p.T * p.Hq * DV + at : nullptr;
       const float sc0 = scale_own * inv, sc1 = f1 * inv;
 #pragma unroll 1
-      for (int c = 0; c < DVT; c += 32) {
+      for (int c = C::SHARE ? u * (DVT / 2) : 0; c < (C::SHARE ? (u + 1) * (DVT / 2) : DVT); c += 32) {
         uint32_t x[32];
         if (have) {
           tmem_ld32(o_t + c, x);
@@ -757,14 +818,15 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
           for (int e = 0; e < 8; ++e) d4[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
         }
       }
-      if (wo != nullptr && valid && dv0 == 0)
+      if (wo != nullptr && valid && dv0 == 0 && (!C::SHARE || u == 0))
         p.ws_lse[((size_t)sp * p.T + tok) * p.Hq + head] =
             l > 0.f || l != l ? (M == -FLT_MAX ? 0.f : M) + __log2f(l) : -FLT_MAX;
       if (s_bad && valid) {   // rare: non-finite values of masked tiles, for the rows that see them
-        const TaRow row = ta_row(p, q0, n, ctx, node, valid);
+        const TaRow row = row_here(rr);
         for (int pg = t0 * PPT; pg < min(t1 * PPT, npages); ++pg)
           if (pg / PPT >= shut || pg / PPT < open)
-            ta_add_bad(p, row, C::F8, q0, b, kh, pg, DV, dv0, DVT, wo, wo == nullptr ? p.o + at : nullptr);
+            ta_add_bad(p, row, C::F8, q0, b, kh, pg, DV, dv0, C::SHARE ? u * (DVT / 2) : 0,
+                       C::SHARE ? (u + 1) * (DVT / 2) : DVT, wo, wo == nullptr ? p.o + at : nullptr);
       }
     }
   }
@@ -977,7 +1039,7 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   else if (D == 192 && DV == 128)
     r = tt_rows<TtCfg<192, 128, 64, 1, 4, 4>, TtCfg<192, 128, 64, 2, 3, 3>>(tk, tv, p, rows, DV, B, s);
   else if (D == 256 && DV == 256)
-    r = tt_rows<TtCfg<256, 128, 64, 1, 3, 4>, TtCfg<256, 128, 64, 2, 2, 2>>(tk, tv, p, rows, DV, B, s);
+    r = tt_launch<TtCfg<256, 256, 64, 1, 3, 2>>(tk, tv, p, (rows + 127) / 128, DV, B, s);
   if (r < 0 || splits == 1) return r;
   const int heads = T * Hq;
   const cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((heads + 7) / 8), dim3(256), 0, s,

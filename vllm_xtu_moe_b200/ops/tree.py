@@ -184,8 +184,8 @@ def tree_splits(num_seqs: int, num_kv_heads: int, rows: int, seen: int, d: int =
     waves * (key tiles per split + 5) + (4 for the merge of the splits), in key tiles: a CTA's start
     and end cost about 9 us and the merge 7, a key tile 1.8 us.  Measured (4 x 14.6K keys, 8 KV
     heads): 732 rows 211 / 172 us at 1 / 3 splits, 192 rows 78 / 84 us at 4 / 9."""
-    tiles = 1 if rows <= 128 else -(-rows // 256)
-    ctas = max(1, tiles * num_kv_heads * num_seqs * (2 if dv == 256 else 1))
+    tiles = -(-rows // 128) if dv > 128 else 1 if rows <= 128 else -(-rows // 256)
+    ctas = max(1, tiles * num_kv_heads * num_seqs)
     keys = -(-seen // (128 if d <= 128 else 64))
 
     def cost(s):
