@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
       s.pt[i] = in ? tv_load1(probs + (long long)(q0 + p) * ldp + t) : -1.f;
       if (DRAFT) s.qt[i] = in ? tv_load1(draft + (long long)(q0 + p) * ldq + t) : 0.f;
     }
-    __syncthreads();
   }
+  cl.sync();   // the nodes are there, and so is every CTA whose shared memory rank 0 writes to
   for (bool have_sum = false;;) {
     if (rank == 0 && warp == 0) {
       TvCmd c{};

@@ -51,6 +51,7 @@ struct TaParams {
   float* ws_lse;            // [splits, T, Hq] m + log2(l), -FLT_MAX for an empty one
   const void* v_raw;        // V cache (non-finite values of masked pages)
   int num_blocks;
+  int max_nodes;            // rows of the grid
   XtuStatus* status;
 };
 
@@ -187,20 +188,40 @@ __device__ __forceinline__ uint32_t bad_bf16x2(uint32_t w) {
 }
 
 // ---------------------------------------------------------------------------------------
-// tensor-memory kernel: 128-row tiles
+// the kernel: 128-row tiles, S, P and O in tensor memory
 // ---------------------------------------------------------------------------------------
-// One CTA = ROWT row tiles of 128 query rows of one (sequence, kv head, kv split, DV columns).
-// Two softmax units of 128 threads keep the tensor core busy in turn:
+// One CTA = ROWT row tiles of 128 query rows of one (sequence, kv head, kv split).  Two softmax
+// units of 128 threads, a thread a row, keep the tensor core busy in turn:
 //   ROWT = 2  unit u owns row tile u; every K / V tile serves both
 //   ROWT = 1  both units own the same rows; unit u takes the key tiles t = u (mod 2) with a
-//             maximum, sum and accumulator of its own, and they merge at the end
-//   warp 0       TMA producer: key tiles of BN keys into a K ring and a V ring
+//             maximum, sum and accumulator of its own, and they merge at the end (SHARE: one
+//             accumulator, see there)
+//   warp 0       TMA producer: key tiles of BN keys into a ring (K0 V0 K1 V1 ..)
 //   warp 1       MMA issuer: S_u = Q K^T into TMEM, O_u += P_u V with P_u from TMEM, the units in turn
 //   warp 2       gives the ring's slots back
-//   warps 4-7    unit 0;  warps 8-11 unit 1: S_u -> registers, mask, online softmax, P_u (16 bit)
-//                over S_u's own columns, a thread a row
+//   warps 4-11   units 0 and 1: S_u -> registers, mask, online softmax, P_u (16 bit) over S_u's columns
+//   warps 12-15  fp8 caches: raw e4m3 tiles -> f16 operand tiles (exact)
 // The issuer alternates PV_u(t), S_u(t + 1): S_u's completion (one commit) also tells unit u that
 // PV_u(t) is done, so P and O need no barriers of their own and S and P share columns.
+//
+// What bounds it.  A unit's way from S to the next S (TMEM load, max, 128 ex2, P, 256 + 512 cycles
+// of MMA, and about 900 cycles of hand-overs) is 3300 cycles per 128-key tile while the
+// other unit's runs beside it; the MMAs of both take 2048 of them.  Measured with parts left
+// out: no exponentials -6 %, no softmax at all -8 %, 1/8 of the S products -27 %: the
+// chain, not one pipe.  Variants that were slower: two warps a row with half a row's keys each (266
+// against 227 us, 61-node case), 64-key tiles with S double-buffered (281: an N = 64 MMA costs as
+// much as an N = 128 one), ex2 partly as a cubic on the FMA pipe (no change), the maximum
+// taken between the exponentials (246: registers).
+// 4 sequences x 14.6K keys, 96 / 8 heads of 128 (KV 240 MB, 36 us at the copy rate):
+//   60 rows a KV head (ROWT = 1)    47 us = 0.78 of the copy rate + 6 us merge of 4 splits
+//   192 rows                        66 us + 7;  732 rows 172 us (153 GFLOP, 0.53 of the GEMM rate)
+//   192 rows over the fp8 cache     88 us with the merge: the widening's shared-memory traffic and the
+//                                   chain above, not the 18 us of its bytes
+// Split counts are chosen on the host (ops/tree.py); a CTA's start and end cost about 6 us.
+//
+// Masked pages: a tile that hides a key from some row of the CTA (the tree's own, the last, those a
+// window cuts) is masked bit by bit in S, and V's non-finite values are zeroed in shared memory
+// first, since 0 * NaN would reach every row; the rows that do see such a key get it at the end.
 template <int D_, int DVT_, int BN_, int ROWT_, int SK, int SV, int NR_ = 0>
 struct TtCfg {
   static constexpr int D = D_, DVT = DVT_, BN = BN_, ROWT = ROWT_;
@@ -320,6 +341,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
   const bool two = ROWT == 2 ? r0 + 128 < rows_all : nt > 1;   // unit 1 has work
 
   if (threadIdx.x == 0) {
+    // (nodes that the grid does not cover, keys that the table does not name: cut, and told)
+    if (n > p.max_nodes) report_error(p.status, XTU_ERR_BOUNDS, 245, n);
+    if (L > p.bt_cols * TA_PAGE) report_error(p.status, XTU_ERR_BOUNDS, 246, L);
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
     s_bad = 0;
@@ -468,8 +492,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
             if (ok && C::v_again(t, nt)) mma_commit(&empty[C::v_slot(t)]);
             ok = ok && (i + 1 >= nu || wait_k(tile_of(u, i + 1)));
           } else {
-            if (u == 0) ok = wait_v(t) && (i + 1 >= nu || wait_k(t + 1));
+            // (fp8: K is still being widened when PV may start)
+            if (u == 0) ok = wait_v(t) && (C::F8 || i + 1 >= nu || wait_k(t + 1));
             ok = ok && mma_o(u, i);
+            if (C::F8 && u == 0) ok = ok && (i + 1 >= nu || wait_k(t + 1));
           }
           if (!ok) break;
           if (i + 1 < nu) mma_s(u, i + 1);
@@ -956,7 +982,8 @@ int tt_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, i
   return e == cudaSuccess ? 1 : -(int)e;
 }
 
-// rows: of the largest tree; one row tile, or two that share their K / V tiles
+// rows: of the largest tree.  Up to 128: one row tile, the units on alternate key tiles (47 us at 60 rows,
+// where two row tiles would leave a unit idle: 66); more: two row tiles that share their K / V tiles
 template <class ONE, class TWO>
 int tt_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int DV, int B, cudaStream_t s) {
   if (rows <= 128) return tt_launch<ONE>(tk, tv, p, 1, DV, B, s);
@@ -1009,6 +1036,7 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   p.ws_lse = ws ? ws + (size_t)splits * T * Hq * DV : nullptr;
   p.v_raw = v_cache;
   p.num_blocks = num_blocks;
+  p.max_nodes = max_nodes;
   p.status = reinterpret_cast<XtuStatus*>(status);
   const uint64_t krows = (uint64_t)num_blocks * Hkv * TA_PAGE;
   CUtensorMap tk, tv;
@@ -1030,7 +1058,7 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   if (fp8 && D == 64 && DV == 64)
     r = tt_rows<TtCfg<64, 64, 128, 1, 3, 3, 6>, TtCfg<64, 64, 128, 2, 3, 3, 6>>(tk, tv, p, rows, DV, B, s);
   else if (fp8 && D == 128 && DV == 128)
-    r = tt_rows<TtCfg<128, 128, 128, 1, 2, 2, 4>, TtCfg<128, 128, 128, 2, 2, 1, 4>>(tk, tv, p, rows, DV, B, s);
+    r = tt_rows<TtCfg<128, 128, 128, 1, 2, 2, 4>, TtCfg<128, 128, 128, 2, 2, 2, 2>>(tk, tv, p, rows, DV, B, s);
   else if (fp8) return -6;
   else if (D == 64 && DV == 64)
     r = tt_rows<TtCfg<64, 64, 128, 1, 6, 6>, TtCfg<64, 64, 128, 2, 5, 5>>(tk, tv, p, rows, DV, B, s);

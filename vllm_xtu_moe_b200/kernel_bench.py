@@ -666,6 +666,54 @@ def bench_cpu_bridge(layers=46, T=1, E=8, H=4096, I=256, K=2, reps=20) -> dict:
     return {"op": "cpu_bridge_round_trip", "shape": dict(layers=layers, T=T, E=E, H=H, I=I, K=K), **res}
 
 
+def bench_tree(Bn=4, ctx=14600, nodes=16, Hq=96, Hkv=8, D=128, kv_dtype="bf16", layers=46, V=151552, iters=20) -> list:
+    """The calls of one speculative step over trees of ``nodes`` drafted tokens: mask, attention of one
+    layer, sampled verification, cache commit of ``layers`` layers (64 cache blocks each)."""
+    from .ops import tree as TR
+    g = torch.Generator(device="cuda").manual_seed(0)
+    T = Bn * nodes
+    i = torch.arange(nodes, dtype=torch.int32, device="cuda")
+    par = torch.where(i > 0, (i - 1) // 2, -1).to(torch.int32).repeat(Bn)          # binary trees
+    qs = torch.arange(0, T + 1, nodes, dtype=torch.int32, device="cuda")
+    nb = (ctx + nodes + 63) // 64
+    fp8 = kv_dtype == "fp8"
+    t = torch.float8_e4m3fn if fp8 else torch.bfloat16
+    k = torch.randn(Bn * nb, Hkv, 64, D, device="cuda", generator=g).to(t)
+    v = torch.randn(*((Bn * nb, Hkv, D, 64) if fp8 else (Bn * nb, Hkv, 64, D)), device="cuda", generator=g).to(t)
+    q = torch.randn(T, Hq, D, device="cuda", generator=g).to(torch.bfloat16)
+    mask, depth = TR.tree_mask(par, qs, nodes)
+    meta = TR.TreeMetadata(num_seqs=Bn, q_start=qs, kv_len=torch.full((Bn,), ctx + nodes, dtype=torch.int32, device="cuda"),
+                           block_table=torch.arange(Bn * nb, dtype=torch.int32, device="cuda").view(Bn, nb), mask=mask,
+                           depth=depth, max_nodes=nodes, max_kv_len=ctx + nodes)
+    probs = torch.softmax(torch.randn(T, V, device="cuda", generator=g), -1)
+    toks = torch.randint(0, V, (T,), device="cuda", generator=g, dtype=torch.int32)
+    u, ud = torch.rand(T, device="cuda", generator=g), torch.rand(Bn, device="cuda", generator=g)
+    kc = torch.zeros(layers, 64, Hkv, 64, D, dtype=t, device="cuda")
+    vc = torch.zeros(*((layers, 64, Hkv, D, 64) if fp8 else (layers, 64, Hkv, 64, D)), dtype=t, device="cuda")
+    path = torch.full((Bn, nodes), -1, dtype=torch.int32, device="cuda")
+    down = [0]
+    while 2 * down[-1] + 2 < nodes:      # the right-most branch: every accepted node moves
+        down.append(2 * down[-1] + 2)
+    path[:, :len(down)] = torch.tensor(down, dtype=torch.int32, device="cuda")
+    acc = torch.full((Bn,), len(down) - 1, dtype=torch.int32, device="cuda")
+    kl = torch.full((Bn,), 40 + nodes, dtype=torch.int32, device="cuda")
+    bt = torch.arange(64, dtype=torch.int32, device="cuda").view(1, 64)[:, :16 * 4].repeat(Bn, 1)
+    bt = torch.stack([torch.roll(bt[b], -(b * 64 // max(1, Bn))) for b in range(Bn)]).contiguous()
+    size = 1 if fp8 else 2
+    shape = dict(B=Bn, ctx=ctx, nodes=nodes, Hq=Hq, Hkv=Hkv, D=D, kv=kv_dtype)
+    words = mask.shape[1]
+    return [
+        _report("tree_mask", shape, time_fn(lambda: TR.tree_mask(par, qs, nodes, mask, depth), iters),
+                T * 4.0 * (2 + words), 0),
+        _report("tree_attention", shape, time_fn(lambda: TR.tree_attention(q, k, v, meta), iters),
+                Bn * (ctx + nodes) * Hkv * 2.0 * D * size + T * Hq * D * 4.0, 4.0 * T * Hq * (ctx + nodes / 4) * D),
+        _report("verify_tree", dict(shape, V=V), time_fn(lambda: TR.verify_tree(probs, toks, par, qs, nodes, u, ud), iters),
+                Bn * V * 4.0 + T * 24.0, Bn * V * 1.0),
+        _report("commit_tree", dict(shape, layers=layers),
+                time_fn(lambda: TR.commit_tree(kc, vc, path, acc, qs, kl, bt), iters),
+                2.0 * Bn * (len(down) - 1) * layers * Hkv * 2 * D * size, 0)]
+
+
 OPS = {
     "moe_prefill_fp8": lambda a: bench_moe(a.tokens or 8192, "fp8"),
     "moe_prefill_bf16": lambda a: bench_moe(a.tokens or 8192, "bf16"),
@@ -680,6 +728,9 @@ OPS = {
     "attention_decode": lambda a: [bench_attn_decode(ql=ql, kv_dtype=kd) for kd in ("bf16", "fp8") for ql in (1, 5)],
     # MTP k=4 verification shape (5 rows per sequence) at several split-KV factors
     "attention_verify": lambda a: [bench_attn_decode(ql=5, splits=sp) for sp in (4, 8, 9, 16, 18)],
+    # a speculative step over trees of drafted tokens
+    "tree_step": lambda a: [r for kd, n in (("bf16", 16), ("bf16", 61), ("fp8", 16))
+                            for r in bench_tree(kv_dtype=kd, nodes=a.tokens or n)],
     "mla_decode": lambda a: bench_mla_decode(),
     "attention_prefill": lambda a: bench_attn_prefill(min(a.tokens or 8192, 16384)),
     "rmsnorm": lambda a: bench_rmsnorm(),
