@@ -982,11 +982,14 @@ int tt_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, i
   return e == cudaSuccess ? 1 : -(int)e;
 }
 
-// rows: of the largest tree.  Up to 128: one row tile, the units on alternate key tiles (47 us at 60 rows,
-// where two row tiles would leave a unit idle: 66); more: two row tiles that share their K / V tiles
+// rows: of the largest tree.  row_tiles = 2: two row tiles a CTA that share their K / V tiles (732 rows:
+// 182 us against 197 with one a CTA); 1: one, the units on alternate key tiles (60 rows, 2 splits: 74 us
+// against 109 with an idle unit; 312 rows of a 128-key window: 18.6 against 24.6, twice the
+// CTAs).  The host weighs them (ops/tree.py).
 template <class ONE, class TWO>
-int tt_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int DV, int B, cudaStream_t s) {
-  if (rows <= 128) return tt_launch<ONE>(tk, tv, p, 1, DV, B, s);
+int tt_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int row_tiles, int DV, int B,
+            cudaStream_t s) {
+  if (row_tiles == 1) return tt_launch<ONE>(tk, tv, p, (rows + 127) / 128, DV, B, s);
   return tt_launch<TWO>(tk, tv, p, (rows + 255) / 256, DV, B, s);
 }
 
@@ -999,15 +1002,16 @@ extern "C" {
 
 // q [T, Hq, D] (strides q_ts, q_hs), caches [num_blocks, Hkv, 64, D | DV] bf16, or fp8 K
 // [num_blocks, Hkv, 64, D] and V [num_blocks, Hkv, DV, 64]; o [T, Hq, DV] bf16.  ws: splits *
-// T * Hq * (DV + 2) floats when splits > 1 (<= 64).  Returns the launches, < 0 on error.
+// T * Hq * (DV + 2) floats when splits > 1 (<= 64).  row_tiles: 128-row tiles of a CTA (1 or 2; heads of 256
+// always 1).  Returns the launches, < 0 on error.
 int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_cache, const void* v_cache, int fp8,
                        void* o, const int* q_start, const int* kv_len, const int* block_table, int bt_stride,
                        int bt_cols, const int* mask, int W, const int* depth, int window, int B, int max_nodes, int T,
                        int Hq, int Hkv, int D, int DV, int num_blocks, float scale, float k_scale, float v_scale,
-                       const float* sinks, int splits, float* ws, void* status, cudaStream_t s) {
+                       const float* sinks, int row_tiles, int splits, float* ws, void* status, cudaStream_t s) {
   if (B <= 0 || T <= 0 || max_nodes <= 0) return 0;
   if (Hkv <= 0 || Hq % Hkv != 0 || B > 65535 || Hkv > 65535 || W <= 0) return -2;
-  if (splits < 1 || splits > 64 || (splits > 1 && ws == nullptr)) return -3;
+  if (row_tiles < 1 || row_tiles > 2 || splits < 1 || splits > 64 || (splits > 1 && ws == nullptr)) return -3;
   if (window > 0 && depth == nullptr) return -4;
   TaParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -1056,16 +1060,16 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   const int rows = max_nodes * p.G;
   int r = -6;   // head sizes not served
   if (fp8 && D == 64 && DV == 64)
-    r = tt_rows<TtCfg<64, 64, 128, 1, 3, 3, 6>, TtCfg<64, 64, 128, 2, 3, 3, 6>>(tk, tv, p, rows, DV, B, s);
+    r = tt_rows<TtCfg<64, 64, 128, 1, 3, 3, 6>, TtCfg<64, 64, 128, 2, 3, 3, 6>>(tk, tv, p, rows, row_tiles, DV, B, s);
   else if (fp8 && D == 128 && DV == 128)
-    r = tt_rows<TtCfg<128, 128, 128, 1, 2, 2, 4>, TtCfg<128, 128, 128, 2, 2, 2, 2>>(tk, tv, p, rows, DV, B, s);
+    r = tt_rows<TtCfg<128, 128, 128, 1, 2, 2, 4>, TtCfg<128, 128, 128, 2, 2, 2, 2>>(tk, tv, p, rows, row_tiles, DV, B, s);
   else if (fp8) return -6;
   else if (D == 64 && DV == 64)
-    r = tt_rows<TtCfg<64, 64, 128, 1, 6, 6>, TtCfg<64, 64, 128, 2, 5, 5>>(tk, tv, p, rows, DV, B, s);
+    r = tt_rows<TtCfg<64, 64, 128, 1, 6, 6>, TtCfg<64, 64, 128, 2, 5, 5>>(tk, tv, p, rows, row_tiles, DV, B, s);
   else if (D == 128 && DV == 128)
-    r = tt_rows<TtCfg<128, 128, 128, 1, 3, 3>, TtCfg<128, 128, 128, 2, 3, 2>>(tk, tv, p, rows, DV, B, s);
+    r = tt_rows<TtCfg<128, 128, 128, 1, 3, 3>, TtCfg<128, 128, 128, 2, 3, 2>>(tk, tv, p, rows, row_tiles, DV, B, s);
   else if (D == 192 && DV == 128)
-    r = tt_rows<TtCfg<192, 128, 64, 1, 4, 4>, TtCfg<192, 128, 64, 2, 3, 3>>(tk, tv, p, rows, DV, B, s);
+    r = tt_rows<TtCfg<192, 128, 64, 1, 4, 4>, TtCfg<192, 128, 64, 2, 3, 3>>(tk, tv, p, rows, row_tiles, DV, B, s);
   else if (D == 256 && DV == 256)
     r = tt_launch<TtCfg<256, 256, 64, 1, 3, 2>>(tk, tv, p, (rows + 127) / 128, DV, B, s);
   if (r < 0 || splits == 1) return r;

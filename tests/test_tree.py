@@ -185,6 +185,18 @@ TREES = [([1], [0]), ([1, 1], [1, 200]), ([5], [0]), ([7, 1, 12], [63, 64, 65]),
          ([61, 17], [130, 1000])]
 
 
+def test_plan():
+    """Every size gets a plan within the kernels' limits; a given split count stays."""
+    for B in (1, 3, 64, 2000):
+        for rows in (1, 128, 129, 5000):
+            for seen in (0, 1, 700, 10 ** 6):
+                for d, dv in tree.HEAD_DIMS:
+                    t, s = tree.tree_plan(B, 8, rows, seen, d, dv)
+                    assert t in (1, 2) and 1 <= s <= tree.MAX_SPLITS and (t == 1 or (rows > 128 and dv <= 128))
+                    assert tree.tree_plan(B, 8, rows, seen, d, dv, 5)[1] == 5
+    assert tree.tree_plan(4, 8, 732, 14817) == (2, 3) and tree.tree_plan(8, 8, 208, 218, 192, 128)[0] == 1
+
+
 @pytest.mark.parametrize("trees", TREES[:5])
 def test_attention_cpu(trees):
     s = make_attention(4, 2, 64, 64, *trees, seed=2)
@@ -194,14 +206,17 @@ def test_attention_cpu(trees):
 @pytest.mark.gpu
 @pytest.mark.parametrize("trees", TREES)
 @pytest.mark.parametrize("shape", SHAPES)
-def test_attention(shape, trees):
+def test_attention(shape, trees, monkeypatch):
     Hq, Hk, D, Dv, fp8 = shape
     s = make_attention(Hq, Hk, D, Dv, *trees, fp8=fp8, seed=3, device="cuda")
     o, a = attention_oracle(s)
     check_attention(s, run_attention(s), o, a)
+    plan = tree.tree_plan
     for splits in (1, 3, 64):                     # more splits than pages leaves empty ones
         s["meta"].num_splits = splits
-        check_attention(s, run_attention(s), o, a)
+        for tiles in (1, 2) if Dv <= 128 else (1,):
+            monkeypatch.setattr(tree, "tree_plan", lambda *a: (tiles, plan(*a)[1]))
+            check_attention(s, run_attention(s), o, a)
     N.check_status()
 
 

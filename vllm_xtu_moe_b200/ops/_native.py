@@ -72,8 +72,8 @@ _SIGS: dict[str, list] = {
                             c_float, c_float, c_float, P, c_int, P, P],
     "xtu_tree_mask": [P, P, c_int, c_int, c_int, P, P, P, P],
     "xtu_tree_attention": [P, c_longlong, c_int, P, P, c_int, P, P, P, P, c_int, c_int, P, c_int, P, c_int, c_int,
-                           c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_float, P, c_int, P, P,
-                           P],
+                           c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_float, P, c_int, c_int, P,
+                           P, P],
     "xtu_tree_verify_greedy": [P, P, P, P, c_int, c_int, P, P, P, P, P, P],
     "xtu_tree_verify": [P, c_longlong, P, c_longlong, c_int, c_int, P, P, P, P, P, c_int, c_int, P, P, P, P, P, P],
     "xtu_tree_commit": [P, P, c_longlong, c_longlong, c_longlong, c_longlong, c_int, P, c_int, P, P, P, P, c_int,

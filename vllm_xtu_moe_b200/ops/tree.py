@@ -175,22 +175,25 @@ def tree_attention_ref(q, k_cache, v_cache, meta: TreeMetadata, scale: float, ou
 
 
 @functools.lru_cache(maxsize=4096)
-def tree_splits(num_seqs: int, num_kv_heads: int, rows: int, seen: int, d: int = 128, dv: int = 128,
-                num_sms: int = 148) -> int:
-    """KV splits of a step.  ``rows``: query rows of the largest tree per KV head, ``seen``: keys that a
-    sequence attends to.
+def tree_plan(num_seqs: int, num_kv_heads: int, rows: int, seen: int, d: int = 128, dv: int = 128, splits: int = 0,
+              num_sms: int = 148) -> tuple[int, int]:
+    """(row tiles of a CTA, KV splits) of a step.  ``rows``: query rows of the largest tree per KV head,
+    ``seen``: keys that a sequence attends to, ``splits``: a split count that is given.
 
-    One CTA per SM takes a row tile of a (sequence, KV head, split), so the time is about
-    waves * (key tiles per split + 5) + (4 for the merge of the splits), in key tiles: a CTA's start
-    and end cost about 9 us and the merge 7, a key tile 1.8 us.  Measured (4 x 14.6K keys, 8 KV
-    heads): 732 rows 211 / 172 us at 1 / 3 splits, 192 rows 78 / 84 us at 4 / 9."""
-    tiles = -(-rows // 128) if dv > 128 else 1 if rows <= 128 else -(-rows // 256)
-    ctas = max(1, tiles * num_kv_heads * num_seqs)
+    One CTA per SM takes one or two 128-row tiles of a (sequence, KV head, split).  In microseconds a
+    key tile costs about 1.8 for two row tiles and 1.2 for one, a CTA's start and end 9 and the merge
+    of the splits 7, so the time is about waves * (key tiles per split * that + 9) + 7.  Measured (4 x
+    14.6K keys, 8 KV heads): 732 rows, two row tiles 223 / 182 us at 1 / 3 splits, one 197 at 3; 192 rows,
+    two 82 / 86 at 4 / 9 splits, one 80 at 2."""
     keys = -(-seen // (128 if d <= 128 else 64))
-
-    def cost(s):
-        return -(-ctas * s // num_sms) * (-(-keys // s) + 5) + (4 if s > 1 else 0)
-    return min(range(1, max(1, min(MAX_SPLITS, keys)) + 1), key=cost)
+    best = None
+    for tiles in ((1,) if dv > 128 or rows <= 128 else (1, 2)):
+        ctas = max(1, -(-rows // (128 * tiles)) * num_kv_heads * num_seqs)
+        for s in ((splits,) if splits else range(1, max(1, min(MAX_SPLITS, keys)) + 1)):
+            cost = -(-ctas * s // num_sms) * (-(-keys // s) * (1.8 if tiles == 2 else 1.2) + 9) + (7 if s > 1 else 0)
+            if best is None or cost < best[0]:
+                best = (cost, tiles, s)
+    return best[1], best[2]
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta: TreeMetadata,
@@ -271,9 +274,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError("q rows must be contiguous and start on 16-byte boundaries")
     rows = meta.max_nodes * (Hq // Hk)
     seen = min(meta.max_kv_len, window + meta.max_nodes + KV_BLOCK) if window > 0 else meta.max_kv_len
-    splits = meta.num_splits if meta.num_splits > 0 else tree_splits(B, Hk, rows, seen, D, Dv)
-    if splits > MAX_SPLITS:
-        raise ValueError(f"at most {MAX_SPLITS} splits")
+    tiles, splits = tree_plan(B, Hk, rows, seen, D, Dv, meta.num_splits)
+    if not 1 <= splits <= MAX_SPLITS:
+        raise ValueError(f"1 .. {MAX_SPLITS} splits, not {splits}")
     ws = None
     if splits > 1:
         need = splits * T * Hq * (Dv + 2)
@@ -286,7 +289,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     N.call("xtu_tree_attention", q.data_ptr(), q_ts, q_hs, k_cache.data_ptr(), v_cache.data_ptr(),
            int(fp8), out.data_ptr(), meta.q_start.data_ptr(), meta.kv_len.data_ptr(), bt.data_ptr(), bt.stride(0),
            bt.shape[1], meta.mask.data_ptr(), W, N.ptr(meta.depth), int(window), B, meta.max_nodes, T, Hq, Hk, D, Dv,
-           nb, float(scale), float(k_scale), float(v_scale), N.ptr(sinks), splits, N.ptr(ws),
+           nb, float(scale), float(k_scale), float(v_scale), N.ptr(sinks), tiles, splits, N.ptr(ws),
            _status(dev), N.stream_ptr(dev))
     return out
 
