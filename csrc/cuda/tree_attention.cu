@@ -875,12 +875,22 @@ __global__ void __launch_bounds__(256) tree_attn_merge_kernel(const float* __res
   griddep_wait();
   griddep_launch_dependents();
   const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int used = q_start[B] * Hq;            // rows behind the last sequence stay as they are
-  if (w >= min(rows, used) || w < q_start[0] * Hq) return;
+  if (w >= rows) return;
+  // the first four splits' values are fetched beside the log-sum-exps that weigh them (an empty split
+  // wrote no values: what is read in their place is dropped)
+  auto fetch = [&](int s0, int d, float4 (&v)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[k] = s0 + k < splits && d < DV ? __ldg(reinterpret_cast<const float4*>(ws_o + ((size_t)(s0 + k) * rows + w) * DV + d))
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  float4 v[4];
+  fetch(0, lane * 4, v);
   const float sk = sinks != nullptr ? __ldg(sinks + w % Hq) * LOG2E : -FLT_MAX;
   // lane s holds split s (at most 64 splits: two per lane)
   const float a = lane < splits ? __ldg(ws_lse + (size_t)lane * rows + w) : -FLT_MAX;
   const float c = lane + 32 < splits ? __ldg(ws_lse + (size_t)(lane + 32) * rows + w) : -FLT_MAX;
+  if (w >= q_start[B] * Hq || w < q_start[0] * Hq) return;   // rows behind the last sequence stay as they are
   float M = fmaxf(a, c);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
@@ -895,25 +905,18 @@ __global__ void __launch_bounds__(256) tree_attn_merge_kernel(const float* __res
   for (int d0 = 0; d0 < DV; d0 += 128) {
     const int d = d0 + lane * 4;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < splits; s0 += 4) {   // four splits' loads under way at a time
-      float4 v[4];
-      float ws[4];
+    for (int s0 = 0; s0 < splits; s0 += 4) {   // in the order of the splits, four fetched at a time
+      if (d0 + s0 > 0) fetch(s0, d, v);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int s = s0 + k;
         const float ls = __shfl_sync(0xffffffffu, s < 32 ? a : c, s & 31);
-        ws[k] = __shfl_sync(0xffffffffu, s < 32 ? wa : wc, s & 31);
-        const bool there = s < splits && ls != -FLT_MAX && d < DV;   // (an empty split wrote nothing)
-        v[k] = there ? __ldg(reinterpret_cast<const float4*>(ws_o + ((size_t)s * rows + w) * DV + d))
-                     : make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!there) ws[k] = 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        acc[0] += ws[k] * v[k].x;
-        acc[1] += ws[k] * v[k].y;
-        acc[2] += ws[k] * v[k].z;
-        acc[3] += ws[k] * v[k].w;
+        const float ws = __shfl_sync(0xffffffffu, s < 32 ? wa : wc, s & 31);
+        if (s >= splits || ls == -FLT_MAX) continue;
+        acc[0] += ws * v[k].x;
+        acc[1] += ws * v[k].y;
+        acc[2] += ws * v[k].z;
+        acc[3] += ws * v[k].w;
       }
     }
     if (d >= DV) continue;
