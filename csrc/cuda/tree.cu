@@ -141,12 +141,19 @@ __global__ void __launch_bounds__(32) tree_verify_greedy_kernel(
 //
 // Rows of the vocabulary are the traffic (one per sequence, two with q, a pass for every
 // rejection of a drawn child), so a cluster of C CTAs shares a sequence's row: each sums a
-// slice, rank 0 walks the tree and tells the others what to do through their shared
-// memory.  Every decision is rank 0's, so all CTAs meet at the same cluster barriers
-// whatever the inputs hold.  Weights and sums are 64-bit: with 150K terms a 32-bit sum is off
-// by more than many tokens' weight, and the drawn token would depend on the split.
+// slice, and the sums meet in every CTA's shared memory.  The walk runs in all of them on one
+// copy of the nodes (rank 0's, read through shared memory once) and on the same sums in the
+// same order, so they agree on every step and meet at the same cluster barriers whatever the
+// inputs hold or do meanwhile; a walk by rank 0 that told the others took a second barrier a
+// pass (55 against 50 us for 32 trees of 26 nodes).  Weights and sums are 64-bit: with 150K terms a
+// 32-bit sum is off by more than many tokens' weight, and the drawn token would depend on the
+// split.  
+// What bounds it: 32 trees of 26 nodes over a vocabulary of 151552 visit 2.5 nodes each on average,
+// so they load about 97 MB (15 us at the copy rate) in a chain of load, two block barriers and a
+// cluster barrier per pass, 18 clusters at a time: 50 us.  One sequence: 15 us, of which the
+// three dependent loads before the walk are 3.  32-bit arithmetic would take 6 % off.
 struct TvCmd {
-  int op;        // 0 sum the weights, 1 draw here, 2 done
+  int op;        // 0 sum the weights, 1 draw, 2 done
   int row;       // row of probs
   int rej;       // rejected children of it so far
   int owner;     // draw: rank that holds the drawn token
@@ -157,8 +164,8 @@ struct TvCmd {
 
 // Drawn children: a pass for every rejection, so 1024 threads whose registers hold their slices of p and
 // q (20 weights each: a vocabulary of 163840 over 8 CTAs) from pass to pass; measured (32
-// sequences of 26 nodes, V = 151552): 512 threads that read them again 72 us, 1024 that read
-// again 64.  Drafts chosen outright: one pass, 512 threads start sooner (18.4 us against 20.5).
+// sequences of 26 nodes, V = 151552): 50 us, 512 threads at two CTAs an SM that read them again 63.
+// Drafts chosen outright: one pass, 512 threads start sooner (18.4 us against 20.5).
 template <bool DRAFT>
 struct TvCfg {
   static constexpr int THREADS = DRAFT ? 1024 : 512, WARPS = THREADS / 32;
@@ -187,8 +194,10 @@ struct TvShared {
   float u[TREE_MAX_NODES], pt[TREE_MAX_NODES], qt[TREE_MAX_NODES];
   int rejected[TREE_MAX_NODES];       // tokens of the rejected children of the current node
   double zi[TREE_MAX_NODES];          // zi[r]: 1 / (sum of the weights after r rejections)
-  double slice[TV_MAX_C];             // rank 0: the CTAs' sums
+  double slice[2][TV_MAX_C];          // the CTAs' sums, of this pass and the one before
+  int n, q0;
   double warp_sum[TV_MAX_WARPS];
+  float u_draw;
   int found, best;                    // the draw: the first weight past the target, the last positive one
   TvCmd cmd;
 };
@@ -269,46 +278,68 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
   const long long first = (long long)(rank * TV_WARPS + warp) * per;
   const int lo = (int)(first < V ? first : V), hi = (int)(first + per < V ? first + per : V);
 
-  int n = 0, q0 = 0;
-  int cur = 0, from = 1, a = 0, rej = 0;     // rank 0, warp 0: the walk
+  int cur = 0, from = 1, a = 0, rej = 0;     // warp 0: the walk, the same in every CTA
   double gone = 0.0;                         // point mass: probability of the rejected tokens
   double z = 1.0;                            // drawn children: sum of the weights at hand
   bool plain = false;                        // nothing was left: draw from p itself
-  int* pb = path + (size_t)b * P;
-  int* ob = out + (size_t)b * P;
   if (rank == 0) {
-    n = tree_nodes(q_start, b, P, st, 242);
-    q0 = q_start[b];
-    for (int i = tid; i < n; i += TV_THREADS) {
-      const int p = parents[q0 + i], t = tokens[q0 + i];
+    const int nn = tree_nodes(q_start, b, P, st, 242), qq = q_start[b];
+    if (tid == 0) {
+      s.n = nn;
+      s.q0 = qq;
+    }
+    for (int i = tid; i < nn; i += TV_THREADS) {
+      const int p = parents[qq + i], t = tokens[qq + i];
       const bool ok = p >= 0 && p < i;
       s.par[i] = ok ? p : -1;
       s.tok[i] = t;
-      s.u[i] = u_accept[q0 + i];
+      s.u[i] = u_accept[qq + i];
       const bool in = ok && t >= 0 && t < V;   // a token outside the vocabulary is never accepted
-      s.pt[i] = in ? tv_load1(probs + (long long)(q0 + p) * ldp + t) : -1.f;
-      if (DRAFT) s.qt[i] = in ? tv_load1(draft + (long long)(q0 + p) * ldq + t) : 0.f;
+      s.pt[i] = in ? tv_load1(probs + (long long)(qq + p) * ldp + t) : -1.f;
+      s.qt[i] = DRAFT && in ? tv_load1(draft + (long long)(qq + p) * ldq + t) : 0.f;
     }
   }
-  cl.sync();   // the nodes are there, and so is every CTA whose shared memory rank 0 writes to
-  for (bool have_sum = false;;) {
-    if (rank == 0 && warp == 0) {
+  if (tid == 0) s.u_draw = u_draw[b];
+  cl.sync();   // the nodes are there, and so is every CTA whose shared memory the others write to
+  if (rank != 0) {
+    const TvShared* r0 = cl.map_shared_rank(&s, 0);
+    const int nn = r0->n;
+    if (tid == 0) {
+      s.n = nn;
+      s.q0 = r0->q0;
+      s.u_draw = r0->u_draw;
+    }
+    for (int i = tid; i < nn; i += TV_THREADS) {
+      s.par[i] = r0->par[i];
+      s.tok[i] = r0->tok[i];
+      s.u[i] = r0->u[i];
+      s.pt[i] = r0->pt[i];
+      s.qt[i] = r0->qt[i];
+    }
+    __syncthreads();
+  }
+  const int n = s.n, q0 = s.q0;
+  if (n == 0) cl.sync();   // (the others have read rank 0's shared memory before it ends)
+  int* pb = path + (size_t)b * P;
+  int* ob = out + (size_t)b * P;
+  for (int pass = 0;; ++pass) {
+    if (warp == 0) {
+      const bool first = pass == 0;
+      bool have_sum = !first;
       TvCmd c{};
+      double tot = 0.0;
       if (n == 0) {
         c.op = 2;
       } else {
         if (have_sum) {                       // the sum that was asked for
-          double tot = 0.0;
-          for (int r = 0; r < C; ++r) tot += s.slice[r];
-          if (lane == 0) s.zi[rej] = tot > 0.0 ? 1.0 / tot : 1.0;
+          for (int r = 0; r < C; ++r) tot += s.slice[(pass - 1) & 1][r];
           z = tot > 0.0 ? tot : 1.0;
+          if (lane == 0) s.zi[rej] = 1.0 / z;
           __syncwarp();
-          c.op = -1;
         }
-        int next = -1;
         // walk on, unless the sum was that of the final weights (no child left)
         for (;;) {
-          next = plain ? -1 : next_child(s.par, n, from, cur);
+          const int next = plain ? -1 : next_child(s.par, n, from, cur);
           if (next < 0) break;
           from = next + 1;
           const int x = s.tok[next];
@@ -324,8 +355,9 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
             take = !dup && s.pt[next] >= 0.f && (double)s.u[next] * (1.0 - gone) < (double)s.pt[next];
             if (!take && !dup && s.pt[next] > 0.f) gone += (double)s.pt[next];
           }
+          have_sum = false;
           if (take) {
-            if (lane == 0) {
+            if (lane == 0 && rank == 0) {
               ob[a] = x;
               pb[a + 1] = next;
             }
@@ -333,62 +365,43 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
             cur = next;
             rej = 0;
             gone = 0.0;
-            have_sum = false;
             continue;
           }
           if (lane == 0) s.rejected[rej] = x;
           ++rej;
           __syncwarp();
-          have_sum = false;
           if (DRAFT) break;                   // the next test (or the draw) needs the new sum
         }
         c.row = q0 + cur;
         c.rej = plain ? 0 : rej;
-        if (!have_sum) {
-          c.op = 0;
-        } else {                              // the sum of the final weights is known: draw
-          double tot = 0.0;
-          for (int r = 0; r < C; ++r) tot += s.slice[r];
-          if (!(tot > 0.0) && !plain) {       // nothing left of p: the draw is from p itself
-            plain = true;
-            c.op = 0;
-            c.rej = 0;
-          } else {
-            const double t = (double)u_draw[b] * tot;
-            double before = 0.0;
-            int owner = -1, last = 0;
-            double at = 0.0;
-            for (int r = 0; r < C; ++r) {
-              const double x = s.slice[r];
-              if (owner < 0 && x > 0.0 && before + x > t) {
-                owner = r;
-                at = t - before;
-              }
-              if (x > 0.0) last = r;
-              before += x;
+        if (have_sum && !(tot > 0.0) && !plain) {   // nothing left of p: the draw is from p itself
+          plain = true;
+          have_sum = false;
+          c.rej = 0;
+        }
+        if (have_sum) {                       // the sum of the final weights is known: draw
+          const double t = (double)s.u_draw * tot;
+          double before = 0.0, at = 0.0;
+          int owner = -1, last = 0;
+          for (int r = 0; r < C; ++r) {
+            const double x = s.slice[(pass - 1) & 1][r];
+            if (owner < 0 && x > 0.0 && before + x > t) {
+              owner = r;
+              at = t - before;
             }
-            c.op = 1;
-            c.any = owner < 0;
-            c.owner = owner < 0 ? last : owner;
-            c.target = at;
-            c.slot = a;
+            if (x > 0.0) last = r;
+            before += x;
           }
+          c.op = 1;
+          c.any = owner < 0;
+          c.owner = owner < 0 ? last : owner;
+          c.target = at;
+          c.slot = a;
         }
       }
-      have_sum = c.op == 0;
-      // lanes 0 .. C-1 each hand the command to one CTA (the rejected tokens and sums with it)
-      if (lane < C) *cl.map_shared_rank(&s.cmd, lane) = c;
-      if (c.op != 2)
-        for (int r = 1; r < C; ++r)
-          for (int i = lane; i < c.rej; i += 32) {
-            if (DRAFT) {
-              cl.map_shared_rank(s.zi, r)[i] = s.zi[i];
-            } else {
-              cl.map_shared_rank(s.rejected, r)[i] = s.rejected[i];
-            }
-          }
+      if (lane == 0) s.cmd = c;
     }
-    cl.sync();
+    __syncthreads();
     const TvCmd c = s.cmd;
     if (c.op == 2) break;
     TvRow<E, DRAFT> row;
@@ -421,10 +434,9 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
       sum = tv_warp_sum(sum);
       if (lane == 0) s.warp_sum[warp] = sum;
       __syncthreads();
-      if (tid == 0) {
-        double tot = 0.0;
-        for (int w = 0; w < TV_WARPS; ++w) tot += s.warp_sum[w];
-        cl.map_shared_rank(s.slice, 0)[rank] = tot;
+      if (warp == 0) {
+        const double tot = tv_warp_sum(lane < TV_WARPS ? s.warp_sum[lane] : 0.0);
+        if (lane < C) cl.map_shared_rank(&s, lane)->slice[pass & 1][rank] = tot;
       }
       cl.sync();
       continue;
