@@ -147,11 +147,12 @@ __global__ void __launch_bounds__(32) tree_verify_greedy_kernel(
 // inputs hold or do meanwhile; a walk by rank 0 that told the others took a second barrier a
 // pass (55 against 50 us for 32 trees of 26 nodes).  Weights and sums are 64-bit: with 150K terms a
 // 32-bit sum is off by more than many tokens' weight, and the drawn token would depend on the
-// split.  
-// What bounds it: 32 trees of 26 nodes over a vocabulary of 151552 visit 2.5 nodes each on average,
-// so they load about 97 MB (15 us at the copy rate) in a chain of load, two block barriers and a
-// cluster barrier per pass, 18 clusters at a time: 50 us.  One sequence: 15 us, of which the
-// three dependent loads before the walk are 3.  32-bit arithmetic would take 6 % off.
+// split.
+// What bounds it is latency: three dependent loads before the walk (the sequence's bounds, its nodes,
+// their probabilities), then per pass a load of the slice (the first at its node), two block
+// barriers and a cluster barrier, and the search for the drawn token.  One sequence, V = 151552: 17 us
+// cold.  32 trees of 26 nodes: 50 us for the 30 MB that they read (5 us at the copy rate), in two waves:
+// 18 clusters of 8 fit.  32-bit arithmetic would take 6 % off.
 struct TvCmd {
   int op;        // 0 sum the weights, 1 draw, 2 done
   int row;       // row of probs

@@ -212,12 +212,14 @@ __device__ __forceinline__ uint32_t bad_bf16x2(uint32_t w) {
 // against 227 us, 61-node case), 64-key tiles with S double-buffered (281: an N = 64 MMA costs as
 // much as an N = 128 one), ex2 partly as a cubic on the FMA pipe (no change), the maximum
 // taken between the exponentials (246: registers).
-// 4 sequences x 14.6K keys, 96 / 8 heads of 128 (KV 240 MB, 36 us at the copy rate):
-//   60 rows a KV head (ROWT = 1)    47 us = 0.78 of the copy rate + 6 us merge of 4 splits
-//   192 rows                        66 us + 7;  732 rows 172 us (153 GFLOP, 0.53 of the GEMM rate)
-//   192 rows over the fp8 cache     88 us with the merge: the widening's shared-memory traffic and the
-//                                   chain above, not the 18 us of its bytes
-// Split counts are chosen on the host (ops/tree.py); a CTA's start and end cost about 6 us.
+// 4 sequences x 14.6K keys, 96 / 8 heads of 128 (KV 240 MB, 36 us at the copy rate), cold:
+//   60 rows a KV head (ROWT = 1)    46 us, DRAM 63 % of its peak (0.78 of the copy rate) + 4 us merge of 4 splits
+//   192 rows                        75 us + 6;  732 rows 179 us + 11 (153 GFLOP: 0.51 of the GEMM rate, MMA pipe
+//                                   52 % busy, XU 53 %)
+//   192 rows over the fp8 cache     82 us + 6: the same chain, and the second read of S that 128 registers
+//                                   force; its bytes are 18 us
+// 16 sequences of up to 12K keys, 16 / 2 heads of 256: 58 us + 5 (197 MB: 30 us).  A CTA's start and end cost
+// about 6 us, and 9 to 16 us is a call over a few pages.  Split counts: ops/tree.py.
 //
 // Masked pages: a tile that hides a key from some row of the CTA (the tree's own, the last, those a
 // window cuts) is masked bit by bit in S, and V's non-finite values are zeroed in shared memory
