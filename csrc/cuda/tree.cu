@@ -20,11 +20,13 @@ namespace cg = cooperative_groups;
 
 constexpr int TREE_MAX_NODES = 1024;   // nodes of one sequence: the shared arrays below
 
-// rows of sequence b, at most `most`; a longer one is cut and reported (site)
-__device__ __forceinline__ int tree_nodes(const int* q_start, int b, int most, XtuStatus* st, int site) {
-  const int n = q_start[b + 1] - q_start[b];
-  if (n > most) report_error(st, XTU_ERR_BOUNDS, site, n);
-  return n < 0 ? 0 : n > most ? most : n;
+// rows of sequence b, at most `most` (a longer one is cut and reported), none when they lie outside
+// the call's T rows (reported)
+__device__ __forceinline__ int tree_nodes(const int* q_start, int b, int T, int most, XtuStatus* st, int site) {
+  const int q0 = q_start[b], q1 = q_start[b + 1], n = q1 - q0;
+  const bool inside = q0 >= 0 && q0 <= q1 && q1 <= T;
+  if (!inside || n > most) report_error(st, XTU_ERR_BOUNDS, site, inside ? n : q1);
+  return !inside ? 0 : n > most ? most : n;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -33,14 +35,14 @@ __device__ __forceinline__ int tree_nodes(const int* q_start, int b, int most, X
 // parents in shared memory meets the words of the row in falling order and writes each once.
 // Latency bound: the walk is `depth` dependent shared-memory reads.
 __global__ void __launch_bounds__(128) tree_mask_kernel(const int* __restrict__ parents,
-                                                        const int* __restrict__ q_start, int max_nodes, int W,
+                                                        const int* __restrict__ q_start, int T, int max_nodes, int W,
                                                         int* __restrict__ mask, int* __restrict__ depth,
                                                         XtuStatus* st) {
   griddep_wait();
   griddep_launch_dependents();
   __shared__ int par[TREE_MAX_NODES];
   const int b = blockIdx.x;
-  const int n = tree_nodes(q_start, b, max_nodes, st, 240);
+  const int n = tree_nodes(q_start, b, T, max_nodes, st, 248);
   const int q0 = q_start[b];
   const int i0 = blockIdx.y * 128;
   if (i0 >= n) return;
@@ -87,13 +89,13 @@ __device__ __forceinline__ int next_child(const int* par, int n, int from, int c
 // token at the current node, until none is.  One warp per sequence.
 __global__ void __launch_bounds__(32) tree_verify_greedy_kernel(
     const int* __restrict__ target, const int* __restrict__ tokens, const int* __restrict__ parents,
-    const int* __restrict__ q_start, int P, int* __restrict__ accepted, int* __restrict__ path,
+    const int* __restrict__ q_start, int T, int P, int* __restrict__ accepted, int* __restrict__ path,
     int* __restrict__ out, int* __restrict__ last_row, XtuStatus* st) {
   griddep_wait();
   griddep_launch_dependents();
   __shared__ int par[TREE_MAX_NODES], tok[TREE_MAX_NODES], tgt[TREE_MAX_NODES];
   const int b = blockIdx.x, lane = threadIdx.x;
-  const int n = tree_nodes(q_start, b, P, st, 241);
+  const int n = tree_nodes(q_start, b, T, P, st, 249);
   const int q0 = q_start[b];
   for (int i = lane; i < n; i += 32) {
     const int p = parents[q0 + i];
@@ -259,7 +261,7 @@ template <typename E, bool DRAFT>
 __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
     const E* __restrict__ probs, long long ldp, const E* __restrict__ draft, long long ldq, int V, int vec,
     const int* __restrict__ tokens, const int* __restrict__ parents, const int* __restrict__ q_start,
-    const float* __restrict__ u_accept, const float* __restrict__ u_draw, int P, int* __restrict__ accepted,
+    const float* __restrict__ u_accept, const float* __restrict__ u_draw, int T, int P, int* __restrict__ accepted,
     int* __restrict__ path, int* __restrict__ out, int* __restrict__ last_row, XtuStatus* st) {
   griddep_wait();
   griddep_launch_dependents();
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
   double z = 1.0;                            // drawn children: sum of the weights at hand
   bool plain = false;                        // nothing was left: draw from p itself
   if (rank == 0) {
-    const int nn = tree_nodes(q_start, b, P, st, 242), qq = q_start[b];
+    const int nn = tree_nodes(q_start, b, T, P, st, 242), qq = q_start[b];
     if (tid == 0) {
       s.n = nn;
       s.q0 = qq;
@@ -654,7 +656,7 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
 
 template <typename E, bool DRAFT>
 int tv_launch(const void* probs, long long ldp, const void* draft, long long ldq, int V, const int* tokens,
-              const int* parents, const int* q_start, const float* u_accept, const float* u_draw, int B, int P,
+              const int* parents, const int* q_start, const float* u_accept, const float* u_draw, int B, int T, int P,
               int* accepted, int* path, int* out, int* last_row, void* status, cudaStream_t s) {
   // CTAs per sequence: a slice of at least 4096 elements each
   const int C = V <= 4096 ? 1 : V <= 8192 ? 2 : V <= 16384 ? 4 : 8;
@@ -676,7 +678,7 @@ int tv_launch(const void* probs, long long ldp, const void* draft, long long ldq
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_verify_kernel<E, DRAFT>, static_cast<const E*>(probs), ldp,
                                            static_cast<const E*>(draft), ldq, V, (int)vec, tokens, parents, q_start,
-                                           u_accept, u_draw, P, accepted, path, out, last_row,
+                                           u_accept, u_draw, T, P, accepted, path, out, last_row,
                                            reinterpret_cast<XtuStatus*>(status));
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
@@ -693,23 +695,23 @@ using namespace xtu;
 extern "C" {
 
 // parents [T] -> mask [T, W] (W words of 32 nodes) and depth [T]; max_nodes <= 1024, W >= ceil(max_nodes / 32)
-int xtu_tree_mask(const int* parents, const int* q_start, int B, int max_nodes, int W, int* mask, int* depth,
+int xtu_tree_mask(const int* parents, const int* q_start, int B, int T, int max_nodes, int W, int* mask, int* depth,
                   void* status, cudaStream_t s) {
   if (B <= 0 || max_nodes <= 0) return 0;
   if (max_nodes > TREE_MAX_NODES || W * 32 < max_nodes) return -2;
   const cudaError_t e = launch_pdl(tree_mask_kernel, dim3(B, (max_nodes + 127) / 128), dim3(128), 0, s, parents,
-                                   q_start, max_nodes, W, mask, depth, reinterpret_cast<XtuStatus*>(status));
+                                   q_start, T, max_nodes, W, mask, depth, reinterpret_cast<XtuStatus*>(status));
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? 1 : -(int)e;
 }
 
 // accepted [B], path [B, P], out [B, P], last_row [B]; P = the largest tree
-int xtu_tree_verify_greedy(const int* target, const int* tokens, const int* parents, const int* q_start, int B, int P,
-                           int* accepted, int* path, int* out, int* last_row, void* status, cudaStream_t s) {
+int xtu_tree_verify_greedy(const int* target, const int* tokens, const int* parents, const int* q_start, int B, int T,
+                           int P, int* accepted, int* path, int* out, int* last_row, void* status, cudaStream_t s) {
   if (B <= 0 || P <= 0) return 0;
   if (P > TREE_MAX_NODES) return -2;
   const cudaError_t e = launch_pdl(tree_verify_greedy_kernel, dim3(B), dim3(32), 0, s, target, tokens, parents,
-                                   q_start, P, accepted, path, out, last_row, reinterpret_cast<XtuStatus*>(status));
+                                   q_start, T, P, accepted, path, out, last_row, reinterpret_cast<XtuStatus*>(status));
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? 1 : -(int)e;
 }
@@ -717,12 +719,12 @@ int xtu_tree_verify_greedy(const int* target, const int* tokens, const int* pare
 // probs [T, V] (row stride ldp elements), draft the same or null; bf16: both bf16, else fp32
 int xtu_tree_verify(const void* probs, long long ldp, const void* draft, long long ldq, int bf16, int V,
                     const int* tokens, const int* parents, const int* q_start, const float* u_accept,
-                    const float* u_draw, int B, int P, int* accepted, int* path, int* out, int* last_row,
+                    const float* u_draw, int B, int T, int P, int* accepted, int* path, int* out, int* last_row,
                     void* status, cudaStream_t s) {
   if (B <= 0 || P <= 0) return 0;
   if (P > TREE_MAX_NODES || V <= 0 || B > 65535) return -2;
 #define XTU_TV(E, D)                                                                                              \
-  return tv_launch<E, D>(probs, ldp, draft, ldq, V, tokens, parents, q_start, u_accept, u_draw, B, P, accepted, \
+  return tv_launch<E, D>(probs, ldp, draft, ldq, V, tokens, parents, q_start, u_accept, u_draw, B, T, P, accepted, \
                          path, out, last_row, status, s)
   if (bf16) {
     if (draft) XTU_TV(__nv_bfloat16, true);

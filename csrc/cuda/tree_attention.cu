@@ -150,10 +150,10 @@ __device__ __forceinline__ float ta_v_at(const TaParams& p, bool f8, int DV, int
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p.v_raw)[(((size_t)page * p.Hkv + kh) * TA_PAGE + off) * DV + d]);
 }
 
-// a row's output (32-bit partial or bf16 result from column dv0 on; its columns d0 .. d1 - 1) plus the non-finite
+// a row's output (32-bit partial or bf16 result; its columns d0 .. d1 - 1) plus the non-finite
 // values of the keys of logical page pg that it sees
 __device__ __noinline__ void ta_add_bad(const TaParams& p, const TaRow& r, bool f8, int q0, int b, int kh, int pg, int DV,
-                                        int dv0, int d0, int d1, float* wo, __nv_bfloat16* o) {
+                                        int d0, int d1, float* wo, __nv_bfloat16* o) {
   const int page = __ldg(p.block_table + (size_t)b * p.bt_stride + pg);
   if (page < 0 || page >= p.num_blocks) return;
 #pragma unroll 1
@@ -161,7 +161,7 @@ __device__ __noinline__ void ta_add_bad(const TaParams& p, const TaRow& r, bool 
     if (!ta_sees(p, r, q0, pg * TA_PAGE + k)) continue;
 #pragma unroll 1
     for (int d = d0; d < d1; ++d) {
-      const float y = ta_v_at(p, f8, DV, page, kh, k, dv0 + d);
+      const float y = ta_v_at(p, f8, DV, page, kh, k, d);
       if (isfinite(y)) continue;
       if (wo != nullptr) wo[d] += y;
       else o[d] = __float2bfloat16(__bfloat162float(o[d]) + y);
@@ -236,8 +236,8 @@ struct TtCfg {
   static constexpr int RAW = BN * D;                   // bytes of an fp8 tile
   static constexpr int Q_BYTES = ROWT * 128 * D * 2;
   static constexpr int K_BYTES = BN * D * 2, V_BYTES = BN * DVT * 2;
-  // one ring of SK + SV slots where a K and a V tile are the same size (K0 V0 K1 V1 ..: an odd count
-  // halves no lookahead), else a ring each
+  // one ring of SK + SV slots where a K and a V tile are the same size (K0 V0 K1 V1 ..; the count
+  // may be odd), else a ring each
   static constexpr bool ONE = K_BYTES == V_BYTES;
   static constexpr int NS = SK + SV, RING = SK * K_BYTES + SV * V_BYTES;
   __device__ static int k_slot(int t) { return ONE ? 2 * t % NS : t % SK; }
@@ -252,7 +252,7 @@ struct TtCfg {
   static constexpr int BYTES = Q_BYTES + RING + NR * RAW + BARS * 8 + 16 + (SHARE ? 512 : 0);
   static constexpr int O_COL = 2 * BN;                 // S0 S1 | O0 O1
   static constexpr int P_COL = F8 ? BN / 2 : 0;        // P's first column in S's
-  static constexpr int COLS = 2 * BN + NO * DVT <= 256 ? 256 : 512;
+  static constexpr int COLS = 512;                     // (every tiling takes more than 256)
   static constexpr int MLD = DVT + 4;                  // ROWT = 1: unit 1's O in shared memory (floats)
   static constexpr int THREADS = F8 ? 512 : 384;
   static_assert(2 * BN + NO * DVT <= 512, "tensor memory");
@@ -296,7 +296,7 @@ __device__ __forceinline__ uint32_t tt_bad(uint32_t w) {   // the halves to clea
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tk,
                                                                      const __grid_constant__ CUtensorMap tv,
-                                                                     const __grid_constant__ TaParams p, int DV) {
+                                                                     const __grid_constant__ TaParams p) {
   griddep_wait();
   constexpr int D = C::D, DVT = C::DVT, BN = C::BN, ROWT = C::ROWT;
   constexpr int PPT = BN / TA_PAGE;                    // pages of a key tile
@@ -318,16 +318,18 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
   float* m_row = reinterpret_cast<float*>(tmem_slot + 2);  // [128] SHARE: the rows' running maximum
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.z, halves = DV / DVT;
-  const int kh = blockIdx.y / halves, dv0 = (blockIdx.y - kh * halves) * DVT;
+  const int b = blockIdx.z, kh = blockIdx.y;
   // row tiles of one split lie next to each other, so that they meet the same K / V in L2
   const int rt = gridDim.x / p.splits;
   const int sp = blockIdx.x / rt, tile = blockIdx.x - sp * rt;
-  const int q0 = __ldg(p.q_start + b), n = __ldg(p.q_start + b + 1) - q0;
+  const int q0 = __ldg(p.q_start + b), q1 = __ldg(p.q_start + b + 1);
+  const bool inside = q0 >= 0 && q1 <= p.T;            // rows outside the call's tensors: no tree here, and told
+  const int n = inside ? q1 - q0 : 0;
   const int L = __ldg(p.kv_len + b), ctx = L - n;
   const int r0 = tile * (128 * ROWT);
   const int rows_all = n * p.G;
   if (r0 >= rows_all) {                                // uniform: no such row tile here
+    if (!inside && threadIdx.x == 0) report_error(p.status, XTU_ERR_BOUNDS, 247, q1);
     griddep_launch_dependents();
     return;
   }
@@ -400,35 +402,34 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         if (!ok)   // let the copies in flight land (bounded) before the CTA ends
           for (int i = max(0, in - C::NR); i < in; ++i) ta_wait(&r_full[i % C::NR], (i / C::NR) & 1, nullptr, 0, 50000000ull);
       } else {
-      int kn = 0, vn = 0;
-      auto load = [&](int slot, int turn, int bytes, const CUtensorMap* map, int c0, int cols, const int (&rows)[PPT],
-                      int site) {
-        if (turn > 0 && !ta_wait(&empty[slot], (turn - 1) & 1, p.status, site)) return false;
-        mbar_arrive_expect_tx(&full[slot], bytes);
-        uint8_t* dst = sK + C::slot_at(slot);
-#pragma unroll
-        for (int sb = 0; sb < PPT; ++sb)
-#pragma unroll
-          for (int c = 0; c < cols / 64; ++c)
-            tma_load_2d(dst + c * (BN * 128) + sb * (TA_PAGE * 128), map, &full[slot], c0 + c * 64, rows[sb]);
-        return true;
-      };
-      for (int t = 0; t < nt && ok; ++t) {
-        ok = load(C::k_slot(t), C::k_turn(t), C::K_BYTES, &tk, 0, D, krow, 150);
-        kn += ok;
-#pragma unroll
-        for (int sb = 0; sb < PPT; ++sb) vrow[sb] = krow[sb];
-        if (t + 1 < nt) {
-#pragma unroll
-          for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(t + 1, sb);   // under way while V's slot gets free
+        int kn = 0, vn = 0;
+        auto load = [&](int slot, int turn, int bytes, const CUtensorMap* map, int cols, const int (&rows)[PPT], int site) {
+          if (turn > 0 && !ta_wait(&empty[slot], (turn - 1) & 1, p.status, site)) return false;
+          mbar_arrive_expect_tx(&full[slot], bytes);
+          uint8_t* dst = sK + C::slot_at(slot);
+  #pragma unroll
+          for (int sb = 0; sb < PPT; ++sb)
+  #pragma unroll
+            for (int c = 0; c < cols / 64; ++c)
+              tma_load_2d(dst + c * (BN * 128) + sb * (TA_PAGE * 128), map, &full[slot], c * 64, rows[sb]);
+          return true;
+        };
+        for (int t = 0; t < nt && ok; ++t) {
+          ok = load(C::k_slot(t), C::k_turn(t), C::K_BYTES, &tk, D, krow, 150);
+          kn += ok;
+  #pragma unroll
+          for (int sb = 0; sb < PPT; ++sb) vrow[sb] = krow[sb];
+          if (t + 1 < nt) {
+  #pragma unroll
+            for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(t + 1, sb);   // under way while V's slot gets free
+          }
+          ok = ok && load(C::v_slot(t), C::v_turn(t), C::V_BYTES, &tv, DVT, vrow, 151);
+          vn += ok;
         }
-        ok = ok && load(C::v_slot(t), C::v_turn(t), C::V_BYTES, &tv, dv0, DVT, vrow, 151);
-        vn += ok;
-      }
-      if (!ok) {   // let the copies in flight land (bounded) before the CTA ends
-        for (int t = max(0, kn - C::NS); t < kn; ++t) ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, nullptr, 0, 50000000ull);
-        for (int t = max(0, vn - C::NS); t < vn; ++t) ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, nullptr, 0, 50000000ull);
-      }
+        if (!ok) {   // let the copies in flight land (bounded) before the CTA ends
+          for (int t = max(0, kn - C::NS); t < kn; ++t) ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, nullptr, 0, 50000000ull);
+          for (int t = max(0, vn - C::NS); t < vn; ++t) ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, nullptr, 0, 50000000ull);
+        }
       }
     }
   } else if (warp == 1) {
@@ -810,8 +811,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     if (ROWT == 2 ? (u == 0 || two) : C::SHARE || u == 0) {
       if (p.sinks != nullptr && p.splits == 1 && M != -FLT_MAX && valid) l += ta_ex2(__ldg(p.sinks + head) * LOG2E - M);
       const float inv = l > 0.f || l != l ? p.out_scale / l : 0.f;
-      const size_t at = ((size_t)tok * p.Hq + head) * DV + dv0;
-      float* wo = p.splits > 1 ? p.ws_o + (size_t)sp * p.T * p.Hq * DV + at : nullptr;
+      const size_t at = ((size_t)tok * p.Hq + head) * DVT;
+      float* wo = p.splits > 1 ? p.ws_o + (size_t)sp * p.T * p.Hq * DVT + at : nullptr;
       const float sc0 = scale_own * inv, sc1 = f1 * inv;
 #pragma unroll 1
       for (int c = C::SHARE ? u * (DVT / 2) : 0; c < (C::SHARE ? (u + 1) * (DVT / 2) : DVT); c += 32) {
@@ -846,14 +847,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
           for (int e = 0; e < 8; ++e) d4[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
         }
       }
-      if (wo != nullptr && valid && dv0 == 0 && (!C::SHARE || u == 0))
+      if (wo != nullptr && valid && (!C::SHARE || u == 0))
         p.ws_lse[((size_t)sp * p.T + tok) * p.Hq + head] =
             l > 0.f || l != l ? (M == -FLT_MAX ? 0.f : M) + __log2f(l) : -FLT_MAX;
       if (s_bad && valid) {   // rare: non-finite values of masked tiles, for the rows that see them
         const TaRow row = row_here(rr);
         for (int pg = t0 * PPT; pg < min(t1 * PPT, npages); ++pg)
           if (pg / PPT >= shut || pg / PPT < open)
-            ta_add_bad(p, row, C::F8, q0, b, kh, pg, DV, dv0, C::SHARE ? u * (DVT / 2) : 0,
+            ta_add_bad(p, row, C::F8, q0, b, kh, pg, DVT, C::SHARE ? u * (DVT / 2) : 0,
                        C::SHARE ? (u + 1) * (DVT / 2) : DVT, wo, wo == nullptr ? p.o + at : nullptr);
       }
     }
@@ -977,12 +978,11 @@ int ta_allow(K kern, int bytes, bool (&done)[64]) {
 }
 
 template <class C>
-int tt_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int tiles, int DV, int B,
-              cudaStream_t s) {
+int tt_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int tiles, int B, cudaStream_t s) {
   static bool done[64] = {};
   if (const int rc = ta_allow(tree_attn_tc_kernel<C>, C::BYTES, done)) return rc;
-  const cudaError_t e = launch_pdl(tree_attn_tc_kernel<C>, dim3(tiles * p.splits, p.Hkv * (DV / C::DVT), B),
-                                   dim3(C::THREADS), C::BYTES, s, tk, tv, p, DV);
+  const cudaError_t e = launch_pdl(tree_attn_tc_kernel<C>, dim3(tiles * p.splits, p.Hkv, B),
+                                   dim3(C::THREADS), C::BYTES, s, tk, tv, p);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? 1 : -(int)e;
 }
@@ -992,10 +992,10 @@ int tt_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, i
 // against 109 with an idle unit; 312 rows of a 128-key window: 18.6 against 24.6, twice the
 // CTAs).  The host weighs them (ops/tree.py).
 template <class ONE, class TWO>
-int tt_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int row_tiles, int DV, int B,
+int tt_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int row_tiles, int B,
             cudaStream_t s) {
-  if (row_tiles == 1) return tt_launch<ONE>(tk, tv, p, (rows + 127) / 128, DV, B, s);
-  return tt_launch<TWO>(tk, tv, p, (rows + 255) / 256, DV, B, s);
+  if (row_tiles == 1) return tt_launch<ONE>(tk, tv, p, (rows + 127) / 128, B, s);
+  return tt_launch<TWO>(tk, tv, p, (rows + 255) / 256, B, s);
 }
 
 }  // namespace
@@ -1065,18 +1065,18 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   const int rows = max_nodes * p.G;
   int r = -6;   // head sizes not served
   if (fp8 && D == 64 && DV == 64)
-    r = tt_rows<TtCfg<64, 64, 128, 1, 3, 3, 6>, TtCfg<64, 64, 128, 2, 3, 3, 6>>(tk, tv, p, rows, row_tiles, DV, B, s);
+    r = tt_rows<TtCfg<64, 64, 128, 1, 3, 3, 6>, TtCfg<64, 64, 128, 2, 3, 3, 6>>(tk, tv, p, rows, row_tiles, B, s);
   else if (fp8 && D == 128 && DV == 128)
-    r = tt_rows<TtCfg<128, 128, 128, 1, 2, 2, 4>, TtCfg<128, 128, 128, 2, 2, 2, 2>>(tk, tv, p, rows, row_tiles, DV, B, s);
+    r = tt_rows<TtCfg<128, 128, 128, 1, 2, 2, 4>, TtCfg<128, 128, 128, 2, 2, 2, 2>>(tk, tv, p, rows, row_tiles, B, s);
   else if (fp8) return -6;
   else if (D == 64 && DV == 64)
-    r = tt_rows<TtCfg<64, 64, 128, 1, 6, 6>, TtCfg<64, 64, 128, 2, 5, 5>>(tk, tv, p, rows, row_tiles, DV, B, s);
+    r = tt_rows<TtCfg<64, 64, 128, 1, 6, 6>, TtCfg<64, 64, 128, 2, 5, 5>>(tk, tv, p, rows, row_tiles, B, s);
   else if (D == 128 && DV == 128)
-    r = tt_rows<TtCfg<128, 128, 128, 1, 3, 3>, TtCfg<128, 128, 128, 2, 3, 2>>(tk, tv, p, rows, row_tiles, DV, B, s);
+    r = tt_rows<TtCfg<128, 128, 128, 1, 3, 3>, TtCfg<128, 128, 128, 2, 3, 2>>(tk, tv, p, rows, row_tiles, B, s);
   else if (D == 192 && DV == 128)
-    r = tt_rows<TtCfg<192, 128, 64, 1, 4, 4>, TtCfg<192, 128, 64, 2, 3, 3>>(tk, tv, p, rows, row_tiles, DV, B, s);
+    r = tt_rows<TtCfg<192, 128, 64, 1, 4, 4>, TtCfg<192, 128, 64, 2, 3, 3>>(tk, tv, p, rows, row_tiles, B, s);
   else if (D == 256 && DV == 256)
-    r = tt_launch<TtCfg<256, 256, 64, 1, 3, 2>>(tk, tv, p, (rows + 127) / 128, DV, B, s);
+    r = tt_launch<TtCfg<256, 256, 64, 1, 3, 2>>(tk, tv, p, (rows + 127) / 128, B, s);
   if (r < 0 || splits == 1) return r;
   const int heads = T * Hq;
   const cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((heads + 7) / 8), dim3(256), 0, s,

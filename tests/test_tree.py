@@ -293,6 +293,19 @@ def test_attention_ignores_what_a_row_does_not_see(shape, splits):
     N.check_status()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_of_a_node_with_an_infinite_value(device):
+    """A node's V that some rows see and others do not."""
+    s = make_attention(2, 1, 64, 64, [12], [3], seed=8, device=device)
+    m = s["meta"]
+    clean = run_attention(s)
+    s["v"][int(m.block_table[0, 0]), :, 3 + 4, 1] = float("inf")
+    out = run_attention(s)
+    sees = torch.tensor([bool(int(m.mask[i, 0]) >> 4 & 1) for i in range(12)])
+    assert 0 < int(sees.sum()) < 12
+    assert torch.equal(out[~sees], clean[~sees]) and bool((out[sees][:, :, 1] == float("inf")).all())
+
+
 @pytest.mark.gpu
 def test_attention_strides_out_and_rows_behind():
     s = make_attention(24, 2, 128, 128, [5, 18], [90, 300], seed=7, device="cuda")
@@ -322,6 +335,15 @@ def test_attention_long_context_large_tree():
     """A long context in shuffled pages against an oracle over all of it."""
     for fp8 in (False, True):
         s = make_attention(12, 1, 128, 128, [64], [9000], fp8=fp8, seed=8, device="cuda")
+        check_attention(s, run_attention(s))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_attention_of_the_largest_tree(fp8):
+    """1024 nodes (32 mask words), several row tiles and heads of both kinds of grouping."""
+    for Hq, Hk, lens in ((2, 1, [1024]), (3, 1, [1000, 1, 130])):
+        s = make_attention(Hq, Hk, 64, 64, lens, [100, 0, 63][:len(lens)], fp8=fp8, seed=12, device="cuda")
         check_attention(s, run_attention(s))
 
 
@@ -852,6 +874,29 @@ def test_refusals_gpu():
     no("16-byte", lambda: tree.tree_attention(torch.zeros(8 * 4 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:]
                                               .view(8, 4, 64), k, v, m))
     no("on cuda", lambda: tree.tree_attention(q, k.cpu(), v.cpu(), m))
+    # sizes that the device finds wrong are told: rows past the tensors, more nodes than max_nodes, keys
+    # past the table
+    import dataclasses
+
+    def told():
+        with pytest.raises(RuntimeError, match="bounds"):
+            N.check_status()
+    for change in (dict(q_start=i32([0, 5, 9], "cuda")), dict(max_nodes=4), dict(block_table=m.block_table[:, :1])):
+        tree.tree_attention(q, k, v, dataclasses.replace(m, **change))
+        told()
+    par, tok = random_trees([5, 3], 2, "cuda")[0], torch.ones(8, dtype=torch.int32, device="cuda")
+    pr, u = torch.full((8, 20), 0.05, device="cuda"), torch.zeros(8, device="cuda")
+    for qs in (i32([0, 5, 9], "cuda"), i32([-1, 3], "cuda"), i32([0, 5, 3], "cuda")):
+        B = len(qs) - 1
+        tree.tree_mask(par, qs, 5)
+        told()
+        v1 = tree.verify_tree_greedy(tok, tok, par, qs, 5)
+        told()
+        v2 = tree.verify_tree(pr, tok, par, qs, 5, u, u[:B])
+        told()
+        for vd in (v1, v2):                      # such a sequence has no nodes
+            assert int(vd.last_row[B - 1]) == -1 and int(vd.accepted[B - 1]) == 0
+            assert bool((vd.path[B - 1] == -1).all()) and bool((vd.tokens[B - 1] == -1).all())
     # a tree larger than max_nodes is cut and reported
     par, qs = random_trees([9], 1, "cuda")
     tree.tree_mask(par, qs, 4)

@@ -70,12 +70,13 @@ _SIGS: dict[str, list] = {
     "xtu_deltanet_spec_commit": [P, P, c_int, c_int, P, P, ctypes.c_longlong, P, P, ctypes.c_longlong, P],
     "xtu_grouped_gemm_ex": [P, P, P, P, c_int, P, c_int, c_int, c_int, c_int, c_int, P, P, c_int, c_int, P, P,
                             c_float, c_float, c_float, P, c_int, P, P],
-    "xtu_tree_mask": [P, P, c_int, c_int, c_int, P, P, P, P],
+    "xtu_tree_mask": [P, P, c_int, c_int, c_int, c_int, P, P, P, P],
     "xtu_tree_attention": [P, c_longlong, c_int, P, P, c_int, P, P, P, P, c_int, c_int, P, c_int, P, c_int, c_int,
                            c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_float, P, c_int, c_int, P,
                            P, P],
-    "xtu_tree_verify_greedy": [P, P, P, P, c_int, c_int, P, P, P, P, P, P],
-    "xtu_tree_verify": [P, c_longlong, P, c_longlong, c_int, c_int, P, P, P, P, P, c_int, c_int, P, P, P, P, P, P],
+    "xtu_tree_verify_greedy": [P, P, P, P, c_int, c_int, c_int, P, P, P, P, P, P],
+    "xtu_tree_verify": [P, c_longlong, P, c_longlong, c_int, c_int, P, P, P, P, P, c_int, c_int, c_int, P, P, P, P, P,
+                        P],
     "xtu_tree_commit": [P, P, c_longlong, c_longlong, c_longlong, c_longlong, c_int, P, c_int, P, P, P, P, c_int,
                         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P],
     "xtu_ipc_handle_size": [],

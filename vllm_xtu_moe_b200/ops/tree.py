@@ -125,7 +125,7 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, max_nodes: int, mask
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return tree_mask(parents, q_start, max_nodes, mask, depth)
-    N.call("xtu_tree_mask", parents.data_ptr(), q_start.data_ptr(), B, max_nodes, W, mask.data_ptr(),
+    N.call("xtu_tree_mask", parents.data_ptr(), q_start.data_ptr(), B, T, max_nodes, W, mask.data_ptr(),
            depth.data_ptr(), _status(dev), N.stream_ptr(dev))
     return mask, depth
 
@@ -152,9 +152,10 @@ def tree_attention_ref(q, k_cache, v_cache, meta: TreeMetadata, scale: float, ou
         tree = (meta.mask[r0:r0 + n].long()[:, node >> 5] >> (node & 31) & 1).bool()            # [i, j]
         see = torch.ones(n, kl[b], dtype=torch.bool, device=q.device)
         if window > 0:
-            far = meta.depth[r0:r0 + n].long().clamp(0, n - 1)[:, None] - window
+            deep = meta.depth[r0:r0 + n].long().clamp(0, n - 1)
+            far = deep[:, None] - window
             see[:, :ctx] = torch.arange(ctx, device=q.device)[None] > ctx + far
-            tree &= meta.depth[r0:r0 + n].long()[None] > far
+            tree &= deep[None] > far
         see[:, ctx:] = tree
         s = torch.einsum("qhd,khd->hqk", q[r0:r0 + n].float(), k) * scale
         s = s.masked_fill(~see[None], float("-inf"))
@@ -167,14 +168,28 @@ def tree_attention_ref(q, k_cache, v_cache, meta: TreeMetadata, scale: float, ou
         z = p.sum(-1, keepdim=True)
         if sinks is not None:
             z = z + torch.exp(sk - m)
-        p = torch.where(see.any(-1)[None, :, None], p / z, 0.0)
-        # a key that no row sees (stale cache contents) must not meet 0 * NaN
-        v = torch.where(see.any(0)[:, None, None], v, 0.0)
-        out[r0:r0 + n] = torch.einsum("hqk,khd->qhd", p, v).to(out.dtype)
+        p = torch.where(z == 0.0, 0.0, p / z)
+        # a key that a row does not see must not reach it as 0 * NaN
+        if torch.isfinite(v).all():
+            o = torch.einsum("hqk,khd->qhd", p, v)
+        else:
+            o = torch.stack([torch.einsum("hk,khd->hd", p[:, i, see[i]], v[see[i]]) for i in range(n)])
+        out[r0:r0 + n] = o.to(out.dtype)
     return out
 
 
 @functools.lru_cache(maxsize=4096)
+def _plan(groups: int, rows: int, keys: int, one: bool, splits: int, num_sms: int) -> tuple[int, int]:
+    best = None
+    for tiles in ((1,) if one or rows <= 128 else (1, 2)):
+        ctas = max(1, -(-rows // (128 * tiles)) * groups)
+        for s in ((splits,) if splits else range(1, max(1, min(MAX_SPLITS, keys)) + 1)):
+            cost = -(-ctas * s // num_sms) * (-(-keys // s) * (1.8 if tiles == 2 else 1.2) + 9) + (7 if s > 1 else 0)
+            if best is None or cost < best[0]:
+                best = (cost, tiles, s)
+    return best[1], best[2]
+
+
 def tree_plan(num_seqs: int, num_kv_heads: int, rows: int, seen: int, d: int = 128, dv: int = 128, splits: int = 0,
               num_sms: int = 148) -> tuple[int, int]:
     """(row tiles of a CTA, KV splits) of a step.  ``rows``: query rows of the largest tree per KV head,
@@ -185,15 +200,7 @@ def tree_plan(num_seqs: int, num_kv_heads: int, rows: int, seen: int, d: int = 1
     of the splits 7, so the time is about waves * (key tiles per split * that + 9) + 7.  Measured (4 x
     14.6K keys, 8 KV heads): 732 rows, two row tiles 223 / 182 us at 1 / 3 splits, one 197 at 3; 192 rows,
     two 82 / 86 at 4 / 9 splits, one 80 at 2."""
-    keys = -(-seen // (128 if d <= 128 else 64))
-    best = None
-    for tiles in ((1,) if dv > 128 or rows <= 128 else (1, 2)):
-        ctas = max(1, -(-rows // (128 * tiles)) * num_kv_heads * num_seqs)
-        for s in ((splits,) if splits else range(1, max(1, min(MAX_SPLITS, keys)) + 1)):
-            cost = -(-ctas * s // num_sms) * (-(-keys // s) * (1.8 if tiles == 2 else 1.2) + 9) + (7 if s > 1 else 0)
-            if best is None or cost < best[0]:
-                best = (cost, tiles, s)
-    return best[1], best[2]
+    return _plan(num_seqs * num_kv_heads, rows, -(-seen // (128 if d <= 128 else 64)), dv > 128, splits, num_sms)
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta: TreeMetadata,
@@ -204,13 +211,14 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
     Node i sees its sequence's context and the nodes of its mask row; with ``window`` > 0 only
     keys at positions above its own minus the window (node j lies at context + ``meta.depth[j]``).
-    ``sinks`` fp32 [Hq]: learned logits in the denominator.  A row that sees nothing is zero.
+    ``sinks`` fp32 [Hq]: learned logits in the denominator.  A row that sees nothing (or only
+    scores of minus infinity) is zero.
     Keys outside a row's view never reach it, whatever the cache holds there; rows behind the
     last sequence are left as they are.
 
     Caches as in :func:`attention.paged_attention`: bf16 ``[blocks, Hkv, 64, D]`` / ``[.., Dv]`` with
-    (D, Dv) in ``HEAD_DIMS``, or fp8 (e4m3) K and per-block transposed V with ``FP8_HEAD_DIMS``.  MLA
-    latent caches are not served.  ``workspace``: fp32, ``splits * T * Hq * (Dv + 2)`` elements when
+    (D, Dv) in ``HEAD_DIMS``, or fp8 (e4m3) K and per-block transposed V with ``FP8_HEAD_DIMS`` (their
+    products take q as fp16: magnitudes up to 65504).  MLA latent caches are not served.  ``workspace``: fp32, ``splits * T * Hq * (Dv + 2)`` elements when
     the KV range is split; allocated when None or too small.  One that is passed in belongs to
     the call until its work is done: calls that may overlap take one each."""
     if q.dim() != 3 or (q.is_cuda and q.dtype is not torch.bfloat16):
@@ -362,7 +370,7 @@ def verify_tree_greedy(target: torch.Tensor, tokens: torch.Tensor, parents: torc
         with torch.cuda.device(dev):
             return verify_tree_greedy(target, tokens, parents, q_start, max_nodes)
     v = _verdict(B, max_nodes, tokens)
-    N.call("xtu_tree_verify_greedy", target.data_ptr(), tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), B,
+    N.call("xtu_tree_verify_greedy", target.data_ptr(), tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), B, T,
            max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
            _status(dev), N.stream_ptr(dev))
     return v
@@ -457,7 +465,7 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     v = _verdict(B, max_nodes, tokens)
     N.call("xtu_tree_verify", probs.data_ptr(), probs.stride(0), N.ptr(draft_probs),
            0 if draft_probs is None else draft_probs.stride(0), int(probs.dtype == torch.bfloat16), probs.shape[1],
-           tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(), B,
+           tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(), B, T,
            max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
            _status(dev), N.stream_ptr(dev))
     return v
