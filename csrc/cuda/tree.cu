@@ -13,6 +13,20 @@
 #include "launch.cuh"
 #include "ptx.cuh"
 
+extern "C" struct XtuTreeVerify {
+  const void* probs;
+  long long ldp;
+  const void* draft;
+  long long ldq;
+  int bf16, V;
+  const int *tokens, *parents, *q_start;
+  const float *u_accept, *u_draw;
+  int B, T, P;
+  int *accepted, *path, *out, *last_row;
+  void* status;
+  cudaStream_t s;
+};
+
 namespace xtu {
 namespace {
 
@@ -655,18 +669,16 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
 }
 
 template <typename E, bool DRAFT>
-int tv_launch(const void* probs, long long ldp, const void* draft, long long ldq, int V, const int* tokens,
-              const int* parents, const int* q_start, const float* u_accept, const float* u_draw, int B, int T, int P,
-              int* accepted, int* path, int* out, int* last_row, void* status, cudaStream_t s) {
+int tv_launch(const XtuTreeVerify& a) {
   // CTAs per sequence: a slice of at least 4096 elements each
-  const int C = V <= 4096 ? 1 : V <= 8192 ? 2 : V <= 16384 ? 4 : 8;
+  const int C = a.V <= 4096 ? 1 : a.V <= 8192 ? 2 : a.V <= 16384 ? 4 : 8;
   constexpr int VE = 16 / sizeof(E);
-  const bool vec = V % VE == 0 && ldp % VE == 0 && (reinterpret_cast<uintptr_t>(probs) & 15) == 0 &&
-                   (!DRAFT || (ldq % VE == 0 && (reinterpret_cast<uintptr_t>(draft) & 15) == 0));
+  const bool vec = a.V % VE == 0 && a.ldp % VE == 0 && (reinterpret_cast<uintptr_t>(a.probs) & 15) == 0 &&
+                   (!DRAFT || (a.ldq % VE == 0 && (reinterpret_cast<uintptr_t>(a.draft) & 15) == 0));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(C, B);
+  cfg.gridDim = dim3(C, a.B);
   cfg.blockDim = dim3(TvCfg<DRAFT>::THREADS);
-  cfg.stream = s;
+  cfg.stream = a.s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = C;
@@ -676,10 +688,11 @@ int tv_launch(const void* probs, long long ldp, const void* draft, long long ldq
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_verify_kernel<E, DRAFT>, static_cast<const E*>(probs), ldp,
-                                           static_cast<const E*>(draft), ldq, V, (int)vec, tokens, parents, q_start,
-                                           u_accept, u_draw, T, P, accepted, path, out, last_row,
-                                           reinterpret_cast<XtuStatus*>(status));
+  const cudaError_t e =
+      cudaLaunchKernelEx(&cfg, tree_verify_kernel<E, DRAFT>, static_cast<const E*>(a.probs), a.ldp,
+                         static_cast<const E*>(a.draft), a.ldq, a.V, (int)vec, a.tokens, a.parents, a.q_start,
+                         a.u_accept, a.u_draw, a.T, a.P, a.accepted, a.path, a.out, a.last_row,
+                         static_cast<XtuStatus*>(a.status));
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return -(int)e;
@@ -694,67 +707,83 @@ using namespace xtu;
 
 extern "C" {
 
+// Each entry takes its arguments as one struct (the binding packs them: ops/_native.py).
+
+struct XtuTreeMask {
+  const int *parents, *q_start;
+  int B, T, max_nodes, W;
+  int *mask, *depth;
+  void* status;
+  cudaStream_t s;
+};
+
 // parents [T] -> mask [T, W] (W words of 32 nodes) and depth [T]; max_nodes <= 1024, W >= ceil(max_nodes / 32)
-int xtu_tree_mask(const int* parents, const int* q_start, int B, int T, int max_nodes, int W, int* mask, int* depth,
-                  void* status, cudaStream_t s) {
-  if (B <= 0 || max_nodes <= 0) return 0;
-  if (max_nodes > TREE_MAX_NODES || W * 32 < max_nodes) return -2;
-  const cudaError_t e = launch_pdl(tree_mask_kernel, dim3(B, (max_nodes + 127) / 128), dim3(128), 0, s, parents,
-                                   q_start, T, max_nodes, W, mask, depth, reinterpret_cast<XtuStatus*>(status));
+int xtu_tree_mask(const XtuTreeMask* a) {
+  if (a->B <= 0 || a->max_nodes <= 0) return 0;
+  if (a->max_nodes > TREE_MAX_NODES || a->W * 32 < a->max_nodes) return -2;
+  const cudaError_t e = launch_pdl(tree_mask_kernel, dim3(a->B, (a->max_nodes + 127) / 128), dim3(128), 0, a->s,
+                                   a->parents, a->q_start, a->T, a->max_nodes, a->W, a->mask, a->depth,
+                                   static_cast<XtuStatus*>(a->status));
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? 1 : -(int)e;
 }
 
+struct XtuTreeVerifyGreedy {
+  const int *target, *tokens, *parents, *q_start;
+  int B, T, P;
+  int *accepted, *path, *out, *last_row;
+  void* status;
+  cudaStream_t s;
+};
+
 // accepted [B], path [B, P], out [B, P], last_row [B]; P = the largest tree
-int xtu_tree_verify_greedy(const int* target, const int* tokens, const int* parents, const int* q_start, int B, int T,
-                           int P, int* accepted, int* path, int* out, int* last_row, void* status, cudaStream_t s) {
-  if (B <= 0 || P <= 0) return 0;
-  if (P > TREE_MAX_NODES) return -2;
-  const cudaError_t e = launch_pdl(tree_verify_greedy_kernel, dim3(B), dim3(32), 0, s, target, tokens, parents,
-                                   q_start, T, P, accepted, path, out, last_row, reinterpret_cast<XtuStatus*>(status));
+int xtu_tree_verify_greedy(const XtuTreeVerifyGreedy* a) {
+  if (a->B <= 0 || a->P <= 0) return 0;
+  if (a->P > TREE_MAX_NODES) return -2;
+  const cudaError_t e = launch_pdl(tree_verify_greedy_kernel, dim3(a->B), dim3(32), 0, a->s, a->target, a->tokens,
+                                   a->parents, a->q_start, a->T, a->P, a->accepted, a->path, a->out, a->last_row,
+                                   static_cast<XtuStatus*>(a->status));
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? 1 : -(int)e;
 }
 
 // probs [T, V] (row stride ldp elements), draft the same or null; bf16: both bf16, else fp32
-int xtu_tree_verify(const void* probs, long long ldp, const void* draft, long long ldq, int bf16, int V,
-                    const int* tokens, const int* parents, const int* q_start, const float* u_accept,
-                    const float* u_draw, int B, int T, int P, int* accepted, int* path, int* out, int* last_row,
-                    void* status, cudaStream_t s) {
-  if (B <= 0 || P <= 0) return 0;
-  if (P > TREE_MAX_NODES || V <= 0 || B > 65535) return -2;
-#define XTU_TV(E, D)                                                                                              \
-  return tv_launch<E, D>(probs, ldp, draft, ldq, V, tokens, parents, q_start, u_accept, u_draw, B, T, P, accepted, \
-                         path, out, last_row, status, s)
-  if (bf16) {
-    if (draft) XTU_TV(__nv_bfloat16, true);
-    XTU_TV(__nv_bfloat16, false);
-  }
-  if (draft) XTU_TV(float, true);
-  XTU_TV(float, false);
-#undef XTU_TV
+int xtu_tree_verify(const XtuTreeVerify* a) {
+  if (a->B <= 0 || a->P <= 0) return 0;
+  if (a->P > TREE_MAX_NODES || a->V <= 0 || a->B > 65535) return -2;
+  if (a->bf16) return a->draft ? tv_launch<__nv_bfloat16, true>(*a) : tv_launch<__nv_bfloat16, false>(*a);
+  return a->draft ? tv_launch<float, true>(*a) : tv_launch<float, false>(*a);
 }
 
 // k_ptrs / v_ptrs: host arrays of L cache addresses, or null: layer l at k_base + l * k_step
 // bytes.  kb / vb: bytes of one head's K / V row (vb 16-byte pieces; fp8_v: V is [Dv][64]
 // inside a block and vb is unused).
-int xtu_tree_commit(const long long* k_ptrs, const long long* v_ptrs, long long k_base, long long k_step,
-                    long long v_base, long long v_step, int L, const int* path, int P, const int* accepted,
-                    const int* q_start, const int* kv_len, const int* bt, int bt_stride, int bt_cols, int B,
-                    int num_blocks, int Hkv, int kb, int vb, int fp8_v, int Dv, cudaStream_t s) {
-  if (B <= 0 || L <= 0 || P <= 1) return 0;
-  if (kb % 16 != 0 || (!fp8_v && vb % 16 != 0)) return -2;
-  const int parts = fp8_v ? 1 + (Hkv * Dv + 255) / 256 : 1;
+struct XtuTreeCommit {
+  const long long *k_ptrs, *v_ptrs;
+  long long k_base, k_step, v_base, v_step;
+  int L;
+  const int* path;
+  int P;
+  const int *accepted, *q_start, *kv_len, *bt;
+  int bt_stride, bt_cols, B, num_blocks, Hkv, kb, vb, fp8_v, Dv;
+  cudaStream_t s;
+};
+
+int xtu_tree_commit(const XtuTreeCommit* a) {
+  if (a->B <= 0 || a->L <= 0 || a->P <= 1) return 0;
+  if (a->kb % 16 != 0 || (!a->fp8_v && a->vb % 16 != 0)) return -2;
+  const int parts = a->fp8_v ? 1 + (a->Hkv * a->Dv + 255) / 256 : 1;
   int launches = 0;
-  for (int l0 = 0; l0 < L; l0 += TC_LAYERS) {
-    const int m = L - l0 < TC_LAYERS ? L - l0 : TC_LAYERS;
+  for (int l0 = 0; l0 < a->L; l0 += TC_LAYERS) {
+    const int m = a->L - l0 < TC_LAYERS ? a->L - l0 : TC_LAYERS;
     TcLayers t{};
     for (int l = 0; l < m; ++l) {
-      t.k[l] = reinterpret_cast<void*>(k_ptrs ? k_ptrs[l0 + l] : k_base + (l0 + l) * k_step);
-      t.v[l] = reinterpret_cast<void*>(v_ptrs ? v_ptrs[l0 + l] : v_base + (l0 + l) * v_step);
+      t.k[l] = reinterpret_cast<void*>(a->k_ptrs ? a->k_ptrs[l0 + l] : a->k_base + (l0 + l) * a->k_step);
+      t.v[l] = reinterpret_cast<void*>(a->v_ptrs ? a->v_ptrs[l0 + l] : a->v_base + (l0 + l) * a->v_step);
     }
-    const cudaError_t e = launch_pdl(tree_commit_kernel, dim3(B, m, parts), dim3(256), 0, s, t, path, P, accepted, q_start,
-                                     kv_len, bt, bt_stride, bt_cols, num_blocks, Hkv, kb, vb, fp8_v, Dv);
+    const cudaError_t e = launch_pdl(tree_commit_kernel, dim3(a->B, m, parts), dim3(256), 0, a->s, t, a->path, a->P,
+                                     a->accepted, a->q_start, a->kv_len, a->bt, a->bt_stride, a->bt_cols,
+                                     a->num_blocks, a->Hkv, a->kb, a->vb, a->fp8_v, a->Dv);
     if (e != cudaSuccess) {
       (void)cudaGetLastError();
       return -(int)e;

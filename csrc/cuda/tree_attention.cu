@@ -1009,44 +1009,66 @@ extern "C" {
 // [num_blocks, Hkv, 64, D] and V [num_blocks, Hkv, DV, 64]; o [T, Hq, DV] bf16.  ws: splits *
 // T * Hq * (DV + 2) floats when splits > 1 (<= 64).  row_tiles: 128-row tiles of a CTA (1 or 2; heads of 256
 // always 1).  Returns the launches, < 0 on error.
-int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_cache, const void* v_cache, int fp8,
-                       void* o, const int* q_start, const int* kv_len, const int* block_table, int bt_stride,
-                       int bt_cols, const int* mask, int W, const int* depth, int window, int B, int max_nodes, int T,
-                       int Hq, int Hkv, int D, int DV, int num_blocks, float scale, float k_scale, float v_scale,
-                       const float* sinks, int row_tiles, int splits, float* ws, void* status, cudaStream_t s) {
-  if (B <= 0 || T <= 0 || max_nodes <= 0) return 0;
-  if (Hkv <= 0 || Hq % Hkv != 0 || B > 65535 || Hkv > 65535 || W <= 0) return -2;
-  if (row_tiles < 1 || row_tiles > 2 || splits < 1 || splits > 64 || (splits > 1 && ws == nullptr)) return -3;
-  if (window > 0 && depth == nullptr) return -4;
+struct XtuTreeAttention {
+  const void* q;
+  long long q_ts;
+  int q_hs;
+  const void *k_cache, *v_cache;
+  int fp8;
+  void* o;
+  const int *q_start, *kv_len, *block_table;
+  int bt_stride, bt_cols;
+  const int* mask;
+  int W;
+  const int* depth;
+  int window, B, max_nodes, T, Hq, Hkv, D, DV, num_blocks;
+  float scale, k_scale, v_scale;
+  const float* sinks;
+  int row_tiles, splits;
+  float* ws;
+  void* status;
+  cudaStream_t s;
+};
+
+int xtu_tree_attention(const XtuTreeAttention* a) {
+  const int B = a->B, T = a->T, Hq = a->Hq, Hkv = a->Hkv, D = a->D, DV = a->DV, splits = a->splits;
+  const int row_tiles = a->row_tiles, num_blocks = a->num_blocks;
+  const bool fp8 = a->fp8 != 0;
+  cudaStream_t s = a->s;
+  if (B <= 0 || T <= 0 || a->max_nodes <= 0) return 0;
+  if (Hkv <= 0 || Hq % Hkv != 0 || B > 65535 || Hkv > 65535 || a->W <= 0) return -2;
+  if (row_tiles < 1 || row_tiles > 2 || splits < 1 || splits > 64 || (splits > 1 && a->ws == nullptr)) return -3;
+  if (a->window > 0 && a->depth == nullptr) return -4;
   TaParams p{};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.q_ts = q_ts;
-  p.q_hs = q_hs;
-  p.o = static_cast<__nv_bfloat16*>(o);
-  p.q_start = q_start;
-  p.kv_len = kv_len;
-  p.block_table = block_table;
-  p.bt_stride = bt_stride;
-  p.bt_cols = bt_cols;
-  p.mask = mask;
-  p.W = W;
-  p.depth = depth;
-  p.window = window > 0 ? window : 0;
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.q_ts = a->q_ts;
+  p.q_hs = a->q_hs;
+  p.o = static_cast<__nv_bfloat16*>(a->o);
+  p.q_start = a->q_start;
+  p.kv_len = a->kv_len;
+  p.block_table = a->block_table;
+  p.bt_stride = a->bt_stride;
+  p.bt_cols = a->bt_cols;
+  p.mask = a->mask;
+  p.W = a->W;
+  p.depth = a->depth;
+  p.window = a->window > 0 ? a->window : 0;
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.G = Hq / Hkv;
   p.T = T;
   p.g_inv = p.G > 1 ? (uint32_t)(((1ull << 32) + p.G - 1) / p.G) : 0u;
-  p.scale_log2 = scale * LOG2E * (fp8 ? k_scale : 1.f);
-  p.out_scale = fp8 ? v_scale : 1.f;
-  p.sinks = sinks;
+  p.scale_log2 = a->scale * LOG2E * (fp8 ? a->k_scale : 1.f);
+  p.out_scale = fp8 ? a->v_scale : 1.f;
+  p.sinks = a->sinks;
   p.splits = splits;
-  p.ws_o = ws;
-  p.ws_lse = ws ? ws + (size_t)splits * T * Hq * DV : nullptr;
-  p.v_raw = v_cache;
+  p.ws_o = a->ws;
+  p.ws_lse = a->ws ? a->ws + (size_t)splits * T * Hq * DV : nullptr;
+  p.v_raw = a->v_cache;
   p.num_blocks = num_blocks;
-  p.max_nodes = max_nodes;
-  p.status = reinterpret_cast<XtuStatus*>(status);
+  p.max_nodes = a->max_nodes;
+  p.status = static_cast<XtuStatus*>(a->status);
+  const void *k_cache = a->k_cache, *v_cache = a->v_cache;
   const uint64_t krows = (uint64_t)num_blocks * Hkv * TA_PAGE;
   CUtensorMap tk, tv;
   int rc;
@@ -1062,7 +1084,7 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
                   CU_TENSOR_MAP_SWIZZLE_128B);
   }
   if (rc) return rc;
-  const int rows = max_nodes * p.G;
+  const int rows = p.max_nodes * p.G;
   int r = -6;   // head sizes not served
   if (fp8 && D == 64 && DV == 64)
     r = tt_rows<TtCfg<64, 64, 128, 1, 3, 3, 6>, TtCfg<64, 64, 128, 2, 3, 3, 6>>(tk, tv, p, rows, row_tiles, B, s);
@@ -1080,8 +1102,8 @@ int xtu_tree_attention(const void* q, long long q_ts, int q_hs, const void* k_ca
   if (r < 0 || splits == 1) return r;
   const int heads = T * Hq;
   const cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((heads + 7) / 8), dim3(256), 0, s,
-                                   (const float*)p.ws_o, (const float*)p.ws_lse, splits, heads, Hq, DV, q_start, B,
-                                   sinks, p.o);
+                                   (const float*)p.ws_o, (const float*)p.ws_lse, splits, heads, Hq, DV, p.q_start, B,
+                                   p.sinks, p.o);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? r + 1 : -(int)e;
 }

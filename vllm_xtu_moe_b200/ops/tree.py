@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import functools
 import math
+from array import array
 from dataclasses import dataclass
 
 import torch
@@ -81,6 +82,10 @@ def _elsewhere(device: torch.device) -> bool:
     return device.index != torch.cuda.current_device()
 
 
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _status(device: torch.device) -> int:
     st = N._status.get(device.index)
     return (st if st is not None else N.status_buffer(device)).data_ptr()
@@ -116,7 +121,7 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, max_nodes: int, mask
     _ints("q_start", q_start, (B + 1,), dev)
     W = (max_nodes + 31) // 32
     mask = mask if mask is not None else parents.new_empty((T, W))
-    depth = depth if depth is not None else parents.new_empty(T)
+    depth = depth if depth is not None else torch.empty_like(parents)
     _ints("mask", mask, (T, W), dev)
     _ints("depth", depth, (T,), dev)
     if not parents.is_cuda:
@@ -125,7 +130,7 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, max_nodes: int, mask
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return tree_mask(parents, q_start, max_nodes, mask, depth)
-    N.call("xtu_tree_mask", parents.data_ptr(), q_start.data_ptr(), B, T, max_nodes, W, mask.data_ptr(),
+    N.call_packed("xtu_tree_mask", parents.data_ptr(), q_start.data_ptr(), B, T, max_nodes, W, mask.data_ptr(),
            depth.data_ptr(), _status(dev), N.stream_ptr(dev))
     return mask, depth
 
@@ -258,7 +263,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if not (scale > 0 and k_scale > 0):
         raise ValueError("scales must be positive")
     if out is None:
-        out = q.new_empty((T, Hq, Dv))
+        out = torch.empty_like(q) if Dv == D and q.is_contiguous() else q.new_empty((T, Hq, Dv))
     elif out.shape != (T, Hq, Dv) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out must be contiguous {q.dtype} [{T}, {Hq}, {Dv}] on {dev}")
     if not q.is_cuda:
@@ -294,10 +299,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             raise ValueError(f"workspace must be contiguous fp32 on {dev}, on a 16-byte boundary")
         if ws is None or ws.numel() < need:
             ws = torch.empty(need, dtype=torch.float32, device=dev)
-    N.call("xtu_tree_attention", q.data_ptr(), q_ts, q_hs, k_cache.data_ptr(), v_cache.data_ptr(),
+    N.call_packed("xtu_tree_attention", q.data_ptr(), q_ts, q_hs, k_cache.data_ptr(), v_cache.data_ptr(),
            int(fp8), out.data_ptr(), meta.q_start.data_ptr(), meta.kv_len.data_ptr(), bt.data_ptr(), bt.stride(0),
-           bt.shape[1], meta.mask.data_ptr(), W, N.ptr(meta.depth), int(window), B, meta.max_nodes, T, Hq, Hk, D, Dv,
-           nb, float(scale), float(k_scale), float(v_scale), N.ptr(sinks), tiles, splits, N.ptr(ws),
+           bt.shape[1], meta.mask.data_ptr(), W, _ptr(meta.depth), int(window), B, meta.max_nodes, T, Hq, Hk, D, Dv,
+           nb, float(scale), float(k_scale), float(v_scale), _ptr(sinks), tiles, splits, _ptr(ws),
            _status(dev), N.stream_ptr(dev))
     return out
 
@@ -306,8 +311,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 # verification
 # ---------------------------------------------------------------------------
 def _verdict(B: int, max_nodes: int, like: torch.Tensor) -> TreeVerdict:
-    return TreeVerdict(like.new_empty(B), like.new_empty((B, max_nodes)), like.new_empty((B, max_nodes)),
-                       like.new_empty(B))
+    accepted, path = like.new_empty(B), like.new_empty((B, max_nodes))
+    return TreeVerdict(accepted, path, torch.empty_like(path), torch.empty_like(accepted))
 
 
 def _children(parents: list, n: int, at: int) -> list:
@@ -370,7 +375,7 @@ def verify_tree_greedy(target: torch.Tensor, tokens: torch.Tensor, parents: torc
         with torch.cuda.device(dev):
             return verify_tree_greedy(target, tokens, parents, q_start, max_nodes)
     v = _verdict(B, max_nodes, tokens)
-    N.call("xtu_tree_verify_greedy", target.data_ptr(), tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), B, T,
+    N.call_packed("xtu_tree_verify_greedy", target.data_ptr(), tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), B, T,
            max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
            _status(dev), N.stream_ptr(dev))
     return v
@@ -463,7 +468,7 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
         with torch.cuda.device(dev):
             return verify_tree(probs, tokens, parents, q_start, max_nodes, u_accept, u_draw, draft_probs)
     v = _verdict(B, max_nodes, tokens)
-    N.call("xtu_tree_verify", probs.data_ptr(), probs.stride(0), N.ptr(draft_probs),
+    N.call_packed("xtu_tree_verify", probs.data_ptr(), probs.stride(0), _ptr(draft_probs),
            0 if draft_probs is None else draft_probs.stride(0), int(probs.dtype == torch.bfloat16), probs.shape[1],
            tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(), B, T,
            max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
@@ -551,17 +556,18 @@ def commit_tree(k_caches, v_caches, path: torch.Tensor, accepted: torch.Tensor, 
     es = k0.element_size()
     if D * es % 16 or (not fp8 and Dv * es % 16):
         raise ValueError("head rows must be multiples of 16 bytes")
-    kp = vp = None
-    kb = ks = vb = vs = 0
+    kp = vp = kb = ks = vb = vs = 0
     if stacked:
         kb, ks, vb, vs = k0.data_ptr(), k_caches.stride(0) * es, v0.data_ptr(), v_caches.stride(0) * es
         odd = (kb | ks | vb | vs) & 15
     else:
         kl, vl = [k.data_ptr() for k in k_caches], [v.data_ptr() for v in v_caches]
-        kp, vp = (N.c_longlong * L)(*kl), (N.c_longlong * L)(*vl)
+        lists = array("q", kl + vl)            # (lives until the call is over)
+        kp = lists.buffer_info()[0]
+        vp = kp + 8 * L
         odd = any(x & 15 for x in kl) or any(x & 15 for x in vl)
     if odd:
         raise ValueError("the caches must start on 16-byte boundaries")
-    N.call("xtu_tree_commit", kp, vp, kb, ks, vb, vs, L, path.data_ptr(), P, accepted.data_ptr(), q_start.data_ptr(),
+    N.call_packed("xtu_tree_commit", kp, vp, kb, ks, vb, vs, L, path.data_ptr(), P, accepted.data_ptr(), q_start.data_ptr(),
            kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], B, nb, Hk, D * es,
            Dv * es, int(fp8), Dv, N.stream_ptr(dev))
