@@ -160,15 +160,15 @@ __global__ void __launch_bounds__(32) tree_verify_greedy_kernel(
 // slice, and the sums meet in every CTA's shared memory.  The walk runs in all of them on one
 // copy of the nodes (rank 0's, read through shared memory once) and on the same sums in the
 // same order, so they agree on every step and meet at the same cluster barriers whatever the
-// inputs hold or do meanwhile; a walk by rank 0 that told the others took a second barrier a
-// pass (55 against 50 us for 32 trees of 26 nodes).  Weights and sums are 64-bit: with 150K terms a
-// 32-bit sum is off by more than many tokens' weight, and the drawn token would depend on the
-// split.
-// What bounds it is latency: three dependent loads before the walk (the sequence's bounds, its nodes,
-// their probabilities), then per pass a load of the slice (the first at its node), two block
-// barriers and a cluster barrier, and the search for the drawn token.  One sequence, V = 151552: 17 us
-// cold.  32 trees of 26 nodes: 50 us for the 30 MB that they read (5 us at the copy rate), in two waves:
-// 18 clusters of 8 fit.  32-bit arithmetic would take 6 % off.
+// inputs hold or do meanwhile (a walk by rank 0 that told the others took a second barrier a
+// pass).  Weights and sums are 64-bit: with 150K terms a 32-bit sum is off by more than many
+// tokens' weight, and the drawn token would depend on the split.
+// What bounds it is latency.  In cycles: three dependent loads before the walk (the sequence's bounds,
+// its nodes, their probabilities) 5500, the first steps 3500; then per pass the load of the slice (the
+// first at its node) 3000 to 6000, its weights 1100 with no rejection, 3000 with one and 1100 for each
+// further one (64-bit arithmetic), sums and cluster barrier 2000, the walk 1700; the search for the drawn token 4000.
+// One sequence, V = 151552: 16 us cold.  32 trees of 26 nodes: 31 us for the 30 MB that they read (5 us
+// at the copy rate), in two waves: 18 clusters of 8 fit.
 struct TvCmd {
   int op;        // 0 sum the weights, 1 draw, 2 done
   int row;       // row of probs
@@ -179,16 +179,15 @@ struct TvCmd {
   double target; // draw: target less the slices before the owner's
 };
 
-// Drawn children: a pass for every rejection, so 1024 threads whose registers hold their slices of p and
-// q (20 weights each: a vocabulary of 163840 over 8 CTAs) from pass to pass; measured (32
-// sequences of 26 nodes, V = 151552): 50 us, 512 threads at two CTAs an SM that read them again 63.
-// Drafts chosen outright: one pass, 512 threads start sooner (18.4 us against 20.5).
+constexpr int TV_THREADS = 512, TV_WARPS = TV_THREADS / 32;
+// Weights of a thread in flight (bf16: whole 16-byte loads of them).  Drawn children take a pass for every
+// rejection, so the registers hold the slices of p and q from pass to pass: 40 weights each are a vocabulary of
+// 163840 over 8 CTAs.  Measured (32 sequences of 26 nodes, V = 151552): 30.7 us; 1024 threads with 20 each 37.3,
+// 384 with 56 33.2, 256 with 80 39.8, slices that are read again 33.6.  Drafts chosen outright take one pass.
 template <bool DRAFT>
 struct TvCfg {
-  static constexpr int THREADS = DRAFT ? 1024 : 512, WARPS = THREADS / 32;
-  static constexpr int HELD = DRAFT ? 20 : 16;   // weights of a thread in flight (bf16: whole 16-byte loads of them)
+  static constexpr int HELD = DRAFT ? 40 : 16;
 };
-constexpr int TV_MAX_WARPS = 32;
 constexpr int TV_MAX_C = 8;
 
 __device__ __forceinline__ float tv_load1(const float* p) { return __ldg(p); }
@@ -213,20 +212,37 @@ struct TvShared {
   double zi[TREE_MAX_NODES];          // zi[r]: 1 / (sum of the weights after r rejections)
   double slice[2][TV_MAX_C];          // the CTAs' sums, of this pass and the one before
   int n, q0;
-  double warp_sum[TV_MAX_WARPS];
+  double warp_sum[TV_WARPS];
   float u_draw;
   int found, best;                    // the draw: the first weight past the target, the last positive one
   TvCmd cmd;
 };
 
-// weight of an element after `rej` rejections (drawn children), from its p and q
-__device__ __forceinline__ double tv_weight(float p, float q, const double* zi, int rej) {
-  double w = p > 0.f ? (double)p : 0.0;      // NaN and negative entries weigh nothing
-  if (rej == 0) return w;
-  const double qd = q > 0.f ? (double)q : 0.0;
-  w = fmax(w - qd, 0.0);
-  for (int r = 1; r < rej; ++r) w = fmax(w * zi[r] - qd, 0.0);
-  return w;
+// weights of N elements after `rej` rejections (drawn children), from their p and q.  The elements go
+// through a rejection side by side: a loop per element was one chain of dependent 64-bit operations after
+// another (12400 cycles a pass at two rejections against 2900 at one).
+__device__ __forceinline__ double tv_left(double w) {   // max(w, 0) by its sign bit: 64-bit compares are slow
+  const int hi = __double2hiint(w), keep = ~(hi >> 31);
+  return __hiloint2double(hi & keep, __double2loint(w) & keep);
+}
+template <int N>
+__device__ __forceinline__ void tv_weights(const float (&p)[N], const float (&q)[N], const double* zi, int rej,
+                                           double (&w)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) w[e] = (double)fmaxf(p[e], 0.f);   // NaN and negative entries weigh nothing
+  if (rej == 0) return;
+  double d[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    d[e] = (double)fmaxf(q[e], 0.f);
+    w[e] = tv_left(w[e] - d[e]);
+  }
+#pragma unroll 1
+  for (int r = 1; r < rej; ++r) {
+    const double z = zi[r];
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = tv_left(w[e] * z - d[e]);
+  }
 }
 
 // One warp's view of a row: `weights(i, w)` gives the VE weights from element i on (0 past the row).
@@ -254,14 +270,17 @@ struct TvRow {
     }
   }
   __device__ __forceinline__ void weigh(int i, const float (&x)[VE], const float (&y)[VE], double (&w)[VE]) const {
-    unsigned gone = 0;                       // point mass: rejected tokens among these
-    for (int r = 0; !DRAFT && r < rej; ++r) {
-      const unsigned d = (unsigned)(rejected[r] - i);
-      if (d < (unsigned)VE) gone |= 1u << d;
-    }
+    if constexpr (DRAFT) {
+      tv_weights(x, y, zi, rej, w);
+    } else {
+      unsigned gone = 0;                     // point mass: rejected tokens among these
+      for (int r = 0; r < rej; ++r) {
+        const unsigned d = (unsigned)(rejected[r] - i);
+        if (d < (unsigned)VE) gone |= 1u << d;
+      }
 #pragma unroll
-    for (int e = 0; e < VE; ++e)
-      w[e] = DRAFT ? tv_weight(x[e], y[e], zi, rej) : x[e] > 0.f && !((gone >> e) & 1u) ? (double)x[e] : 0.0;
+      for (int e = 0; e < VE; ++e) w[e] = (gone >> e) & 1u ? 0.0 : (double)fmaxf(x[e], 0.f);
+    }
   }
 };
 
@@ -271,8 +290,31 @@ __device__ __forceinline__ double tv_warp_sum(double x) {
   return x;
 }
 
+// inclusive prefix sums over the lanes
+__device__ __forceinline__ double tv_warp_scan(double x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += up;
+  }
+  return x;
+}
+
+// the first lane whose prefix sum passes t (or -1: none does), the last lane that holds anything (or 0) and
+// what is left of t at the former.  (64-bit additions take some 40 cycles one after another: lanes, not a loop.)
+__device__ __forceinline__ int tv_find(double x, double sum, double t, int& last, double& at) {
+  const unsigned some = __ballot_sync(0xffffffffu, x > 0.0), past = __ballot_sync(0xffffffffu, x > 0.0 && sum > t);
+  last = some ? 31 - __clz(some) : 0;
+  const double before = __shfl_up_sync(0xffffffffu, sum, 1);
+  const int first = past ? __ffs(past) - 1 : -1;
+  at = t - __shfl_sync(0xffffffffu, before, first > 0 ? first : 0);
+  if (first == 0) at = t;
+  return first;
+}
+
 template <typename E, bool DRAFT>
-__global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
+__global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
     const E* __restrict__ probs, long long ldp, const E* __restrict__ draft, long long ldq, int V, int vec,
     const int* __restrict__ tokens, const int* __restrict__ parents, const int* __restrict__ q_start,
     const float* __restrict__ u_accept, const float* __restrict__ u_draw, int T, int P, int* __restrict__ accepted,
@@ -283,7 +325,7 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
   cg::cluster_group cl = cg::this_cluster();
   const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int VE = 16 / sizeof(E), TV_THREADS = TvCfg<DRAFT>::THREADS, TV_WARPS = TvCfg<DRAFT>::WARPS;
+  constexpr int VE = 16 / sizeof(E);
   // this warp's slice of the vocabulary: whole 32 x VE steps
   const int step = 32 * VE;
   constexpr int TV_BATCH = (TvCfg<DRAFT>::HELD + VE - 1) / VE;   // 16-byte loads of a lane under way at a time
@@ -344,15 +386,15 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
       const bool first = pass == 0;
       bool have_sum = !first;
       TvCmd c{};
-      double tot = 0.0;
+      double tot = 0.0, part = 0.0, upto = 0.0;        // the CTAs' sums: all, this lane's, up to this lane's
       if (n == 0) {
         c.op = 2;
       } else {
         if (have_sum) {                       // the sum that was asked for
-          for (int r = 0; r < C; ++r) tot += s.slice[(pass - 1) & 1][r];
+          part = lane < C ? s.slice[(pass - 1) & 1][lane] : 0.0;
+          upto = tv_warp_scan(part);
+          tot = __shfl_sync(0xffffffffu, upto, 31);
           z = tot > 0.0 ? tot : 1.0;
-          if (lane == 0) s.zi[rej] = 1.0 / z;
-          __syncwarp();
         }
         // walk on, unless the sum was that of the final weights (no child left)
         for (;;) {
@@ -362,9 +404,11 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
           const int x = s.tok[next];
           bool take;
           if (DRAFT) {
-            const double w = tv_weight(s.pt[next], s.qt[next], s.zi, rej);
-            const double q = s.qt[next] > 0.f ? (double)s.qt[next] : 0.0;
-            take = s.pt[next] >= 0.f && (double)s.u[next] * q * (rej > 0 ? z : 1.0) < w;
+            const float p1[1] = {s.pt[next]}, q1[1] = {s.qt[next]};
+            double w[1];
+            tv_weights(p1, q1, s.zi, rej, w);
+            const double q = q1[0] > 0.f ? (double)q1[0] : 0.0;
+            take = p1[0] >= 0.f && (double)s.u[next] * q * (rej > 0 ? z : 1.0) < w[0];
           } else {
             bool dup = false;
             for (int r = lane; r < rej; r += 32) dup |= s.rejected[r] == x;
@@ -384,7 +428,10 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
             gone = 0.0;
             continue;
           }
-          if (lane == 0) s.rejected[rej] = x;
+          if (lane == 0) {
+            s.rejected[rej] = x;
+            if (DRAFT && rej > 0) s.zi[rej] = 1.0 / z;
+          }
           ++rej;
           __syncwarp();
           if (DRAFT) break;                   // the next test (or the draw) needs the new sum
@@ -397,18 +444,9 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
           c.rej = 0;
         }
         if (have_sum) {                       // the sum of the final weights is known: draw
-          const double t = (double)s.u_draw * tot;
-          double before = 0.0, at = 0.0;
-          int owner = -1, last = 0;
-          for (int r = 0; r < C; ++r) {
-            const double x = s.slice[(pass - 1) & 1][r];
-            if (owner < 0 && x > 0.0 && before + x > t) {
-              owner = r;
-              at = t - before;
-            }
-            if (x > 0.0) last = r;
-            before += x;
-          }
+          int last;
+          double at;
+          const int owner = tv_find(part, upto, (double)s.u_draw * tot, last, at);
           c.op = 1;
           c.any = owner < 0;
           c.owner = owner < 0 ? last : owner;
@@ -434,10 +472,12 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
       for (int base = lo; base < hi; base += TV_BATCH * step) {
         if (held != c.row || (DRAFT && c.rej > 0 && !held_q)) {
 #pragma unroll
-          for (int k = 0; k < TV_BATCH; ++k) row.load(base + k * step + lane * VE, x[k], y[k]);
+          for (int k = 0; k < TV_BATCH; ++k)
+            if (base + k * step < hi) row.load(base + k * step + lane * VE, x[k], y[k]);
         }
 #pragma unroll
         for (int k = 0; k < TV_BATCH; ++k) {
+          if (base + k * step >= hi) break;            // (the whole warp)
           double w[VE];
           row.weigh(base + k * step + lane * VE, x[k], y[k], w);
 #pragma unroll
@@ -460,21 +500,13 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
     }
     if (rank == c.owner) {
       // the warp whose slice holds the target (warp_sum is of these weights), then the element
-      double before = 0.0;
-      int mine = -1, last = 0;
-      double at = 0.0;
-      for (int w = 0; w < TV_WARPS; ++w) {
-        const double x = s.warp_sum[w];
-        if (!c.any && mine < 0 && x > 0.0 && before + x > c.target) {
-          mine = w;
-          at = c.target - before;
-        }
-        if (x > 0.0) last = w;
-        before += x;
-      }
+      int last;
+      double at;
+      const double ws = lane < TV_WARPS ? s.warp_sum[lane] : 0.0;
+      const int mine = tv_find(ws, tv_warp_scan(ws), c.target, last, at);
       // that slice again, VE neighbouring weights a thread and a turn of the block (one load latency
       // instead of one warp's chain of them): prefix sums over the lanes, then over the warps
-      const bool any = mine < 0;
+      const bool any = c.any || mine < 0;
       const int wsel = any ? last : mine;
       const long long sf = (long long)(rank * TV_WARPS + wsel) * per;
       const int slo = (int)(sf < V ? sf : V), shi = (int)(sf + per < V ? sf + per : V);
@@ -492,23 +524,15 @@ __global__ void __launch_bounds__(TvCfg<DRAFT>::THREADS) tree_verify_kernel(
           own += w[e];
           if (w[e] > 0.0) last_pos = i + e;
         }
-        double cum = own;                                // lanes up to this one
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double up = __shfl_up_sync(0xffffffffu, cum, o);
-          if (lane >= o) cum += up;
-        }
+        const double cum = tv_warp_scan(own);            // lanes up to this one
         __syncthreads();                                 // (warp_sum was read above, or in the turn before)
         if (lane == 31) s.warp_sum[warp] = cum;
         if (tid == 0) s.found = INT_MAX;
         if (tid == 0 && base == slo) s.best = 0;
         __syncthreads();
-        double c2 = run;
-        for (int k = 0; k < TV_WARPS; ++k) {
-          if (k < warp) c2 += s.warp_sum[k];
-          run += s.warp_sum[k];
-        }
-        c2 += cum - own;
+        const double sums = tv_warp_scan(lane < TV_WARPS ? s.warp_sum[lane] : 0.0);
+        double c2 = run + (warp > 0 ? __shfl_sync(0xffffffffu, sums, warp - 1) : 0.0) + (cum - own);
+        run += __shfl_sync(0xffffffffu, sums, 31);
         int first_pos = INT_MAX;
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
@@ -670,14 +694,17 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
 
 template <typename E, bool DRAFT>
 int tv_launch(const XtuTreeVerify& a) {
-  // CTAs per sequence: a slice of at least 4096 elements each
-  const int C = a.V <= 4096 ? 1 : a.V <= 8192 ? 2 : a.V <= 16384 ? 4 : 8;
+  // CTAs per sequence: a slice of at least 4096 elements each.  18 clusters of 8 run at a time; for more
+  // sequences 4 CTAs a cluster where their registers hold the slice (drawn children, 32 / 64 sequences: V =
+  // 33000 34.8 / 57.3 -> 24.6 / 41.0 us, 65536 34.8 / 53.2 -> 28.7 / 41.0; 16: 26.6 -> 28.7)
+  const bool many = DRAFT && a.B > 18 && a.V <= 4 * TV_THREADS * TvCfg<DRAFT>::HELD;
+  const int C = a.V <= 4096 ? 1 : a.V <= 8192 ? 2 : a.V <= 16384 || many ? 4 : 8;
   constexpr int VE = 16 / sizeof(E);
   const bool vec = a.V % VE == 0 && a.ldp % VE == 0 && (reinterpret_cast<uintptr_t>(a.probs) & 15) == 0 &&
                    (!DRAFT || (a.ldq % VE == 0 && (reinterpret_cast<uintptr_t>(a.draft) & 15) == 0));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C, a.B);
-  cfg.blockDim = dim3(TvCfg<DRAFT>::THREADS);
+  cfg.blockDim = dim3(TV_THREADS);
   cfg.stream = a.s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;

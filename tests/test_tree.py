@@ -476,6 +476,20 @@ def test_verify_vocabulary_of_a_model(mode):
     same_verdict(run_verify(s, "cuda"), oracle_of(s))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["point", "draft"])
+@pytest.mark.parametrize("V", [9000, 20003, 70001])
+def test_verify_many_sequences_and_many_rejections(mode, V):
+    """More sequences than clusters of 8 CTAs run at a time; nodes whose children are rejected one after another."""
+    s = verify_inputs([9, 4, 1, 12] * 6, V, mode, 13, sharp=1.0)
+    same_verdict(run_verify(s, "cuda"), oracle_of(s))
+    s = verify_inputs([40, 3, 25], V, mode, 14, sharp=1.5)
+    s["parents"] = i32([-1] + [0] * 39 + [-1, 0, 0] + [-1] + [0] * 24)
+    s["u_accept"].fill_(0.9995)
+    v = run_verify(s, "cuda")
+    same_verdict(v, oracle_of(s))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("mode", ["point", "draft"])
 def test_verify_edges(device, mode):
