@@ -32,7 +32,7 @@ from .attention import KV_BLOCK, _gather_kv, dequant_fp8_cache
 
 MAX_NODES = 1024          # nodes of one sequence's tree
 MAX_SPLITS = 64
-_FP8 = torch.float8_e4m3fn
+_FP8, _BF16, _F32, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32, torch.int32
 # (K width, V width) that the GPU kernels serve
 HEAD_DIMS = ((64, 64), (128, 128), (192, 128), (256, 256))
 FP8_HEAD_DIMS = ((64, 64), (128, 128))
@@ -61,16 +61,24 @@ class TreeVerdict:
 
 
 # A step makes these calls once per layer and their kernels take a few microseconds, so the checks are
-# written to cost little where they pass: messages are put together only for a refusal.
-def _ints(name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> None:
-    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}, not "
+# written to cost little where they pass: messages are put together only for a refusal, and devices are
+# compared by their index (-1: the CPU), which costs less than torch.device objects.
+def _name(dev: int) -> str:
+    return "cpu" if dev < 0 else f"cuda:{dev}"
+
+
+def _ints(name: str, t: torch.Tensor, shape: tuple, dev: int) -> None:
+    if t.dtype is not _I32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {_name(dev)}, not "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _table(bt: torch.Tensor, B: int, device: torch.device) -> None:
-    if bt.dtype is not torch.int32 or bt.dim() != 2 or bt.shape[0] < B or bt.stride(1) != 1 or bt.device != device:
-        raise ValueError(f"block_table must be int32 [{B}, blocks] with contiguous rows on {device}")
+def _table(bt: torch.Tensor, B: int, dev: int) -> tuple[int, int]:
+    """(row stride, columns) of a block table."""
+    shape, stride = bt.shape, bt.stride()
+    if bt.dtype is not _I32 or len(shape) != 2 or shape[0] < B or stride[1] != 1 or bt.get_device() != dev:
+        raise ValueError(f"block_table must be int32 [{B}, blocks] with contiguous rows on {_name(dev)}")
+    return stride[0], shape[1]
 
 
 def _max_nodes(n: int) -> None:
@@ -78,17 +86,21 @@ def _max_nodes(n: int) -> None:
         raise ValueError(f"max_nodes must be 1 .. {MAX_NODES}, not {n}")
 
 
-def _elsewhere(device: torch.device) -> bool:
-    return device.index != torch.cuda.current_device()
+def _elsewhere(dev: int) -> bool:
+    return dev != torch._C._cuda_getDevice()
 
 
 def _ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _status(device: torch.device) -> int:
-    st = N._status.get(device.index)
-    return (st if st is not None else N.status_buffer(device)).data_ptr()
+def _status(dev: int) -> int:
+    st = N._status.get(dev)
+    return (st if st is not None else N.status_buffer(dev)).data_ptr()
+
+
+def _stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 # ---------------------------------------------------------------------------
@@ -115,8 +127,8 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, max_nodes: int, mask
     Bit j of row i: j is node i or an ancestor of it.  A parent that is negative or not below its
     node means none.  Rows behind the last sequence are left as they are."""
     _max_nodes(max_nodes)
-    dev = parents.device
-    T, B = parents.shape[0], q_start.shape[0] - 1
+    dev = parents.get_device()
+    T, B = len(parents), len(q_start) - 1
     _ints("parents", parents, (T,), dev)
     _ints("q_start", q_start, (B + 1,), dev)
     W = (max_nodes + 31) // 32
@@ -124,14 +136,14 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, max_nodes: int, mask
     depth = depth if depth is not None else torch.empty_like(parents)
     _ints("mask", mask, (T, W), dev)
     _ints("depth", depth, (T,), dev)
-    if not parents.is_cuda:
+    if dev < 0:
         tree_mask_ref(parents, q_start, max_nodes, mask, depth)
         return mask, depth
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return tree_mask(parents, q_start, max_nodes, mask, depth)
     N.call_packed("xtu_tree_mask", parents.data_ptr(), q_start.data_ptr(), B, T, max_nodes, W, mask.data_ptr(),
-           depth.data_ptr(), _status(dev), N.stream_ptr(dev))
+                  depth.data_ptr(), _status(dev), _stream(dev))
     return mask, depth
 
 
@@ -223,70 +235,73 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
     Caches as in :func:`attention.paged_attention`: bf16 ``[blocks, Hkv, 64, D]`` / ``[.., Dv]`` with
     (D, Dv) in ``HEAD_DIMS``, or fp8 (e4m3) K and per-block transposed V with ``FP8_HEAD_DIMS`` (their
-    products take q as fp16: magnitudes up to 65504).  MLA latent caches are not served.  ``workspace``: fp32, ``splits * T * Hq * (Dv + 2)`` elements when
-    the KV range is split; allocated when None or too small.  One that is passed in belongs to
-    the call until its work is done: calls that may overlap take one each."""
-    if q.dim() != 3 or (q.is_cuda and q.dtype is not torch.bfloat16):
+    products take q as fp16: magnitudes up to 65504).  MLA latent caches are not served.
+    ``workspace``: fp32, ``splits * T * Hq * (Dv + 2)`` elements when the KV range is split; allocated
+    when None or too small.  One that is passed in belongs to the call until its work is done: calls
+    that may overlap take one each."""
+    dev = q.get_device()
+    if q.dim() != 3 or (dev >= 0 and q.dtype is not _BF16):
         raise ValueError("q must be [T, Hq, D] bfloat16")
     T, Hq, D = q.shape
-    dev = q.device
     if k_cache.dim() != 4 or v_cache is None or v_cache.dim() != 4:
         raise ValueError("tree attention takes a K and a V cache [blocks, Hkv, 64, D]")
     nb, Hk, bs, Dk = k_cache.shape
-    fp8 = k_cache.dtype is _FP8
-    Dv = v_cache.shape[2] if fp8 else v_cache.shape[3]
-    if v_cache.shape != ((nb, Hk, Dv, bs) if fp8 else (nb, Hk, bs, Dv)) or Dk != D or v_cache.dtype != k_cache.dtype:
-        raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} do not match each other or q")
+    kt, vshape = k_cache.dtype, v_cache.shape
+    fp8 = kt is _FP8
+    Dv = vshape[2] if fp8 else vshape[3]
+    if vshape != ((nb, Hk, Dv, bs) if fp8 else (nb, Hk, bs, Dv)) or Dk != D or v_cache.dtype is not kt:
+        raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(vshape)} do not match each other or q")
     if Hq % Hk:
         raise ValueError(f"{Hq} query heads do not divide over {Hk} KV heads")
-    if k_cache.device != dev or v_cache.device != dev:
-        raise ValueError(f"the caches must be on {dev}")
-    B = meta.num_seqs
-    bt, mask = meta.block_table, meta.mask
-    _max_nodes(meta.max_nodes)
-    _ints("q_start", meta.q_start, (B + 1,), dev)
-    _ints("kv_len", meta.kv_len, (B,), dev)
-    _table(bt, B, dev)
+    if k_cache.get_device() != dev or v_cache.get_device() != dev:
+        raise ValueError(f"the caches must be on {_name(dev)}")
+    B, most = meta.num_seqs, meta.max_nodes
+    q_start, kv_len, bt, mask = meta.q_start, meta.kv_len, meta.block_table, meta.mask
+    _max_nodes(most)
+    _ints("q_start", q_start, (B + 1,), dev)
+    _ints("kv_len", kv_len, (B,), dev)
+    bt_stride, bt_cols = _table(bt, B, dev)
     W = mask.shape[-1]
     _ints("mask", mask, (T, W), dev)
-    if 32 * W < meta.max_nodes:
-        raise ValueError(f"a mask of {W} words is too narrow for {meta.max_nodes} nodes")
+    if 32 * W < most:
+        raise ValueError(f"a mask of {W} words is too narrow for {most} nodes")
     if window > 0:
         if meta.depth is None:
             raise ValueError("a sliding window needs the nodes' depths")
         _ints("depth", meta.depth, (T,), dev)
-    if sinks is not None and (sinks.dtype is not torch.float32 or not sinks.is_contiguous() or sinks.numel() != Hq
-                              or sinks.device != dev):
-        raise ValueError(f"sinks must be contiguous fp32 [{Hq}] on {dev}")
+    if sinks is not None and (sinks.dtype is not _F32 or not sinks.is_contiguous() or sinks.numel() != Hq
+                              or sinks.get_device() != dev):
+        raise ValueError(f"sinks must be contiguous fp32 [{Hq}] on {_name(dev)}")
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if not (scale > 0 and k_scale > 0):
         raise ValueError("scales must be positive")
     if out is None:
         out = torch.empty_like(q) if Dv == D and q.is_contiguous() else q.new_empty((T, Hq, Dv))
-    elif out.shape != (T, Hq, Dv) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f"out must be contiguous {q.dtype} [{T}, {Hq}, {Dv}] on {dev}")
-    if not q.is_cuda:
+    elif out.shape != (T, Hq, Dv) or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != dev:
+        raise ValueError(f"out must be contiguous {q.dtype} [{T}, {Hq}, {Dv}] on {_name(dev)}")
+    if dev < 0:
         return tree_attention_ref(q, k_cache, v_cache, meta, scale, out, window, sinks, k_scale, v_scale)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return tree_attention(q, k_cache, v_cache, meta, scale, out, workspace, window, sinks, k_scale, v_scale)
-    if not fp8 and k_cache.dtype is not torch.bfloat16:
-        raise ValueError(f"the cache must be bfloat16 or float8_e4m3fn, not {k_cache.dtype}")
+    if not fp8 and kt is not _BF16:
+        raise ValueError(f"the cache must be bfloat16 or float8_e4m3fn, not {kt}")
     if (D, Dv) not in (FP8_HEAD_DIMS if fp8 else HEAD_DIMS):
         raise ValueError(f"{'fp8 ' if fp8 else ''}head sizes {D} / {Dv} are not served "
                          f"({FP8_HEAD_DIMS if fp8 else HEAD_DIMS})")
     if bs != KV_BLOCK:
         raise ValueError(f"the GPU kernels read KV blocks of {KV_BLOCK} tokens, not {bs}")
-    if not k_cache.is_contiguous() or not v_cache.is_contiguous() or (k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+    kp, vp, qp = k_cache.data_ptr(), v_cache.data_ptr(), q.data_ptr()
+    if (kp | vp) & 15 or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError("the caches must be contiguous and start on 16-byte boundaries")
     if not 0 < (nb + 1) * Hk * max(bs, Dv) < 2 ** 31:
         raise ValueError("the cache is empty or has more rows than 31 bits count")
     q_ts, q_hs, q1 = q.stride()
-    if q1 != 1 or (q_ts | q_hs) & 7 or q.data_ptr() & 15:
+    if q1 != 1 or (q_ts | q_hs) & 7 or qp & 15:
         raise ValueError("q rows must be contiguous and start on 16-byte boundaries")
-    rows = meta.max_nodes * (Hq // Hk)
-    seen = min(meta.max_kv_len, window + meta.max_nodes + KV_BLOCK) if window > 0 else meta.max_kv_len
+    rows = most * (Hq // Hk)
+    seen = min(meta.max_kv_len, window + most + KV_BLOCK) if window > 0 else meta.max_kv_len
     tiles, splits = tree_plan(B, Hk, rows, seen, D, Dv, meta.num_splits)
     if not 1 <= splits <= MAX_SPLITS:
         raise ValueError(f"1 .. {MAX_SPLITS} splits, not {splits}")
@@ -294,16 +309,15 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if splits > 1:
         need = splits * T * Hq * (Dv + 2)
         ws = workspace
-        if ws is not None and (ws.dtype is not torch.float32 or not ws.is_contiguous() or ws.device != dev
+        if ws is not None and (ws.dtype is not _F32 or not ws.is_contiguous() or ws.get_device() != dev
                                or ws.data_ptr() & 15):
-            raise ValueError(f"workspace must be contiguous fp32 on {dev}, on a 16-byte boundary")
+            raise ValueError(f"workspace must be contiguous fp32 on {_name(dev)}, on a 16-byte boundary")
         if ws is None or ws.numel() < need:
-            ws = torch.empty(need, dtype=torch.float32, device=dev)
-    N.call_packed("xtu_tree_attention", q.data_ptr(), q_ts, q_hs, k_cache.data_ptr(), v_cache.data_ptr(),
-           int(fp8), out.data_ptr(), meta.q_start.data_ptr(), meta.kv_len.data_ptr(), bt.data_ptr(), bt.stride(0),
-           bt.shape[1], meta.mask.data_ptr(), W, _ptr(meta.depth), int(window), B, meta.max_nodes, T, Hq, Hk, D, Dv,
-           nb, float(scale), float(k_scale), float(v_scale), _ptr(sinks), tiles, splits, _ptr(ws),
-           _status(dev), N.stream_ptr(dev))
+            ws = q.new_empty(need, dtype=_F32)
+    N.call_packed("xtu_tree_attention", qp, q_ts, q_hs, kp, vp, fp8, out.data_ptr(), q_start.data_ptr(),
+                  kv_len.data_ptr(), bt.data_ptr(), bt_stride, bt_cols, mask.data_ptr(), W, _ptr(meta.depth), window, B,
+                  most, T, Hq, Hk, D, Dv, nb, scale, k_scale, v_scale, _ptr(sinks), tiles, splits, _ptr(ws),
+                  _status(dev), _stream(dev))
     return out
 
 
@@ -348,7 +362,7 @@ def _walk(tokens, parents, q_start, max_nodes, choose, final) -> TreeVerdict:
 
 def _tree_args(tokens, parents, q_start, max_nodes):
     _max_nodes(max_nodes)
-    T, B, dev = tokens.shape[0], q_start.shape[0] - 1, tokens.device
+    T, B, dev = len(tokens), len(q_start) - 1, tokens.get_device()
     _ints("tokens", tokens, (T,), dev)
     _ints("parents", parents, (T,), dev)
     _ints("q_start", q_start, (B + 1,), dev)
@@ -369,15 +383,15 @@ def verify_tree_greedy(target: torch.Tensor, tokens: torch.Tensor, parents: torc
     with the target's token after the last accepted node (``verify_greedy`` for trees)."""
     T, B, dev = _tree_args(tokens, parents, q_start, max_nodes)
     _ints("target", target, (T,), dev)
-    if not tokens.is_cuda:
+    if dev < 0:
         return verify_tree_greedy_ref(target, tokens, parents, q_start, max_nodes)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return verify_tree_greedy(target, tokens, parents, q_start, max_nodes)
     v = _verdict(B, max_nodes, tokens)
-    N.call_packed("xtu_tree_verify_greedy", target.data_ptr(), tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), B, T,
-           max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
-           _status(dev), N.stream_ptr(dev))
+    N.call_packed("xtu_tree_verify_greedy", target.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
+                  q_start.data_ptr(), B, T, max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(),
+                  v.last_row.data_ptr(), _status(dev), _stream(dev))
     return v
 
 
@@ -453,26 +467,27 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     distribution.  NaN and negative entries weigh nothing, and a draft outside the vocabulary is
     never accepted."""
     T, B, dev = _tree_args(tokens, parents, q_start, max_nodes)
-    if (probs.dim() != 2 or probs.shape[0] != T or probs.shape[1] < 1 or probs.device != dev or probs.stride(1) != 1
-            or probs.dtype not in (torch.float32, torch.bfloat16)):
-        raise ValueError(f"probs must be fp32 or bf16 [{T}, V] with contiguous rows on {dev}")
-    if draft_probs is not None and (draft_probs.shape != probs.shape or draft_probs.dtype != probs.dtype
-                                    or draft_probs.device != dev or draft_probs.stride(1) != 1):
+    shape, stride, dtype = probs.shape, probs.stride(), probs.dtype
+    if (len(shape) != 2 or shape[0] != T or shape[1] < 1 or probs.get_device() != dev or stride[1] != 1
+            or not (dtype is _F32 or dtype is _BF16)):
+        raise ValueError(f"probs must be fp32 or bf16 [{T}, V] with contiguous rows on {_name(dev)}")
+    if draft_probs is not None and (draft_probs.shape != shape or draft_probs.dtype is not dtype
+                                    or draft_probs.get_device() != dev or draft_probs.stride(1) != 1):
         raise ValueError("draft_probs must match probs in shape and type, with contiguous rows")
     for name, u, n in (("u_accept", u_accept, T), ("u_draw", u_draw, B)):
-        if u.dtype is not torch.float32 or u.shape != (n,) or not u.is_contiguous() or u.device != dev:
-            raise ValueError(f"{name} must be contiguous fp32 [{n}] on {dev}")
-    if not tokens.is_cuda:
+        if u.dtype is not _F32 or u.shape != (n,) or not u.is_contiguous() or u.get_device() != dev:
+            raise ValueError(f"{name} must be contiguous fp32 [{n}] on {_name(dev)}")
+    if dev < 0:
         return verify_tree_ref(probs, tokens, parents, q_start, max_nodes, u_accept, u_draw, draft_probs)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return verify_tree(probs, tokens, parents, q_start, max_nodes, u_accept, u_draw, draft_probs)
     v = _verdict(B, max_nodes, tokens)
-    N.call_packed("xtu_tree_verify", probs.data_ptr(), probs.stride(0), _ptr(draft_probs),
-           0 if draft_probs is None else draft_probs.stride(0), int(probs.dtype == torch.bfloat16), probs.shape[1],
-           tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(), B, T,
-           max_nodes, v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(),
-           _status(dev), N.stream_ptr(dev))
+    N.call_packed("xtu_tree_verify", probs.data_ptr(), stride[0], _ptr(draft_probs),
+                  0 if draft_probs is None else draft_probs.stride(0), dtype is _BF16, shape[1], tokens.data_ptr(),
+                  parents.data_ptr(), q_start.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(), B, T, max_nodes,
+                  v.accepted.data_ptr(), v.path.data_ptr(), v.tokens.data_ptr(), v.last_row.data_ptr(), _status(dev),
+                  _stream(dev))
     return v
 
 
@@ -513,41 +528,43 @@ def commit_tree(k_caches, v_caches, path: torch.Tensor, accepted: torch.Tensor, 
     if stacked:
         if k_caches.dim() != 5 or v_caches.dim() != 5:
             raise ValueError("stacked caches are [layers, blocks, Hkv, 64, D]")
-        k0, v0, kshape, vshape, L, Lv = k_caches, v_caches, k_caches.shape[1:], v_caches.shape[1:], \
-            k_caches.shape[0], v_caches.shape[0]
+        k0, v0 = k_caches, v_caches
+        L, *kshape = k0.shape
+        Lv, *vshape = v0.shape
     else:
         L, Lv = len(k_caches), len(v_caches)
         if L == 0 or L != Lv:
             raise ValueError("commit_tree takes as many K as V caches")
         k0, v0 = k_caches[0], v_caches[0]
-        kshape, vshape = k0.shape, v0.shape
+        kshape, vshape = list(k0.shape), list(v0.shape)
         if len(kshape) != 4 or len(vshape) != 4:
             raise ValueError("caches are [blocks, Hkv, 64, D] per layer")
     if L == 0 or L != Lv:
         raise ValueError("commit_tree takes as many K as V caches")
-    dev = k0.device
+    dev, dtype = k0.get_device(), k0.dtype
     nb, Hk, bs, D = kshape
-    fp8 = k0.dtype is _FP8
+    fp8 = dtype is _FP8
     Dv = vshape[2] if fp8 else vshape[3]
-    if vshape != ((nb, Hk, Dv, bs) if fp8 else (nb, Hk, bs, Dv)):
+    if vshape != ([nb, Hk, Dv, bs] if fp8 else [nb, Hk, bs, Dv]):
         raise ValueError(f"K and V caches {tuple(kshape)} and {tuple(vshape)} do not match")
     if bs != KV_BLOCK:
         raise ValueError(f"KV blocks hold 64 tokens, not {bs}")
-    if not fp8 and k0.dtype is not torch.bfloat16 and k0.is_cuda:
-        raise ValueError(f"the caches must be bfloat16 or float8_e4m3fn, not {k0.dtype}")
+    if not fp8 and dtype is not _BF16 and dev >= 0:
+        raise ValueError(f"the caches must be bfloat16 or float8_e4m3fn, not {dtype}")
     B, P = path.shape
     _ints("path", path, (B, P), dev)
     _ints("accepted", accepted, (B,), dev)
     _ints("q_start", q_start, (B + 1,), dev)
     _ints("kv_len", kv_len, (B,), dev)
-    _table(block_table, B, dev)
+    bt_stride, bt_cols = _table(block_table, B, dev)
+    kfull, vfull = k0.shape, v0.shape
     for k, v in ((k0, v0),) if stacked else zip(k_caches, v_caches):
-        if (k.shape != k0.shape or v.shape != v0.shape or k.dtype != k0.dtype or v.dtype != k0.dtype or k.device != dev
-                or v.device != dev):
+        if (k.shape != kfull or v.shape != vfull or k.dtype is not dtype or v.dtype is not dtype
+                or k.get_device() != dev or v.get_device() != dev):
             raise ValueError("the layers' caches must be alike")
         if not k.is_contiguous() or not v.is_contiguous():
             raise ValueError("the caches must be contiguous")
-    if not k0.is_cuda:
+    if dev < 0:
         commit_tree_ref(k_caches, v_caches, path, accepted, q_start, kv_len, block_table)
         return
     if _elsewhere(dev):
@@ -568,6 +585,6 @@ def commit_tree(k_caches, v_caches, path: torch.Tensor, accepted: torch.Tensor, 
         odd = any(x & 15 for x in kl) or any(x & 15 for x in vl)
     if odd:
         raise ValueError("the caches must start on 16-byte boundaries")
-    N.call_packed("xtu_tree_commit", kp, vp, kb, ks, vb, vs, L, path.data_ptr(), P, accepted.data_ptr(), q_start.data_ptr(),
-           kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], B, nb, Hk, D * es,
-           Dv * es, int(fp8), Dv, N.stream_ptr(dev))
+    N.call_packed("xtu_tree_commit", kp, vp, kb, ks, vb, vs, L, path.data_ptr(), P, accepted.data_ptr(),
+                  q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), bt_stride, bt_cols, B, nb, Hk, D * es,
+                  Dv * es, fp8, Dv, _stream(dev))
