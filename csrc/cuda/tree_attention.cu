@@ -81,6 +81,14 @@ __device__ __forceinline__ bool ta_wait(uint64_t* bar, uint32_t parity, XtuStatu
   return ta_wait_on(bar, parity, st, where, limit_ns);
 }
 
+// a first look whose answer is used later: the looks of several barriers are under way together
+__device__ __forceinline__ bool ta_look(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+
 // ---------------------------------------------------------------------------------------
 // visibility
 // ---------------------------------------------------------------------------------------
@@ -190,36 +198,38 @@ __device__ __forceinline__ uint32_t bad_bf16x2(uint32_t w) {
 // ---------------------------------------------------------------------------------------
 // the kernel: 128-row tiles, S, P and O in tensor memory
 // ---------------------------------------------------------------------------------------
-// One CTA = ROWT row tiles of 128 query rows of one (sequence, kv head, kv split).  Two softmax
-// units of 128 threads, a thread a row, keep the tensor core busy in turn:
-//   ROWT = 2  unit u owns row tile u; every K / V tile serves both
-//   ROWT = 1  both units own the same rows; unit u takes the key tiles t = u (mod 2) with a
-//             maximum, sum and accumulator of its own, and they merge at the end (SHARE: one
-//             accumulator, see there)
-//   warp 0       TMA producer: key tiles of BN keys into a ring (K0 V0 K1 V1 ..)
-//   warp 1       MMA issuer: S_u = Q K^T into TMEM, O_u += P_u V with P_u from TMEM, the units in turn
-//   warp 2       gives the ring's slots back
-//   warps 4-11   units 0 and 1: S_u -> registers, mask, online softmax, P_u (16 bit) over S_u's columns
-//   warps 12-15  fp8 caches: raw e4m3 tiles -> f16 operand tiles (exact)
-// The issuer alternates PV_u(t), S_u(t + 1): S_u's completion (one commit) also tells unit u that
-// PV_u(t) is done, so P and O need no barriers of their own and S and P share columns.
+// One CTA = ROWT row tiles of 128 query rows of one (sequence, kv head, kv split).  Softmax units of
+// 128 threads, a thread a row, keep the tensor core busy in turn:
+//   ROWT = 2  two units; unit u owns row tile u, and every K / V tile serves both
+//   ROWT = 1  three units (fp8 caches: two) share the rows, one accumulator and one running maximum; unit u
+//             takes the key tiles t = u (mod 3), and S runs three tiles ahead in buffers of its own
+//   warp 0       TMA producer: key tiles of BN keys into a ring (ROWT = 1: one for K, which runs ahead, one for V)
+//   warp 1       MMA issuer: S = Q K^T into TMEM, O += P V with P from TMEM
+//   warp 2       ROWT = 2: gives the ring's slots back
+//   warps 4 ..   the units: S -> registers, mask, online softmax, P (16 bit) over S's columns
+//   last 4       fp8 caches: raw e4m3 tiles -> f16 operand tiles (exact)
+// ROWT = 2: the issuer alternates PV_u(t), S_u(t + 1): S_u's completion (one commit) also tells unit u that
+// PV_u(t) is done, so P and O need no barriers of their own and S and P share columns.  ROWT = 1: PV(t), S(t + 3)
+// into the buffer that P(t) leaves; a unit that has to rescale O waits for the release of V(t - 1)'s slot.
 //
-// What bounds it.  A unit's way from S to the next S (TMEM load, max, 128 ex2, P, 256 + 512 cycles
+// What bounds it.  ROWT = 2: a unit's way from S to the next S (TMEM load, max, 128 ex2, P, 256 + 512 cycles
 // of MMA, and about 900 cycles of hand-overs) is 3300 cycles per 128-key tile while the
 // other unit's runs beside it; the MMAs of both take 2048 of them.  Measured with parts left
 // out: no exponentials -6 %, no softmax at all -8 %, 1/8 of the S products -27 %: the
 // chain, not one pipe.  Variants that were slower: two warps a row with half a row's keys each (266
 // against 227 us, 61-node case), 64-key tiles with S double-buffered (281: an N = 64 MMA costs as
 // much as an N = 128 one), ex2 partly as a cubic on the FMA pipe (no change), the maximum
-// taken between the exponentials (246: registers).
-// 4 sequences x 14.6K keys, 96 / 8 heads of 128 (KV 240 MB, 36 us at the copy rate), cold:
-//   60 rows a KV head (ROWT = 1)    46 us, DRAM 63 % of its peak (0.78 of the copy rate) + 4 us merge of 4 splits
-//   192 rows                        75 us + 6;  732 rows 179 us + 11 (153 GFLOP: 0.51 of the GEMM rate, MMA pipe
-//                                   52 % busy, XU 53 %)
-//   192 rows over the fp8 cache     82 us + 6: the same chain, and the second read of S that 128 registers
-//                                   force; its bytes are 18 us
-// 16 sequences of up to 12K keys, 16 / 2 heads of 256: 58 us + 5 (197 MB: 30 us).  A CTA's start and end cost
-// about 6 us, and 9 to 16 us is a call over a few pages.  Split counts: ops/tree.py.
+// taken between the exponentials (246: registers; with registers moved from the other warps no change).
+// ROWT = 1 takes that chain off the way of S (two units on alternate tiles with an accumulator each: 1.2 us a
+// tile against 0.85; 16 / 2 heads of 256 62.8 -> 57 us).  In long runs the card's power limit binds:
+// 1.65 of 1.97 GHz.
+// 4 sequences x 14.6K keys, 96 / 8 heads of 128 (KV 240 MB, 36 us at the copy rate), a call among others:
+//   60 rows a KV head   49 us (0.75 of the copy rate);  192 rows 67;  480 rows 110
+//   732 rows            172 to 190 us (153 GFLOP: 0.51 of the GEMM rate, MMA pipe 52 % busy, XU 53 %)
+//   192 rows over the fp8 cache  79 us: the same chain, and the second read of S that 128 registers
+//                       force (one read with registers moved: no change); its bytes are 18 us
+// 16 sequences of up to 12K keys, 16 / 2 heads of 256: 57 us (197 MB: 30 us; N = 64 products).  A CTA's start
+// and end cost about 6 us, and 9 to 16 us is a call over a few pages.  Split counts: ops/tree.py.
 //
 // Masked pages: a tile that hides a key from some row of the CTA (the tree's own, the last, those a
 // window cuts) is masked bit by bit in S, and V's non-finite values are zeroed in shared memory
@@ -229,16 +239,20 @@ struct TtCfg {
   static constexpr int D = D_, DVT = DVT_, BN = BN_, ROWT = ROWT_;
   static constexpr int NR = NR_;                       // slots of the raw ring (fp8 caches)
   static constexpr bool F8 = NR > 0;
-  // ROWT = 1: two accumulators fill the tensor memory at DVT = 128; wider heads share one, with one
-  // running maximum that goes from tile to tile (unit to unit)
-  static constexpr bool SHARE = ROWT == 1 && DVT > 128;
+  // ROWT = 1: one accumulator, with one running maximum that goes from tile to tile (unit to unit), which
+  // leaves tensor memory for a third S
+  static constexpr bool SHARE = ROWT == 1;
   static constexpr int NO = SHARE ? 1 : 2;             // accumulators
+  static constexpr int NSB = SHARE ? 3 : 2;            // S buffers: tile t in t % 3, or one a unit
+  static constexpr int LEAD = SHARE ? 3 : 1;           // K tiles loaded before the first V: K(t + LEAD) follows V(t)
   static constexpr int RAW = BN * D;                   // bytes of an fp8 tile
   static constexpr int Q_BYTES = ROWT * 128 * D * 2;
   static constexpr int K_BYTES = BN * D * 2, V_BYTES = BN * DVT * 2;
-  // one ring of SK + SV slots where a K and a V tile are the same size (K0 V0 K1 V1 ..; the count
-  // may be odd), else a ring each
-  static constexpr bool ONE = K_BYTES == V_BYTES;
+  // ROWT = 2: one ring of SK + SV slots where a K and a V tile are the same size (K0 V0 K1 V1 ..; the count
+  // may be odd); else a ring each
+  static constexpr bool ONE = !SHARE && K_BYTES == V_BYTES;
+  // slots that hold K, V
+  [[maybe_unused]] static constexpr int KS = ONE ? SK + SV : SK, VS = ONE ? SK + SV : SV;
   static constexpr int NS = SK + SV, RING = SK * K_BYTES + SV * V_BYTES;
   __device__ static int k_slot(int t) { return ONE ? 2 * t % NS : t % SK; }
   __device__ static int v_slot(int t) { return ONE ? (2 * t + 1) % NS : SK + t % SV; }
@@ -248,26 +262,51 @@ struct TtCfg {
   // tile t's K (V) slot is filled again before the last of nt tiles
   __device__ static bool k_again(int t, int nt) { return ONE ? 2 * t + NS < 2 * nt : t + SK < nt; }
   __device__ static bool v_again(int t, int nt) { return ONE ? 2 * t + 1 + NS < 2 * nt : t + SV < nt; }
-  static constexpr int BARS = 2 * NS + 2 * NR + 12;
-  static constexpr int BYTES = Q_BYTES + RING + NR * RAW + BARS * 8 + 16 + (SHARE ? 512 : 0);
-  static constexpr int O_COL = 2 * BN;                 // S0 S1 | O0 O1
-  static constexpr int P_COL = F8 ? BN / 2 : 0;        // P's first column in S's
+  // the in-th tile that is loaded (of 2 * nt): K or V, and its number
+  __device__ static bool order(int in, int nt, int& t) {
+    const int lead = LEAD < nt ? LEAD : nt, j = in - lead, pairs = nt - lead;
+    if (j < 0) { t = in; return false; }
+    if (j >= 2 * pairs) { t = j - pairs; return true; }
+    t = (j & 1) ? (j >> 1) + lead : j >> 1;
+    return !(j & 1);
+  }
+  static constexpr int BARS = 2 * NS + 2 * NR + 4 + 3 * NSB;
+  static constexpr int BYTES = Q_BYTES + RING + NR * RAW + BARS * 8 + 16 + (SHARE ? 1024 : 0);
+  static constexpr int O_COL = NSB * BN;               // S0 S1 (S2) | O0 (O1)
   static constexpr int COLS = 512;                     // (every tiling takes more than 256)
-  static constexpr int MLD = DVT + 4;                  // ROWT = 1: unit 1's O in shared memory (floats)
-  static constexpr int THREADS = F8 ? 512 : 384;
-  static_assert(2 * BN + NO * DVT <= 512, "tensor memory");
+  static constexpr int UNITS = SHARE && !F8 ? 3 : 2;   // softmax units of 128 threads
+  static constexpr int THREADS = 128 + 128 * UNITS + (F8 ? 128 : 0);
+  // with 128 registers a thread a unit takes 128 scores in two halves
+  static constexpr bool HALVES = THREADS == 512 && BN == 128;
+  static constexpr int P_COL = HALVES ? BN / 2 : 0;    // P's first column in S's
+  static_assert(NSB * BN + NO * DVT <= 512, "tensor memory");
   // ROWT = 2 gives V(t)'s slot back once S of tile t + 1 stands, whose K the producer must have loaded
   // before it comes to wait for that slot
   static_assert(ROWT == 1 || (ONE ? NS / 2 : SV) >= 1, "the ring would wait for itself");
   static_assert(BYTES <= 232448, "shared memory");
-  static_assert(ROWT == 2 || (SHARE ? 0 : 128 * MLD * 4) + 1024 <= RING, "merge buffer");
-  static_assert(!SHARE || !F8, "fp8 heads are 128 wide at most");
+  // ROWT = 1: a unit at tile t takes the release of V(t - 1)'s slot for the end of its product.  The slot's release
+  // before that has to be over by then: it is tile t - 3's or older, whose product stands before S(t)
+  static_assert(!SHARE || SV >= 2, "the release of a V slot would be ambiguous");
   static_assert(D % 64 == 0 && DVT % 64 == 0 && BN % 64 == 0 && NS >= 3 && (!F8 || (D == DVT && BN == 128 && NR >= 2)), "tiles");
 };
 
 // 16 bytes to shared memory without a register stop; zeros when `there` is false
 __device__ __forceinline__ void tt_copy16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+// a row's running maximum with the tile that it is of, in one 8-byte access of shared memory
+__device__ __forceinline__ void ta_row_max_to(int2* at, float m, int tile) {
+  asm volatile("st.volatile.shared.v2.b32 [%0], {%1, %2};" ::"r"(smem_u32(at)), "r"(__float_as_int(m)), "r"(tile) : "memory");
+}
+__device__ __forceinline__ float ta_row_max(const int2* at, int tile, bool& ok) {   // waits for that tile, bounded
+  int m, of, it = 0;
+#pragma unroll 1
+  do {
+    asm volatile("ld.volatile.shared.v2.b32 {%0, %1}, [%2];" : "=r"(m), "=r"(of) : "r"(smem_u32(at)) : "memory");
+  } while (of != tile && ++it < (1 << 24));
+  ok = of == tile;
+  return __int_as_float(m);
 }
 
 // pairs of floats in one instruction
@@ -309,13 +348,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
   uint64_t* r_full = empty + C::NS;                    // [NR]
   uint64_t* r_empty = r_full + C::NR;                  // [NR]
   uint64_t* q_ready = r_empty + C::NR;
-  uint64_t* s_full = q_ready + 1;                      // [2]
-  uint64_t* p_full = s_full + 2;                       // [2][2] halves of P
-  uint64_t* o_done = p_full + 4;                       // [2], and one for an issuer that gives up
-  uint64_t* checked = o_done + 3;                      // [2] SHARE: the unit's tile has its maximum in m_row
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(checked + 2);
+  uint64_t* s_full = q_ready + 1;                      // [NSB]
+  uint64_t* p_full = s_full + C::NSB;                  // [NSB][2] halves of P
+  uint64_t* o_done = p_full + 2 * C::NSB;                     // [2], and one for an issuer that gives up
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 3);
   int& s_bad = *reinterpret_cast<int*>(tmem_slot + 1);   // a masked tile held a non-finite value
-  float* m_row = reinterpret_cast<float*>(tmem_slot + 2);  // [128] SHARE: the rows' running maximum
+  // SHARE: [128] the rows' running maximum, and the tile that it is of: the unit of the next tile waits for it.  (A
+  // barrier and a load behind it took 500 cycles more a tile.)
+  int2* m_row = reinterpret_cast<int2*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, kh = blockIdx.y;
@@ -342,7 +382,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
   // tiles at or past `shut` or below `open` hide keys from some rows (see the masked pages above)
   const int shut = ctx / BN;
   const int open = p.window > 0 ? (max(0, ctx + n - p.window) + BN - 1) / BN : 0;
-  const bool two = ROWT == 2 ? r0 + 128 < rows_all : nt > 1;   // unit 1 has work
+  const bool two = ROWT == 2 && r0 + 128 < rows_all;   // unit 1 has a row tile
 
   if (threadIdx.x == 0) {
     // (nodes that the grid does not cover, keys that the table does not name: cut, and told)
@@ -353,11 +393,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     s_bad = 0;
     for (int i = 0; i < C::NS; ++i) { mbar_init(&full[i], C::F8 ? 4 : 1); mbar_init(&empty[i], 1); }
     for (int i = 0; i < C::NR; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], 4); }
-    mbar_init(q_ready, 8);
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&o_done[i], 1); mbar_init(&checked[i], 4); }
-    for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
+    mbar_init(q_ready, 4 * C::UNITS);
+    for (int i = 0; i < 2; ++i) mbar_init(&o_done[i], 1);
+    for (int i = 0; i < C::NSB; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[2 * i], 4); mbar_init(&p_full[2 * i + 1], 4); }
     fence_barrier_init();
   }
+  if (C::SHARE && threadIdx.x >= 128 && threadIdx.x < 256) m_row[threadIdx.x - 128] = make_int2(0, -1);
   if (warp == 1) tmem_alloc(tmem_slot, C::COLS);
   tc_fence_before();
   __syncthreads();
@@ -379,56 +420,65 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         if (pg < 0 || pg > p.num_blocks) pg = p.num_blocks;
         return (pg * p.Hkv + kh) * TA_PAGE;
       };
+      // (a V tile's pages are looked up with its K's; LEAD is 1 or 3)
+      int krow[PPT], vrow[C::LEAD][PPT];
       bool ok = true;
-      int krow[PPT], vrow[PPT];
+      int in = 0, kn = 0, vn = 0;
 #pragma unroll
       for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(0, sb);
-      if constexpr (C::F8) {   // K0 V0 K1 V1 .. as they lie: K [64 keys][D bytes], V [DV columns][64 keys] a page
-        int in = 0;
-        for (; in < 2 * nt && ok; ++in) {
-          const int slot = in % C::NR, turn = in / C::NR;
-          if ((in & 1) == 0 && in > 0) {
+      for (; in < 2 * nt && ok; ++in) {
+        int t;
+        const bool isv = C::order(in, nt, t);
+        int rows[PPT];
 #pragma unroll
-            for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(in >> 1, sb);
-          }
+        for (int sb = 0; sb < PPT; ++sb) rows[sb] = isv ? vrow[0][sb] : krow[sb];
+        if constexpr (C::F8) {   // as they lie: K [64 keys][D bytes], V [DV columns][64 keys] a page
+          const int slot = in % C::NR, turn = in / C::NR;
           ok = turn == 0 || ta_wait(&r_empty[slot], (turn - 1) & 1, p.status, 150);
           if (!ok) break;
           mbar_arrive_expect_tx(&r_full[slot], C::RAW);
 #pragma unroll
           for (int sb = 0; sb < PPT; ++sb)
-            tma_load_2d(raw + slot * C::RAW + sb * TA_PAGE * D, in & 1 ? &tv : &tk, &r_full[slot], 0,
-                        in & 1 ? krow[sb] / TA_PAGE * DVT : krow[sb]);
-        }
-        if (!ok)   // let the copies in flight land (bounded) before the CTA ends
-          for (int i = max(0, in - C::NR); i < in; ++i) ta_wait(&r_full[i % C::NR], (i / C::NR) & 1, nullptr, 0, 50000000ull);
-      } else {
-        int kn = 0, vn = 0;
-        auto load = [&](int slot, int turn, int bytes, const CUtensorMap* map, int cols, const int (&rows)[PPT], int site) {
-          if (turn > 0 && !ta_wait(&empty[slot], (turn - 1) & 1, p.status, site)) return false;
-          mbar_arrive_expect_tx(&full[slot], bytes);
+            tma_load_2d(raw + slot * C::RAW + sb * TA_PAGE * D, isv ? &tv : &tk, &r_full[slot], 0,
+                        isv ? rows[sb] / TA_PAGE * DVT : rows[sb]);
+        } else {
+          const int slot = isv ? C::v_slot(t) : C::k_slot(t), turn = isv ? C::v_turn(t) : C::k_turn(t);
+          ok = turn == 0 || ta_wait(&empty[slot], (turn - 1) & 1, p.status, isv ? 151 : 150);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full[slot], isv ? C::V_BYTES : C::K_BYTES);
           uint8_t* dst = sK + C::slot_at(slot);
-  #pragma unroll
+#pragma unroll
           for (int sb = 0; sb < PPT; ++sb)
-  #pragma unroll
-            for (int c = 0; c < cols / 64; ++c)
-              tma_load_2d(dst + c * (BN * 128) + sb * (TA_PAGE * 128), map, &full[slot], c * 64, rows[sb]);
-          return true;
-        };
-        for (int t = 0; t < nt && ok; ++t) {
-          ok = load(C::k_slot(t), C::k_turn(t), C::K_BYTES, &tk, D, krow, 150);
-          kn += ok;
-  #pragma unroll
-          for (int sb = 0; sb < PPT; ++sb) vrow[sb] = krow[sb];
-          if (t + 1 < nt) {
-  #pragma unroll
-            for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(t + 1, sb);   // under way while V's slot gets free
-          }
-          ok = ok && load(C::v_slot(t), C::v_turn(t), C::V_BYTES, &tv, DVT, vrow, 151);
-          vn += ok;
+#pragma unroll
+            for (int c = 0; c < (D > DVT ? D : DVT) / 64; ++c)
+              if (c < (isv ? DVT : D) / 64)
+                tma_load_2d(dst + c * (BN * 128) + sb * (TA_PAGE * 128), isv ? &tv : &tk, &full[slot], c * 64, rows[sb]);
         }
-        if (!ok) {   // let the copies in flight land (bounded) before the CTA ends
-          for (int t = max(0, kn - C::NS); t < kn; ++t) ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, nullptr, 0, 50000000ull);
-          for (int t = max(0, vn - C::NS); t < vn; ++t) ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, nullptr, 0, 50000000ull);
+        if (isv) {
+          ++vn;
+#pragma unroll
+          for (int k = 0; k + 1 < C::LEAD; ++k)
+#pragma unroll
+            for (int sb = 0; sb < PPT; ++sb) vrow[k][sb] = vrow[k + 1][sb];
+        } else {   // queue the pages for V, look up the next tile's while slots get free
+          const int at = C::LEAD == 1 ? 0 : kn - vn;
+#pragma unroll
+          for (int k = 0; k < C::LEAD; ++k)
+#pragma unroll
+            for (int sb = 0; sb < PPT; ++sb) vrow[k][sb] = k == at ? krow[sb] : vrow[k][sb];
+          ++kn;
+          if (kn < nt) {
+#pragma unroll
+            for (int sb = 0; sb < PPT; ++sb) krow[sb] = row_of(kn, sb);
+          }
+        }
+      }
+      if (!ok) {   // let the copies in flight land (bounded) before the CTA ends
+        if constexpr (C::F8) {
+          for (int i = max(0, in - C::NR); i < in; ++i) ta_wait(&r_full[i % C::NR], (i / C::NR) & 1, nullptr, 0, 50000000ull);
+        } else {
+          for (int t = max(0, kn - C::KS); t < kn; ++t) ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, nullptr, 0, 50000000ull);
+          for (int t = max(0, vn - C::VS); t < vn; ++t) ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, nullptr, 0, 50000000ull);
         }
       }
     }
@@ -440,69 +490,88 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       constexpr uint32_t id_s = C::F8 ? idesc_bf16_f32(128, BN, 0, 0) & ~types : idesc_bf16_f32(128, BN, 0, 0);
       constexpr uint32_t id_o = C::F8 ? idesc_bf16_f32(128, DVT, 0, 0) & ~types : idesc_bf16_f32(128, DVT, 0, 1);
       bool ok = ta_wait(q_ready, 0, p.status, 152);
-      auto tile_of = [&](int u, int i) { return ROWT == 2 ? i : 2 * i + u; };   // unit u's i-th tile
       auto wait_k = [&](int t) { return ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, p.status, 153); };
       auto wait_v = [&](int t) { return ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, p.status, 154); };
-      // S_u = Q_u K^T of the unit's i-th tile
-      auto mma_s = [&](int u, int i) {
-        const uint64_t qd = sdesc_kmajor_sw128(smem_u32(sQ) + (ROWT == 2 ? u * (128 * D * 2) : 0));
-        const uint64_t kd = sdesc_kmajor_sw128(smem_u32(sK + C::slot_at(C::k_slot(tile_of(u, i)))));
+      // S = Q K^T of tile t into buffer sb (ROWT = 2: of unit sb)
+      auto mma_s = [&](int sb, int t) {
+        const uint64_t qd = sdesc_kmajor_sw128(smem_u32(sQ) + (ROWT == 2 ? sb * (128 * D * 2) : 0));
+        const uint64_t kd = sdesc_kmajor_sw128(smem_u32(sK + C::slot_at(C::k_slot(t))));
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)   // (descriptors count 16 bytes)
-          mma_f16_ss(tmem + u * BN, qd + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16,
+          mma_f16_ss(tmem + sb * BN, qd + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16,
                      kd + ((k >> 2) * (BN * 128) + (k & 3) * 32) / 16, id_s, k > 0);
-        mma_commit(&s_full[u]);
+        mma_commit(&s_full[sb]);
       };
-      // O_u += P_u V of its i-th tile, the two halves of the keys as P_u gets ready
-      auto mma_o = [&](int u, int i) {
-        const uint32_t va = smem_u32(sK + C::slot_at(C::v_slot(tile_of(u, i))));
+      // O (of accumulator o) += P V of tile t, the two halves of the keys as P gets ready in buffer sb
+      auto mma_o = [&](int o, int sb, int t, int phase) {
+        const uint32_t va = smem_u32(sK + C::slot_at(C::v_slot(t)));
         const uint64_t vd = C::F8 ? sdesc_kmajor_sw128(va) : sdesc_mnmajor_sw128(va, BN * 128, 1024);
+        const bool there[2] = {ta_look(&p_full[2 * sb], phase), ta_look(&p_full[2 * sb + 1], phase)};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (!ta_wait(&p_full[2 * u + h], i & 1, p.status, 155)) return false;
+          if (!there[h] && !ta_wait(&p_full[2 * sb + h], phase, p.status, 155)) return false;
           tc_fence_after();
 #pragma unroll
           for (int e = 0; e < BN / 32; ++e) {
-            const int k = (h ^ C::F8) * (BN / 32) + e;                 // fp8: the second half of the keys first
-            mma_f16_ts(tmem + C::O_COL + u % C::NO * DVT, tmem + u * BN + C::P_COL + k * 8,
+            const int k = (h ^ C::HALVES) * (BN / 32) + e;             // (halves: the second half of the keys first)
+            mma_f16_ts(tmem + C::O_COL + o * DVT, tmem + sb * BN + C::P_COL + k * 8,
                        vd + (C::F8 ? ((k >> 2) * (DVT * 128) + (k & 3) * 32) / 16 : k * 128), id_o,
-                       !(i == 0 && h == 0 && e == 0 && (!C::SHARE || u == 0)));
+                       !(t == 0 && h == 0 && e == 0));
           }
         }
         return true;
       };
-      // the units in turn: PV of the unit's i-th tile, then S of its next
-      const int n0 = ROWT == 2 ? nt : (nt + 1) / 2, n1 = !two ? 0 : ROWT == 2 ? nt : nt / 2;   // the units' tiles
-      for (int u = 0; u < 2 && ok; ++u) {
-        if (u == 1 && n1 == 0) break;
-        ok = (ROWT == 2 && u == 1) || wait_k(tile_of(u, 0));
-        tc_fence_after();
-        if (ok) mma_s(u, 0);
-      }
       // (a wait costs the issuer 100 cycles or more even when it is over, and the issuer's way from P to the
-      // next S is on every unit's path: the waits for K and V come before P's, and once for both
-      // units where they share the tiles)
-      for (int i = 0; i < n0 && ok; ++i) {
-#pragma unroll 1
-        for (int u = 0; u < 2; ++u) {
-          const int nu = u == 0 ? n0 : n1;
-          if (i >= nu) continue;
-          const int t = tile_of(u, i);
-          if (ROWT == 1) {
-            // tiles of one row tile are half as long: PV must not wait for K of the tile after next, and V's
-            // slot goes back by a commit of its own, an S earlier than by the recycler
-            ok = wait_v(t) && mma_o(u, i);
-            if (ok && C::v_again(t, nt)) mma_commit(&empty[C::v_slot(t)]);
-            ok = ok && (i + 1 >= nu || wait_k(tile_of(u, i + 1)));
-          } else {
-            // (fp8: K is still being widened when PV may start)
-            if (u == 0) ok = wait_v(t) && (C::F8 || i + 1 >= nu || wait_k(t + 1));
-            ok = ok && mma_o(u, i);
-            if (C::F8 && u == 0) ok = ok && (i + 1 >= nu || wait_k(t + 1));
+      // next S is on every unit's path)
+      if constexpr (ROWT == 1) {
+        // S three tiles ahead; PV of a tile, then S into the buffer that it leaves.  K's and V's slots go back by
+        // commits of their own
+        auto next_s = [&](int sb, int t) {
+          tc_fence_after();
+          mma_s(sb, t);
+          if (C::k_again(t, nt)) mma_commit(&empty[C::k_slot(t)]);
+        };
+        for (int t = 0; t < min(nt, C::NSB) && ok; ++t) {
+          ok = wait_k(t);
+          if (ok) next_s(t, t);
+        }
+        int sb = 0, phase = 0;
+        for (int t = 0; t < nt && ok; ++t) {
+          const bool more = t + C::NSB < nt;
+          uint64_t *fv = &full[C::v_slot(t)], *fk = &full[C::k_slot(t + C::NSB)];
+          const uint32_t pv = C::v_turn(t) & 1, pk = C::k_turn(t + C::NSB) & 1;
+          const bool v_there = ta_look(fv, pv), k_there = ta_look(fk, pk);
+          ok = v_there || ta_wait(fv, pv, p.status, 154);
+          ok = ok && mma_o(0, sb, t, phase);
+          if (ok) mma_commit(&empty[C::v_slot(t)]);
+          if (ok && more) {
+            ok = k_there || ta_wait(fk, pk, p.status, 153);
+            if (ok) next_s(sb, t + C::NSB);
           }
-          if (!ok) break;
-          if (i + 1 < nu) mma_s(u, i + 1);
-          else mma_commit(&o_done[u]);
+          if (++sb == C::NSB) {
+            sb = 0;
+            phase ^= 1;
+          }
+        }
+        if (ok) mma_commit(&o_done[0]);
+      } else {
+        // the units in turn: PV of a tile, then S of the next.  The waits for K and V come before P's, and once
+        // for both units
+        const int units = two ? 2 : 1;
+        ok = ok && wait_k(0);
+        tc_fence_after();
+        for (int u = 0; u < units && ok; ++u) mma_s(u, 0);
+        for (int t = 0; t < nt && ok; ++t) {
+#pragma unroll 1
+          for (int u = 0; u < units; ++u) {
+            // (fp8: K is still being widened when PV may start)
+            if (u == 0) ok = wait_v(t) && (C::F8 || t + 1 >= nt || wait_k(t + 1));
+            ok = ok && mma_o(u, u, t, t & 1);
+            if (C::F8 && u == 0) ok = ok && (t + 1 >= nt || wait_k(t + 1));
+            if (!ok) break;
+            if (t + 1 < nt) mma_s(u, t + 1);
+            else mma_commit(&o_done[u]);
+          }
         }
       }
       if (!ok) {   // the MMAs in flight end before the CTA gives its tensor memory back
@@ -514,17 +583,16 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       }
     }
   } else if (warp == 2) {
-    // ------------------------------------------------------------ slots back to the producer
-    // A unit's S of a tile stands (s_full): K of that tile is done with, and with two units on the same
-    // tiles (the one that is served last speaks for both) V of the tile before, whose PV the
-    // issuer put before that S.  (Softmax threads' arrivals cost their warp 350 cycles a tile.)
-    if (elect_one()) {
+    // ------------------------------------------------------------ slots back to the producer (ROWT = 2)
+    // S of a tile stands for the unit that is served last (s_full): K of that tile is done with, and V of the
+    // tile before, whose PV the issuer put before that S.  (Softmax threads' arrivals cost their warp 350
+    // cycles a tile.)
+    if (ROWT == 2 && elect_one()) {
       bool ok = true;
       for (int t = 0; t < nt && ok; ++t) {
-        const int u = ROWT == 2 ? (two ? 1 : 0) : t & 1;
-        const bool k = C::k_again(t, nt), v = ROWT == 2 && t > 0 && C::v_again(t - 1, nt);
+        const bool k = C::k_again(t, nt), v = t > 0 && C::v_again(t - 1, nt);
         if (!k && !v) continue;
-        ok = ta_wait(&s_full[u], (ROWT == 2 ? t : t >> 1) & 1, p.status, 159);
+        ok = ta_wait(&s_full[two ? 1 : 0], t & 1, p.status, 159);
         if (!ok) break;
         if (k) mbar_arrive(&empty[C::k_slot(t)]);
         if (v) mbar_arrive(&empty[C::v_slot(t - 1)]);
@@ -536,8 +604,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       const int ct = threadIdx.x - 384;
       bool ok = true;
       for (int in = 0; in < 2 * nt && ok; ++in) {
-        const int rs = in % C::NR, t = in >> 1;
-        const bool isv = in & 1;
+        const int rs = in % C::NR;
+        int t;
+        const bool isv = C::order(in, nt, t);
         const int slot = isv ? C::v_slot(t) : C::k_slot(t), turn = isv ? C::v_turn(t) : C::k_turn(t);
         ok = ta_wait(&r_full[rs], (in / C::NR) & 1, p.status, 162) &&
              (turn == 0 || ta_wait(&empty[slot], (turn - 1) & 1, p.status, 163));
@@ -581,7 +650,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     {
       // Q, whole rows at a time: D / 8 lanes a row (a thread a row touched 32 lines a load: 5 us).
       // 128B-swizzled K-major chunks of [128 rows][64 columns]
-      constexpr int PR = D / 8, TH = ROWT == 2 ? 128 : 256;     // pieces of a row, threads of this tile
+      constexpr int PR = D / 8, TH = ROWT == 2 ? 128 : 128 * C::UNITS;     // pieces of a row, threads of this tile
       uint8_t* dst = sQ + (ROWT == 2 ? u * (128 * D * 2) : 0);
       const int base = r0 + (ROWT == 2 ? u * 128 : 0);
 #pragma unroll 4
@@ -609,14 +678,16 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       if (lane == 0) mbar_arrive(q_ready);
     }
     const uint32_t lanes = (uint32_t)(qd * 32) << 16;
-    const uint32_t s_t = tmem + lanes + u * BN, o_t = tmem + lanes + C::O_COL + u % C::NO * DVT;
+    const uint32_t o_t = tmem + lanes + C::O_COL + u % C::NO * DVT;
     float m = -FLT_MAX, l = 0.f;                       // running maximum (log2 units) and sum
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
-    const int mine = ROWT == 2 ? ((u == 0 || two) ? nt : 0) : (nt - u + 1) / 2;   // this unit's tiles
+    const int mine = ROWT == 2 ? ((u == 0 || two) ? nt : 0) : (nt - u + C::UNITS - 1) / C::UNITS;   // this unit's tiles
     for (int i = 0; i < mine; ++i) {
-      const int t = ROWT == 2 ? i : 2 * i + u;
+      const int t = ROWT == 2 ? i : C::UNITS * i + u;
       const int at = t0 + t;                           // key tile
+      const int buf = ROWT == 2 ? u : t % C::NSB, phase = (ROWT == 2 ? t : t / C::NSB) & 1;
+      const uint32_t s_t = tmem + lanes + buf * BN;
       const bool msk = at >= shut || at < open;
       if (msk) {
         // V's non-finite values become zero (0 * p must stay 0 for keys that a row does not
@@ -637,12 +708,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         }
         fence_proxy_async_smem();
       }
-      ok = ta_wait(&s_full[u], i & 1, p.status, 157);
+      ok = ta_wait(&s_full[buf], phase, p.status, 157);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       // HW columns of S in registers at a time: all of them, or with 16 warps' share of the registers (fp8) a half
-      constexpr int HW = C::F8 ? BN / 2 : BN;
+      constexpr int HW = C::HALVES ? BN / 2 : BN;
       uint32_t sv[HW];
       auto fetch = [&](int c0) {
 #pragma unroll
@@ -670,10 +741,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       if (mx != -FLT_MAX) mx *= p.scale_log2;
       if constexpr (C::SHARE) {
         if (t > 0) {                                   // the maximum that the tile before (the other unit's) left
-          ok = ta_wait(&checked[u ^ 1], (u == 0 ? i - 1 : i) & 1, p.status, 164);
+          const float m_now = ta_row_max(&m_row[r], t - 1, ok);
+          if (!ok) report_error(p.status, XTU_ERR_MBAR_TIMEOUT, 164, t);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const float m_now = m_row[r];
           if (m_now != m) {
             if (m != -FLT_MAX) l *= ta_ex2(m - m_now);
             m = m_now;
@@ -687,9 +758,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       if (__any_sync(0xffffffffu, rescale)) {
         const float f = rescale ? ta_ex2(m - m_new) : 1.f;
         l *= f;
-        if constexpr (C::SHARE) {   // PV of the tile before is done once S of the tile after stands (the issuer's order)
-          ok = t + 1 < nt ? ta_wait(&s_full[u ^ 1], ((t + 1) >> 1) & 1, p.status, 165)
-                          : ta_wait(&o_done[u ^ 1], 0, p.status, 166);
+        if constexpr (C::SHARE) {   // PV of the tile before is done once it gave its V slot back
+          ok = ta_wait(&empty[C::v_slot(t - 1)], C::v_turn(t - 1) & 1, p.status, 165);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -706,9 +776,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       }
       m = m_new;
       if constexpr (C::SHARE) {
-        m_row[r] = m;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&checked[u]);
+        ta_row_max_to(&m_row[r], m, t);
       }
       const float neg = m == -FLT_MAX ? 0.f : -m;
       const float2 ng2 = make_float2(neg, neg);
@@ -729,9 +797,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * u + h]);
+        if (lane == 0) mbar_arrive(&p_full[2 * buf + h]);
       };
-      if constexpr (C::F8) {   // the second half is at hand; P lies over its S, so the first half's still stands
+      if constexpr (C::HALVES) {   // the second half is at hand; P lies over its S, so the first half's still stands
 #pragma unroll
         for (int c = 0; c < HW; c += 32) weigh(c, (HW + c) / 2);
         hand_over(0);
@@ -749,71 +817,35 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
     }
     // ---- end: O / l
-    bool have = mine > 0 && ok;
+    bool have = ok && (C::SHARE ? nt : mine) > 0;
     if (have) {
-      have = ta_wait(&o_done[u], 0, p.status, 158);
+      have = ta_wait(&o_done[C::SHARE ? 0 : u], 0, p.status, 158);
       have = __all_sync(0xffffffffu, have);
       tc_fence_after();
     }
     const bool valid = rr < rows_all;
     const int node = valid ? ta_node(p, rr) : 0, head = kh * p.G + (valid ? rr - node * p.G : 0), tok = q0 + node;
-    float M = m, scale_own = 1.f, f1 = 0.f;
-    const float* oth = nullptr;
+    float M = m;
     if constexpr (C::SHARE) {
-      // one accumulator, each unit's part of the sum in its own last maximum; a unit writes half of the columns.
-      // (O is complete once both units' last products are)
-      if (ok && nt > 0 && (two || u == 1)) {
-        have = ta_wait(&o_done[u ^ 1], 0, p.status, 167);
-        have = __all_sync(0xffffffffu, have);
-        tc_fence_after();
-      }
-      float* ml = reinterpret_cast<float*>(sK);                       // [2 units][m, l][128]
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      // one accumulator, each unit's part of the sum in its own last maximum; a unit writes half of the columns
+      // (with the products done the ring is free)
+      float* ml = reinterpret_cast<float*>(sK);                       // [units][m, l][128]
+      asm volatile("bar.sync 1, %0;" ::"n"(128 * C::UNITS) : "memory");
       ml[u * 256 + r] = mine > 0 ? m : -FLT_MAX;
       ml[u * 256 + 128 + r] = mine > 0 ? l : 0.f;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      M = fmaxf(ml[r], ml[256 + r]);
+      asm volatile("bar.sync 1, %0;" ::"n"(128 * C::UNITS) : "memory");
+      for (int w = 0; w < C::UNITS; ++w) M = fmaxf(M, ml[w * 256 + r]);
       l = 0.f;
-      for (int w = 0; w < 2; ++w) {
+      for (int w = 0; w < C::UNITS; ++w) {
         const float mw = ml[w * 256 + r], lw = ml[w * 256 + 128 + r];
         l += mw == -FLT_MAX ? (lw != lw ? lw : 0.f) : lw * ta_ex2(mw - M);
       }
-    } else if (ROWT == 1) {
-      // unit 1's rows meet unit 0's in shared memory: with both units done the ring is free
-      float* mo = reinterpret_cast<float*>(sK);                       // [128][MLD]
-      float* ml = mo + 128 * C::MLD;                                  // [2][128]
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (u == 1) {
-        ml[r] = have ? m : -FLT_MAX;
-        ml[128 + r] = have ? l : 0.f;
-        if (have) {
-#pragma unroll 1
-          for (int c = 0; c < DVT; c += 32) {
-            uint32_t x[32];
-            tmem_ld32(o_t + c, x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(mo + r * C::MLD + c + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-          }
-        }
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (u == 0 && two) {
-        const float m1 = ml[r], l1 = ml[128 + r];
-        M = fmaxf(m, m1);
-        scale_own = m == -FLT_MAX ? (l != l ? l : 0.f) : ta_ex2(m - M);
-        f1 = m1 == -FLT_MAX ? (l1 != l1 ? l1 : 0.f) : ta_ex2(m1 - M);
-        l = l * scale_own + l1 * f1;
-        oth = mo + r * C::MLD;
-      }
     }
-    if (ROWT == 2 ? (u == 0 || two) : C::SHARE || u == 0) {
+    if (C::SHARE ? u < 2 : u == 0 || two) {
       if (p.sinks != nullptr && p.splits == 1 && M != -FLT_MAX && valid) l += ta_ex2(__ldg(p.sinks + head) * LOG2E - M);
       const float inv = l > 0.f || l != l ? p.out_scale / l : 0.f;
       const size_t at = ((size_t)tok * p.Hq + head) * DVT;
       float* wo = p.splits > 1 ? p.ws_o + (size_t)sp * p.T * p.Hq * DVT + at : nullptr;
-      const float sc0 = scale_own * inv, sc1 = f1 * inv;
 #pragma unroll 1
       for (int c = C::SHARE ? u * (DVT / 2) : 0; c < (C::SHARE ? (u + 1) * (DVT / 2) : DVT); c += 32) {
         uint32_t x[32];
@@ -824,17 +856,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
         if (!valid) continue;
         float v[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = have ? __uint_as_float(x[e]) * sc0 : 0.f;
-        if (oth != nullptr) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 y = *reinterpret_cast<const float4*>(oth + c + e);
-            v[e] += y.x * sc1;
-            v[e + 1] += y.y * sc1;
-            v[e + 2] += y.z * sc1;
-            v[e + 3] += y.w * sc1;
-          }
-        }
+        for (int e = 0; e < 32; ++e) v[e] = have ? __uint_as_float(x[e]) * inv : 0.f;
         if (wo == nullptr) {
           uint4* d4 = reinterpret_cast<uint4*>(p.o + at + c);
 #pragma unroll
@@ -987,10 +1009,8 @@ int tt_launch(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, i
   return e == cudaSuccess ? 1 : -(int)e;
 }
 
-// rows: of the largest tree.  row_tiles = 2: two row tiles a CTA that share their K / V tiles (732 rows:
-// 182 us against 197 with one a CTA); 1: one, the units on alternate key tiles (60 rows, 2 splits: 74 us
-// against 109 with an idle unit; 312 rows of a 128-key window: 18.6 against 24.6, twice the
-// CTAs).  The host weighs them (ops/tree.py).
+// rows: of the largest tree.  row_tiles = 2: two row tiles a CTA that share their K / V tiles; 1: one, and
+// twice the CTAs.  The host weighs them (ops/tree.py, both sides measured there).
 template <class ONE, class TWO>
 int tt_rows(const CUtensorMap& tk, const CUtensorMap& tv, const TaParams& p, int rows, int row_tiles, int B,
             cudaStream_t s) {

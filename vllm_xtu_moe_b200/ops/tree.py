@@ -196,28 +196,30 @@ def tree_attention_ref(q, k_cache, v_cache, meta: TreeMetadata, scale: float, ou
 
 
 @functools.lru_cache(maxsize=4096)
-def _plan(groups: int, rows: int, keys: int, one: bool, splits: int, num_sms: int) -> tuple[int, int]:
+def _plan(groups: int, rows: int, keys: int, one: bool, one_us: float, splits: int, num_sms: int) -> tuple[int, int]:
     best = None
     for tiles in ((1,) if one or rows <= 128 else (1, 2)):
         ctas = max(1, -(-rows // (128 * tiles)) * groups)
         for s in ((splits,) if splits else range(1, max(1, min(MAX_SPLITS, keys)) + 1)):
-            cost = -(-ctas * s // num_sms) * (-(-keys // s) * (1.8 if tiles == 2 else 1.2) + 9) + (7 if s > 1 else 0)
+            cost = -(-ctas * s // num_sms) * (-(-keys // s) * (1.8 if tiles == 2 else one_us) + 9) + (7 if s > 1 else 0)
             if best is None or cost < best[0]:
                 best = (cost, tiles, s)
     return best[1], best[2]
 
 
 def tree_plan(num_seqs: int, num_kv_heads: int, rows: int, seen: int, d: int = 128, dv: int = 128, splits: int = 0,
-              num_sms: int = 148) -> tuple[int, int]:
+              fp8: bool = False, num_sms: int = 148) -> tuple[int, int]:
     """(row tiles of a CTA, KV splits) of a step.  ``rows``: query rows of the largest tree per KV head,
     ``seen``: keys that a sequence attends to, ``splits``: a split count that is given.
 
     One CTA per SM takes one or two 128-row tiles of a (sequence, KV head, split).  In microseconds a
-    key tile costs about 1.8 for two row tiles and 1.2 for one, a CTA's start and end 9 and the merge
-    of the splits 7, so the time is about waves * (key tiles per split * that + 9) + 7.  Measured (4 x
-    14.6K keys, 8 KV heads): 732 rows, two row tiles 223 / 182 us at 1 / 3 splits, one 197 at 3; 192 rows,
-    two 82 / 86 at 4 / 9 splits, one 80 at 2."""
-    return _plan(num_seqs * num_kv_heads, rows, -(-seen // (128 if d <= 128 else 64)), dv > 128, splits, num_sms)
+    key tile costs about 1.8 for two row tiles and 0.85 for one (1.55 from fp8, 1.2 of 256-wide heads),
+    a CTA's start and end 9 and the merge of the splits 7, so the time is about
+    waves * (key tiles per split * that + 9) + 7.  Measured (4 x 14.6K keys, 8 KV heads), one / two row
+    tiles at their best splits: 192 rows 67 / 72 us, 480 rows 110 / 128, 732 rows 193 / 172; fp8: 192
+    rows 107 / 79, 60 rows 56 / 61."""
+    one_us = 1.55 if fp8 else 0.85 if dv <= 128 else 1.2
+    return _plan(num_seqs * num_kv_heads, rows, -(-seen // (128 if d <= 128 else 64)), dv > 128, one_us, splits, num_sms)
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta: TreeMetadata,
@@ -302,7 +304,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError("q rows must be contiguous and start on 16-byte boundaries")
     rows = most * (Hq // Hk)
     seen = min(meta.max_kv_len, window + most + KV_BLOCK) if window > 0 else meta.max_kv_len
-    tiles, splits = tree_plan(B, Hk, rows, seen, D, Dv, meta.num_splits)
+    tiles, splits = tree_plan(B, Hk, rows, seen, D, Dv, meta.num_splits, fp8)
     if not 1 <= splits <= MAX_SPLITS:
         raise ValueError(f"1 .. {MAX_SPLITS} splits, not {splits}")
     ws = None
