@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
   const int rt = gridDim.x / p.splits;
   const int sp = blockIdx.x / rt, tile = blockIdx.x - sp * rt;
   const int q0 = __ldg(p.q_start + b), q1 = __ldg(p.q_start + b + 1);
-  const bool inside = q0 >= 0 && q1 <= p.T;            // rows outside the call's tensors: no tree here, and told
+  const bool inside = q0 >= 0 && q0 <= q1 && q1 <= p.T;   // rows outside the call's tensors: no tree here, and told
   const int n = inside ? q1 - q0 : 0;
   const int L = __ldg(p.kv_len + b), ctx = L - n;
   const int r0 = tile * (128 * ROWT);

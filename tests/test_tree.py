@@ -361,6 +361,30 @@ def test_attention_large_scores_keep_the_maximum():
         check_attention(s, run_attention(s))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention_raises_the_maximum_at_every_tile(shape, monkeypatch):
+    """Scores that climb by about 0.06 a key: 2^11 over 128 keys, so every tile rescales what the tiles before left.
+    They reach 75, a 32-bit error of 75 * 2^-21 in the worst case: below the 2^-12 of the bound."""
+    Hq, Hk, D, Dv, fp8 = shape
+    s = make_attention(Hq, Hk, D, Dv, [20, 3], [1200, 500], fp8=fp8, seed=15, device="cuda")
+    m, q, kf = s["meta"], s["q"], s["k"].float()
+    q[:, :, 0] = 128.0
+    for b in range(2):
+        for t in range(int(m.kv_len[b])):
+            kf[int(m.block_table[b, t // PAGE]), :, t % PAGE, 0] = 0.06 * t * D ** 0.5 / 128 / s["ks"]
+    s["k"] = kf.to(s["k"].dtype)
+    assert torch.isfinite(s["k"].float()).all()
+    o, a = attention_oracle(s)
+    plan = tree.tree_plan
+    for splits in (1, 2):
+        m.num_splits = splits
+        for tiles in (1, 2) if Dv <= 128 else (1,):
+            monkeypatch.setattr(tree, "tree_plan", lambda *x: (tiles, plan(*x)[1]))
+            check_attention(s, run_attention(s), o, a)
+    N.check_status()
+
+
 # ---------------------------------------------------------------- verification
 def verify_oracle(probs, tokens, parents, q_start, P, ua, ud, draft=None, target=None):
     par, tok, qs = parents.tolist(), tokens.tolist(), q_start.tolist()
@@ -895,7 +919,8 @@ def test_refusals_gpu():
     def told():
         with pytest.raises(RuntimeError, match="bounds"):
             N.check_status()
-    for change in (dict(q_start=i32([0, 5, 9], "cuda")), dict(max_nodes=4), dict(block_table=m.block_table[:, :1])):
+    for change in (dict(q_start=i32([0, 5, 9], "cuda")), dict(q_start=i32([0, 5, 3], "cuda")), dict(max_nodes=4),
+                   dict(block_table=m.block_table[:, :1])):
         tree.tree_attention(q, k, v, dataclasses.replace(m, **change))
         told()
     par, tok = random_trees([5, 3], 2, "cuda")[0], torch.ones(8, dtype=torch.int32, device="cuda")
