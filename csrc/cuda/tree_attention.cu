@@ -234,7 +234,7 @@ __device__ __forceinline__ uint32_t bad_bf16x2(uint32_t w) {
 // Masked pages: a tile that hides a key from some row of the CTA (the tree's own, the last, those a
 // window cuts) is masked bit by bit in S, and V's non-finite values are zeroed in shared memory
 // first, since 0 * NaN would reach every row; the rows that do see such a key get it at the end.
-template <int D_, int DVT_, int BN_, int ROWT_, int SK, int SV, int NR_ = 0>
+template <int D_, int DVT_, int BN_, int ROWT_, int SK, int SV_, int NR_ = 0>
 struct TtCfg {
   static constexpr int D = D_, DVT = DVT_, BN = BN_, ROWT = ROWT_;
   static constexpr int NR = NR_;                       // slots of the raw ring (fp8 caches)
@@ -242,6 +242,7 @@ struct TtCfg {
   // ROWT = 1: one accumulator, with one running maximum that goes from tile to tile (unit to unit), which
   // leaves tensor memory for a third S
   static constexpr bool SHARE = ROWT == 1;
+  static constexpr int SV = SV_;
   static constexpr int NO = SHARE ? 1 : 2;             // accumulators
   static constexpr int NSB = SHARE ? 3 : 2;            // S buffers: tile t in t % 3, or one a unit
   static constexpr int LEAD = SHARE ? 3 : 1;           // K tiles loaded before the first V: K(t + LEAD) follows V(t)
@@ -287,6 +288,8 @@ struct TtCfg {
   // ROWT = 1: a unit at tile t takes the release of V(t - 1)'s slot for the end of its product.  The slot's release
   // before that has to be over by then: it is tile t - 3's or older, whose product stands before S(t)
   static_assert(!SHARE || SV >= 2, "the release of a V slot would be ambiguous");
+  // ROWT = 2: what was in V(t)'s slot before is K(t - 1), V(t - 2) or older, whose fill is over when a unit comes to tile t
+  static_assert(SHARE || (ONE ? NS >= 3 : SV >= 2), "the fill of a V slot would be ambiguous");
   static_assert(D % 64 == 0 && DVT % 64 == 0 && BN % 64 == 0 && NS >= 3 && (!F8 || (D == DVT && BN == 128 && NR >= 2)), "tiles");
 };
 
@@ -689,12 +692,13 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
       const int buf = ROWT == 2 ? u : t % C::NSB, phase = (ROWT == 2 ? t : t / C::NSB) & 1;
       const uint32_t s_t = tmem + lanes + buf * BN;
       const bool msk = at >= shut || at < open;
-      if (msk) {
-        // V's non-finite values become zero (0 * p must stay 0 for keys that a row does not
-        // see) and join the rows that do see them at the end
+      // V's non-finite values become zero (0 * p must stay 0 for keys that a row does not see) and join the rows
+      // that do see them at the end.  The wait for V(t) is by parity, so the fill of its slot before that has to
+      // be known to be over, and V(t) cannot leave before P(t)
+      auto clean = [&] {
         ok = ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, p.status, 156);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) return;
         uint4* vw = reinterpret_cast<uint4*>(sK + C::slot_at(C::v_slot(t)));
 #pragma unroll 2
         for (int w = r; w < C::V_BYTES / 16; w += 128) {
@@ -707,11 +711,26 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
           }
         }
         fence_proxy_async_smem();
+      };
+      if (!C::SHARE && msk) {   // the unit has seen S(t - 1), which the issuer put after it had K(t - 1) and V(t - 2)
+        clean();
+        if (!ok) break;
       }
       ok = ta_wait(&s_full[buf], phase, p.status, 157);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
+      if (C::SHARE && msk) {
+        // S(t) stands, so the product of tile t - 3 is over and V(t - SV)'s release (SV >= 2) is the slot's next one
+        // or over; behind it the fill of V(t) is the slot's next one or over
+        if (t >= C::SV) {
+          ok = ta_wait(&empty[C::v_slot(t)], C::v_turn(t - C::SV) & 1, p.status, 166);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        clean();
+        if (!ok) break;
+      }
       // HW columns of S in registers at a time: all of them, or with 16 warps' share of the registers (fp8) a half
       constexpr int HW = C::HALVES ? BN / 2 : BN;
       uint32_t sv[HW];

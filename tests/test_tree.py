@@ -293,6 +293,74 @@ def test_attention_ignores_what_a_row_does_not_see(shape, splits):
     N.check_status()
 
 
+def poison_unused(s, bad):
+    """(k, v) in 32 bits with `bad` in every slot that holds no key of a sequence."""
+    m, fp8 = s["meta"], s["v"].dtype == FP8
+    free = torch.ones(s["k"].shape[0], PAGE, dtype=torch.bool)
+    for b in range(m.num_seqs):
+        t = torch.arange(int(m.kv_len[b]))
+        free[m.block_table[b].cpu().long()[t // PAGE], t % PAGE] = False
+    pg, off = (x.to(s["k"].device) for x in torch.nonzero(free, as_tuple=True))
+    val = torch.tensor(bad, device=s["k"].device)[off % len(bad)][:, None, None]
+    kf, vf = s["k"].float(), s["v"].float()
+    kf[pg, :, off] = val
+    if fp8:
+        vf[pg, :, :, off] = val
+    else:
+        vf[pg, :, off] = val
+    return kf, vf
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,bn,last", [  # BN keys a tile; masked tiles 0 .. last: twice round the V slots and further
+    ((4, 2, 64, 64, False), 128, 13), ((24, 2, 128, 128, False), 128, 7), ((16, 2, 192, 128, False), 64, 9),
+    ((16, 2, 256, 256, False), 64, 5), ((4, 2, 64, 64, True), 128, 7), ((24, 2, 128, 128, True), 128, 5)])
+@pytest.mark.parametrize("splits", [1, 2, 3])
+@pytest.mark.parametrize("tiles", [1, 2])
+def test_attention_of_masked_tiles_at_every_place_of_the_ring(shape, bn, last, splits, tiles, monkeypatch):
+    """The first masked tile is the call's tile 0, 1, .. `last` (within a split: every place up to there), the slots
+    behind the last node and a node's V hold NaN and infinities, and shared memory holds NaN from the kernel before:
+    a row's value is that of the clean cache bit for bit unless it sees the node."""
+    Hq, Hk, D, Dv, fp8 = shape
+    if tiles == 2 and Dv > 128:
+        pytest.skip("heads of 256 take one row tile a CTA")
+    ctx = [t * bn + 5 for t in range(last + 1)] + [t * bn + bn - 4 for t in range(last + 1)]
+    n = 12
+    s = make_attention(Hq, Hk, D, Dv, [n] * len(ctx), ctx, fp8=fp8, seed=16, device="cuda")
+    m = s["meta"]
+    o, a = attention_oracle(s)
+    bad = [float("nan")] if fp8 else [float("nan"), float("inf"), float("-inf")]
+    k, v, t = s["k"], s["v"], s["k"].dtype
+    kf, vf = poison_unused(s, bad)
+    vn = vf.clone()                                 # beside that, column 1 of node 4's V
+    for b, c in enumerate(ctx):
+        pg, off = int(m.block_table[b, (c + 4) // PAGE]), (c + 4) % PAGE
+        vn[pg][(slice(None), 1, off) if fp8 else (slice(None), off, 1)] = bad[-1]
+    sees = (m.mask[:, 0] >> 4 & 1).bool()
+    keep = [c for c in range(Dv) if c != 1]
+    dirt = torch.full((2048, 2048), float("nan"), dtype=torch.bfloat16, device="cuda")
+    plan = tree.tree_plan
+    m.num_splits = splits
+    monkeypatch.setattr(tree, "tree_plan", lambda *x: (tiles, plan(*x)[1]))
+    s["k"], s["v"] = k, v
+    clean = run_attention(s)
+    check_attention(s, clean, o, a)
+    for _ in range(3):
+        s["k"], s["v"] = k, v
+        torch.mm(dirt, dirt)
+        assert torch.equal(run_attention(s), clean)
+        s["k"], s["v"] = kf.to(t), vf.to(t)
+        torch.mm(dirt, dirt)
+        assert torch.equal(run_attention(s), clean)
+        s["v"] = vn.to(t)
+        torch.mm(dirt, dirt)
+        out = run_attention(s)
+        assert torch.equal(out[~sees], clean[~sees])
+        assert not torch.isfinite(out[sees][:, :, 1].float()).any()
+        assert torch.equal(out[sees][:, :, keep], clean[sees][:, :, keep])
+    N.check_status()
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_attention_of_a_node_with_an_infinite_value(device):
     """A node's V that some rows see and others do not."""
