@@ -398,7 +398,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     for (int i = 0; i < C::NR; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], 4); }
     mbar_init(q_ready, 4 * C::UNITS);
     for (int i = 0; i < 2; ++i) mbar_init(&o_done[i], 1);
-    for (int i = 0; i < C::NSB; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[2 * i], 4); mbar_init(&p_full[2 * i + 1], 4); }
+    for (int i = 0; i < C::NSB; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], ROWT == 2 && i == (two ? 1 : 0) ? 5 : 4);   // (and warp 2's)
+    }
     fence_barrier_init();
   }
   if (C::SHARE && threadIdx.x >= 128 && threadIdx.x < 256) m_row[threadIdx.x - 128] = make_int2(0, -1);
@@ -589,16 +593,16 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     // ------------------------------------------------------------ slots back to the producer (ROWT = 2)
     // S of a tile stands for the unit that is served last (s_full): K of that tile is done with, and V of the
     // tile before, whose PV the issuer put before that S.  (Softmax threads' arrivals cost their warp 350
-    // cycles a tile.)
+    // cycles a tile.)  This warp's arrival with that unit's P lets S(t + 1) follow only once S(t) was seen here:
+    // the wait is by parity, and two tiles further on it would be for a phase that never comes.  It is there
+    // long before P.
     if (ROWT == 2 && elect_one()) {
-      bool ok = true;
-      for (int t = 0; t < nt && ok; ++t) {
-        const bool k = C::k_again(t, nt), v = t > 0 && C::v_again(t - 1, nt);
-        if (!k && !v) continue;
-        ok = ta_wait(&s_full[two ? 1 : 0], t & 1, p.status, 159);
-        if (!ok) break;
-        if (k) mbar_arrive(&empty[C::k_slot(t)]);
-        if (v) mbar_arrive(&empty[C::v_slot(t - 1)]);
+      const int last = two ? 1 : 0;
+      for (int t = 0; t < nt; ++t) {
+        if (!ta_wait(&s_full[last], t & 1, p.status, 159)) break;
+        mbar_arrive(&p_full[2 * last + 1]);
+        if (C::k_again(t, nt)) mbar_arrive(&empty[C::k_slot(t)]);
+        if (t > 0 && C::v_again(t - 1, nt)) mbar_arrive(&empty[C::v_slot(t - 1)]);
       }
     }
   } else if (C::F8 && warp >= 12) {
