@@ -1050,7 +1050,7 @@ extern "C" {
 
 // q [T, Hq, D] (strides q_ts, q_hs), caches [num_blocks, Hkv, 64, D | DV] bf16, or fp8 K
 // [num_blocks, Hkv, 64, D] and V [num_blocks, Hkv, DV, 64]; o [T, Hq, DV] bf16.  ws: splits *
-// T * Hq * (DV + 2) floats when splits > 1 (<= 64).  row_tiles: 128-row tiles of a CTA (1 or 2; heads of 256
+// T * Hq * (DV + 2) floats when splits > 1 (<= 64).  q, o, ws and the caches start on 16-byte boundaries.  row_tiles: 128-row tiles of a CTA (1 or 2; heads of 256
 // always 1).  Returns the launches, < 0 on error.
 struct XtuTreeAttention {
   const void* q;
@@ -1082,6 +1082,9 @@ int xtu_tree_attention(const XtuTreeAttention* a) {
   if (Hkv <= 0 || Hq % Hkv != 0 || B > 65535 || Hkv > 65535 || a->W <= 0) return -2;
   if (row_tiles < 1 || row_tiles > 2 || splits < 1 || splits > 64 || (splits > 1 && a->ws == nullptr)) return -3;
   if (a->window > 0 && a->depth == nullptr) return -4;
+  // 16-byte accesses (the caches: ta_map)
+  if (((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->o) | reinterpret_cast<uintptr_t>(a->ws)) & 15) != 0)
+    return -5;
   TaParams p{};
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.q_ts = a->q_ts;

@@ -1009,3 +1009,25 @@ def test_refusals_gpu():
     tree.tree_mask(par, qs, 4)
     with pytest.raises(RuntimeError, match="bounds"):
         N.check_status()
+
+
+def test_the_attention_entry_refuses_unaligned_tensors():
+    """q, out and the workspace are read and written 16 bytes at a time; the entry says so before it starts anything."""
+    base = dict(q=256, o=256, ws=256)
+    for name in base:
+        a = {**base, name: 264}
+        with pytest.raises(RuntimeError, match="code -5"):
+            N.call_packed("xtu_tree_attention", a["q"], 512, 64, 256, 256, 0, a["o"], 0, 0, 0, 1, 1, 0, 1, 0, 0, 1, 1, 1, 4, 2,
+                          64, 64, 1, 1.0, 1.0, 1.0, 0, 1, 2, a["ws"], 0, 0)
+
+
+@pytest.mark.gpu
+def test_attention_refuses_an_unaligned_out():
+    s = make_attention(4, 2, 64, 64, [5, 3], [10, 70], seed=52, device="cuda")
+    for splits in (1, 2):
+        s["meta"].num_splits = splits
+        out = torch.zeros(8 * 4 * 64 + 8, dtype=torch.bfloat16, device="cuda")
+        for odd in (1, 4):
+            with pytest.raises(ValueError, match="16-byte"):
+                run_attention(s, out=out[odd:odd + 8 * 4 * 64].view(8, 4, 64))
+        check_attention(s, run_attention(s, out=out[8:].view(8, 4, 64)))

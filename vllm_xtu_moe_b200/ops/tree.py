@@ -238,6 +238,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     Caches as in :func:`attention.paged_attention`: bf16 ``[blocks, Hkv, 64, D]`` / ``[.., Dv]`` with
     (D, Dv) in ``HEAD_DIMS``, or fp8 (e4m3) K and per-block transposed V with ``FP8_HEAD_DIMS`` (their
     products take q as fp16: magnitudes up to 65504).  MLA latent caches are not served.
+    ``out``: bf16 [T, Hq, Dv], contiguous, on a 16-byte boundary.
     ``workspace``: fp32, ``splits * T * Hq * (Dv + 2)`` elements when the KV range is split; allocated
     when None or too small.  One that is passed in belongs to the call until its work is done: calls
     that may overlap take one each."""
@@ -302,6 +303,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     q_ts, q_hs, q1 = q.stride()
     if q1 != 1 or (q_ts | q_hs) & 7 or qp & 15:
         raise ValueError("q rows must be contiguous and start on 16-byte boundaries")
+    op = out.data_ptr()
+    if op & 15:
+        raise ValueError("out must start on a 16-byte boundary")
     rows = most * (Hq // Hk)
     seen = min(meta.max_kv_len, window + most + KV_BLOCK) if window > 0 else meta.max_kv_len
     tiles, splits = tree_plan(B, Hk, rows, seen, D, Dv, meta.num_splits, fp8)
@@ -316,7 +320,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             raise ValueError(f"workspace must be contiguous fp32 on {_name(dev)}, on a 16-byte boundary")
         if ws is None or ws.numel() < need:
             ws = q.new_empty(need, dtype=_F32)
-    N.call_packed("xtu_tree_attention", qp, q_ts, q_hs, kp, vp, fp8, out.data_ptr(), q_start.data_ptr(),
+    N.call_packed("xtu_tree_attention", qp, q_ts, q_hs, kp, vp, fp8, op, q_start.data_ptr(),
                   kv_len.data_ptr(), bt.data_ptr(), bt_stride, bt_cols, mask.data_ptr(), W, _ptr(meta.depth), window, B,
                   most, T, Hq, Hk, D, Dv, nb, scale, k_scale, v_scale, _ptr(sinks), tiles, splits, _ptr(ws),
                   _status(dev), _stream(dev))
