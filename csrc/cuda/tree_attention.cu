@@ -234,7 +234,7 @@ __device__ __forceinline__ uint32_t bad_bf16x2(uint32_t w) {
 // Masked pages: a tile that hides a key from some row of the CTA (the tree's own, the last, those a
 // window cuts) is masked bit by bit in S, and V's non-finite values are zeroed in shared memory
 // first, since 0 * NaN would reach every row; the rows that do see such a key get it at the end.
-template <int D_, int DVT_, int BN_, int ROWT_, int SK, int SV_, int NR_ = 0>
+template <int D_, int DVT_, int BN_, int ROWT_, int SK_, int SV_, int NR_ = 0>
 struct TtCfg {
   static constexpr int D = D_, DVT = DVT_, BN = BN_, ROWT = ROWT_;
   static constexpr int NR = NR_;                       // slots of the raw ring (fp8 caches)
@@ -242,7 +242,7 @@ struct TtCfg {
   // ROWT = 1: one accumulator, with one running maximum that goes from tile to tile (unit to unit), which
   // leaves tensor memory for a third S
   static constexpr bool SHARE = ROWT == 1;
-  static constexpr int SV = SV_;
+  static constexpr int SK = SK_, SV = SV_;
   static constexpr int NO = SHARE ? 1 : 2;             // accumulators
   static constexpr int NSB = SHARE ? 3 : 2;            // S buffers: tile t in t % 3, or one a unit
   static constexpr int LEAD = SHARE ? 3 : 1;           // K tiles loaded before the first V: K(t + LEAD) follows V(t)
@@ -252,8 +252,6 @@ struct TtCfg {
   // ROWT = 2: one ring of SK + SV slots where a K and a V tile are the same size (K0 V0 K1 V1 ..; the count
   // may be odd); else a ring each
   static constexpr bool ONE = !SHARE && K_BYTES == V_BYTES;
-  // slots that hold K, V
-  [[maybe_unused]] static constexpr int KS = ONE ? SK + SV : SK, VS = ONE ? SK + SV : SV;
   static constexpr int NS = SK + SV, RING = SK * K_BYTES + SV * V_BYTES;
   __device__ static int k_slot(int t) { return ONE ? 2 * t % NS : t % SK; }
   __device__ static int v_slot(int t) { return ONE ? (2 * t + 1) % NS : SK + t % SV; }
@@ -480,13 +478,16 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
           }
         }
       }
-      if (!ok) {   // let the copies in flight land (bounded) before the CTA ends
-        if constexpr (C::F8) {
-          for (int i = max(0, in - C::NR); i < in; ++i) ta_wait(&r_full[i % C::NR], (i / C::NR) & 1, nullptr, 0, 50000000ull);
-        } else {
-          for (int t = max(0, kn - C::KS); t < kn; ++t) ta_wait(&full[C::k_slot(t)], C::k_turn(t) & 1, nullptr, 0, 50000000ull);
-          for (int t = max(0, vn - C::VS); t < vn; ++t) ta_wait(&full[C::v_slot(t)], C::v_turn(t) & 1, nullptr, 0, 50000000ull);
-        }
+      // the copies in flight land (bounded) before the CTA ends, also when another warp gave up: the last fill of
+      // every slot
+      auto landed = [&](uint64_t* bar, int turn) { ta_wait(bar, turn & 1, nullptr, 0, 50000000ull); };
+      if constexpr (C::F8) {
+        for (int i = max(0, in - C::NR); i < in; ++i) landed(&r_full[i % C::NR], i / C::NR);
+      } else if constexpr (C::ONE) {
+        for (int i = max(0, in - C::NS); i < in; ++i) landed(&full[i % C::NS], i / C::NS);
+      } else {
+        for (int t = max(0, kn - C::SK); t < kn; ++t) landed(&full[C::k_slot(t)], C::k_turn(t));
+        for (int t = max(0, vn - C::SV); t < vn; ++t) landed(&full[C::v_slot(t)], C::v_turn(t));
       }
     }
   } else if (warp == 1) {
@@ -581,13 +582,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
           }
         }
       }
-      if (!ok) {   // the MMAs in flight end before the CTA gives its tensor memory back
-        uint64_t* drained = o_done + 2;
+      // the MMAs in flight end (bounded) before the CTA gives its tensor memory back, also when a unit gave up
+      uint64_t* drained = ok ? o_done + (two ? 1 : 0) : o_done + 2;
+      if (!ok) {
         mbar_init(drained, 1);
         fence_barrier_init();
         mma_commit(drained);
-        ta_wait(drained, 0, nullptr, 0, 50000000ull);
       }
+      ta_wait(drained, 0, nullptr, 0, 50000000ull);
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ slots back to the producer (ROWT = 2)
