@@ -3,7 +3,7 @@
 // Each rank owns int flags[world].  Arriving at barrier e stores e into slot [me] of
 // every peer's array (release, system scope); the barrier is passed once every slot
 // of the rank's own array is >= e (acquire, system scope).  Waits are bounded by
-// %globaltimer and by the library's status word: a timeout records
+// %globaltimer and by an error in the library's status word (status_failed): a timeout records
 // XTU_ERR_PEER_TIMEOUT with the missing peer's rank and returns false.
 #pragma once
 #include "../cuda/ptx.cuh"
@@ -39,7 +39,7 @@ __device__ __forceinline__ bool peer_barrier(int* const* peer_flags, int rank, i
           ok = false;
           break;
         }
-        if (st && *reinterpret_cast<volatile uint32_t*>(&st->code) != 0u) { ok = false; break; }
+        if (status_failed(st)) { ok = false; break; }
       }
     }
   }

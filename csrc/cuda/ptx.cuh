@@ -21,7 +21,7 @@ enum : uint32_t {
   XTU_ERR_MBAR_TIMEOUT = 1,    // an intra-CTA mbarrier wait ran out of time
   XTU_ERR_PEER_TIMEOUT = 2,    // a wait on another GPU's flag ran out of time
   XTU_ERR_HOST_TIMEOUT = 3,    // a wait on a host-written flag ran out of time
-  XTU_ERR_BOUNDS = 4,          // a bounds check in a debug build tripped
+  XTU_ERR_BOUNDS = 4,          // an index or size outside what the call covers: that access or row is left out
   XTU_ERR_PROTOCOL = 5,        // a host-bridge request posted into a busy slot, or read back unposted
 };
 
@@ -34,7 +34,10 @@ struct XtuStatus {
 
 __device__ __forceinline__ void report_error(XtuStatus* st, uint32_t code, uint32_t where, uint32_t extra) {
   if (st == nullptr) return;
-  if (atomicCAS(&st->code, 0u, code) == 0u) {
+  // the first error stays, but a wait that ran out takes the place of a bounds report: other waits look for it
+  const uint32_t was = atomicCAS(&st->code, 0u, code);
+  if (was == 0u || (was == XTU_ERR_BOUNDS && code != XTU_ERR_BOUNDS &&
+                    atomicCAS(&st->code, (uint32_t)XTU_ERR_BOUNDS, code) == XTU_ERR_BOUNDS)) {
     st->where = where;
     st->block = blockIdx.x;
     st->extra = extra;
@@ -110,9 +113,12 @@ constexpr uint64_t kIntraCtaWaitNs = 500000000ull;  // 0.5 s
 
 // Bounded parity wait.  Returns false (and records the failure) on timeout.
 // Once any CTA has recorded an error in `st`, every other bounded wait gives up at
-// its next check, so a fault costs one timeout in total rather than one per CTA.
+// its next check, so a fault costs one timeout in total rather than one per CTA.  (A bounds report is no such
+// error: what it is about was left out, and the rest of the call, and later calls, go on.)
 __device__ __forceinline__ bool status_failed(const XtuStatus* st) {
-  return st != nullptr && *reinterpret_cast<const volatile uint32_t*>(&st->code) != 0u;
+  if (st == nullptr) return false;
+  const uint32_t code = *reinterpret_cast<const volatile uint32_t*>(&st->code);
+  return code != XTU_OK && code != XTU_ERR_BOUNDS;
 }
 
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, XtuStatus* st, uint32_t where,

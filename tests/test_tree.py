@@ -1011,6 +1011,31 @@ def test_refusals_gpu():
         N.check_status()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("shape", SHAPES[:6])
+def test_attention_goes_on_beside_what_it_leaves_out(shape, splits):
+    """A sequence outside the call's tensors is reported and left out.  The other sequences of the call, and calls after
+    it whose caller has not asked for the status yet, keep their results although their waits are long."""
+    import dataclasses
+    Hq, Hk, D, Dv, fp8 = shape
+    s = make_attention(Hq, Hk, D, Dv, [12, 3, 9, 12], [6000, 2500, 70, 4000], fp8=fp8, seed=53, device="cuda")
+    m = s["meta"]
+    m.num_splits = splits
+    clean = run_attention(s)
+    N.check_status()
+    row = lambda t: torch.cat([t, t[:1]])                                     # noqa: E731
+    wrong = dataclasses.replace(m, num_seqs=5, q_start=torch.cat([m.q_start, i32([48], "cuda")]), kv_len=row(m.kv_len),
+                                block_table=row(m.block_table).contiguous())
+    for _ in range(10):
+        assert torch.equal(run_attention({**s, "meta": wrong}), clean)
+        assert torch.equal(run_attention(s), clean)                           # the report still stands
+    with pytest.raises(RuntimeError, match="bounds"):
+        N.check_status()
+    assert torch.equal(run_attention(s), clean)
+    N.check_status()
+
+
 def test_the_attention_entry_refuses_unaligned_tensors():
     """q, out and the workspace are read and written 16 bytes at a time; the entry says so before it starts anything."""
     base = dict(q=256, o=256, ws=256)
