@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
   const int n = inside ? q1 - q0 : 0;
   const int L = __ldg(p.kv_len + b), ctx = L - n;
   const int r0 = tile * (128 * ROWT);
-  const int rows_all = n * p.G;
+  const int rows_all = min(n, p.max_nodes) * p.G;
   if (r0 >= rows_all) {                                // uniform: no such row tile here
     if (!inside && threadIdx.x == 0) report_error(p.status, XTU_ERR_BOUNDS, 247, q1);
     griddep_launch_dependents();
@@ -915,12 +915,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
 }
 
 // ---------------------------------------------------------------------------------------
-// the splits' normalised partials by their log-sum-exp: one warp per (token, head)
+// the splits' normalised partials by their log-sum-exp: one warp per (token, head).  Rows that the attention kernel
+// left out (of no sequence, of one outside the tensors, nodes past max_nodes) have no partials and stay as they are:
+// the lanes look through the sequences for the row's own, beside the loads of its values
 // ---------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) tree_attn_merge_kernel(const float* __restrict__ ws_o,
                                                               const float* __restrict__ ws_lse, int splits,
                                                               int rows, int Hq, int DV, const int* __restrict__ q_start,
-                                                              int B, const float* __restrict__ sinks,
+                                                              int B, int max_nodes, const float* __restrict__ sinks,
                                                               __nv_bfloat16* __restrict__ o) {
   griddep_wait();
   griddep_launch_dependents();
@@ -940,7 +942,13 @@ __global__ void __launch_bounds__(256) tree_attn_merge_kernel(const float* __res
   // lane s holds split s (at most 64 splits: two per lane)
   const float a = lane < splits ? __ldg(ws_lse + (size_t)lane * rows + w) : -FLT_MAX;
   const float c = lane + 32 < splits ? __ldg(ws_lse + (size_t)(lane + 32) * rows + w) : -FLT_MAX;
-  if (w >= q_start[B] * Hq || w < q_start[0] * Hq) return;   // rows behind the last sequence stay as they are
+  const int tok = w / Hq, T = rows / Hq;
+  bool owned = false;
+  for (int b = lane; b < B; b += 32) {
+    const int q0 = __ldg(q_start + b), q1 = __ldg(q_start + b + 1);
+    owned |= q0 >= 0 && q0 <= tok && tok < q1 && q1 <= T && tok - q0 < max_nodes;
+  }
+  if (!__any_sync(0xffffffffu, owned)) return;
   float M = fmaxf(a, c);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
@@ -1151,7 +1159,7 @@ int xtu_tree_attention(const XtuTreeAttention* a) {
   const int heads = T * Hq;
   const cudaError_t e = launch_pdl(tree_attn_merge_kernel, dim3((heads + 7) / 8), dim3(256), 0, s,
                                    (const float*)p.ws_o, (const float*)p.ws_lse, splits, heads, Hq, DV, p.q_start, B,
-                                   p.sinks, p.o);
+                                   p.max_nodes, p.sinks, p.o);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? r + 1 : -(int)e;
 }

@@ -1036,6 +1036,34 @@ def test_attention_goes_on_beside_what_it_leaves_out(shape, splits):
     N.check_status()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("lens,starts,most,good", [
+    ([5, 3], [0, 5, 3], 5, range(5)), ([5, 3], [0, 5, 9], 5, range(5)), ([5, 3], [-1, 5, 8], 5, range(5, 8)),
+    ([5, 3], [0, 5, 8], 4, [0, 1, 2, 3, 5, 6, 7]), ([5, 3], [0, 5, 8], 2, [0, 1, 5, 6]), ([3] * 40, None, 2, None)])
+def test_attention_leaves_out_only_what_it_reports(lens, starts, most, good, splits):
+    """Bounds that fall or lie outside q, and more nodes than max_nodes: the other rows are those of a clean call, the
+    rows left out keep what `out` held."""
+    import dataclasses
+    if starts is None:                                        # more sequences than lanes, each cut
+        starts, good = list(range(0, 121, 3)), [3 * b + i for b in range(40) for i in range(2)]
+    for Hq, Hk, D, Dv, fp8 in SHAPES[:6]:
+        s = make_attention(Hq, Hk, D, Dv, lens, [700 + 3 * b for b in range(len(lens))], fp8=fp8, seed=54, device="cuda")
+        m = s["meta"]
+        m.num_splits = splits
+        clean = run_attention(s)
+        N.check_status()
+        out = torch.full_like(clean, 7.0)
+        ws = torch.full((splits * clean.numel() // Dv * (Dv + 2),), float("nan"), device="cuda")
+        wrong = dataclasses.replace(m, q_start=i32(starts, "cuda"), max_nodes=most)
+        run_attention({**s, "meta": wrong}, out=out, workspace=ws)
+        with pytest.raises(RuntimeError, match="bounds"):
+            N.check_status()
+        kept = torch.zeros(len(clean), dtype=torch.bool)
+        kept[list(good)] = True
+        assert torch.equal(out[kept], clean[kept]) and bool((out[~kept] == 7.0).all())
+
+
 def test_the_attention_entry_refuses_unaligned_tensors():
     """q, out and the workspace are read and written 16 bytes at a time; the entry says so before it starts anything."""
     base = dict(q=256, o=256, ws=256)

@@ -233,7 +233,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     ``sinks`` fp32 [Hq]: learned logits in the denominator.  A row that sees nothing (or only
     scores of minus infinity) is zero.
     Keys outside a row's view never reach it, whatever the cache holds there; rows behind the
-    last sequence are left as they are.
+    last sequence are left as they are.  On the GPU ``_native.check_status`` reports a sequence whose
+    rows lie outside q and nodes past ``meta.max_nodes``, whose rows stay as they are too, and keys past
+    the block table, which no row sees.
 
     Caches as in :func:`attention.paged_attention`: bf16 ``[blocks, Hkv, 64, D]`` / ``[.., Dv]`` with
     (D, Dv) in ``HEAD_DIMS``, or fp8 (e4m3) K and per-block transposed V with ``FP8_HEAD_DIMS`` (their
