@@ -774,6 +774,59 @@ def test_commit_moves_nothing_outside_the_tree(device, fp8):
     assert torch.equal(kd.cpu().double(), k1) and torch.equal(vd.cpu().double(), v1)
 
 
+def commit_by_slots(k, v, path, acc, qs, kl, bt):
+    """commit_oracle for tables with columns and ids that name no page: a move needs both of its slots."""
+    fp8 = k.dtype == FP8
+    k1, v1 = (x.view(torch.uint8).clone() if fp8 else x.clone() for x in (k, v))
+    k0, v0 = k1.clone(), v1.clone()
+    for b in range(len(acc)):
+        n = int(qs[b + 1] - qs[b])
+        ctx = int(kl[b]) - n
+        slot = {i: (int(bt[b, (ctx + i) // PAGE]), (ctx + i) % PAGE) for i in range(n)
+                if ctx >= 0 and (ctx + i) // PAGE < bt.shape[1] and 0 <= int(bt[b, (ctx + i) // PAGE]) < k.shape[1]}
+        for j in range(1, int(acc[b]) + 1):
+            f, t = slot.get(int(path[b, j])), slot.get(j)
+            if f is None or t is None:
+                continue
+            k1[:, t[0], :, t[1]] = k0[:, f[0], :, f[1]]
+            if fp8:
+                v1[:, t[0], :, :, t[1]] = v0[:, f[0], :, :, f[1]]
+            else:
+                v1[:, t[0], :, t[1]] = v0[:, f[0], :, f[1]]
+    return k1, v1
+
+
+BAD_PAGES = ["none", "first", "second", "beyond", "columns", "short"]
+
+
+def commit_with_bad_pages(device, fp8, bad):
+    """Trees over two and three pages, of which one is not there."""
+    k, v, path, acc, qs, kl, bt = commit_inputs(2, 2, 64, 64, [60, 130, 9], [30, 40, 62], fp8, 34)
+    for b, n in enumerate([60, 130, 9]):                     # every second node is accepted: all of them move
+        path[b] = -1
+        path[b, :(n + 1) // 2] = torch.arange(0, n, 2, dtype=torch.int32)
+        acc[b] = (n + 1) // 2 - 1
+    if bad in ("first", "second", "beyond"):
+        bt[:, {"first": 0, "second": 1, "beyond": 2}[bad]] = i32([-1, k.shape[1], 10 ** 6])
+    elif bad == "columns":
+        bt = bt[:, :1].contiguous()
+    elif bad == "short":                                     # padding: fewer keys than nodes
+        kl = i32([0, 129, 3])
+    k1, v1 = commit_by_slots(k, v, path, acc, qs, kl, bt)
+    assert bad in ("columns", "short") or not torch.equal(k1, k.view(torch.uint8) if fp8 else k)
+    kd, vd = k.to(device), v.to(device)
+    tree.commit_tree(kd, vd, *[x.to(device) for x in (path, acc, qs, kl, bt)])
+    if fp8:
+        kd, vd = kd.view(torch.uint8), vd.view(torch.uint8)
+    assert torch.equal(kd.cpu(), k1) and torch.equal(vd.cpu(), v1)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("bad", BAD_PAGES)
+def test_commit_cpu_moves_nothing_from_or_to_pages_that_are_not_there(fp8, bad):
+    commit_with_bad_pages("cpu", fp8, bad)
+
+
 # ---------------------------------------------------------------- together
 def two_layer_model(Hq, Hk, D, V, seed, device):
     g = torch.Generator().manual_seed(seed)

@@ -503,16 +503,25 @@ def verify_tree(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
 # cache commit
 # ---------------------------------------------------------------------------
 def commit_tree_ref(k_caches, v_caches, path, accepted, q_start, kv_len, block_table) -> None:
-    qs, kl, acc, pth = q_start.tolist(), kv_len.tolist(), accepted.tolist(), path.tolist()
-    fp8 = k_caches[0].dtype == _FP8
+    qs, kl, acc, pth, bt = q_start.tolist(), kv_len.tolist(), accepted.tolist(), path.tolist(), block_table.tolist()
+    fp8, nb = k_caches[0].dtype == _FP8, k_caches[0].shape[0]
+
+    def page(b, slot):      # -1: the cache has none
+        col = slot // KV_BLOCK
+        return bt[b][col] if col < len(bt[b]) and 0 <= bt[b][col] < nb else -1
+
     for b in range(len(kl)):
         n = qs[b + 1] - qs[b]
         ctx = kl[b] - n
+        if ctx < 0:
+            continue
         for j in range(1, min(acc[b], path.shape[1] - 1, n - 1) + 1):
             if not j < pth[b][j] < n:
                 continue
             f, t = ctx + pth[b][j], ctx + j
-            fb, tb = int(block_table[b, f // KV_BLOCK]), int(block_table[b, t // KV_BLOCK])
+            fb, tb = page(b, f), page(b, t)
+            if fb < 0 or tb < 0:
+                continue
             for k, v in zip(k_caches, v_caches):
                 if fp8:
                     k, v = k.view(torch.uint8), v.view(torch.uint8)
@@ -531,7 +540,9 @@ def commit_tree(k_caches, v_caches, path: torch.Tensor, accepted: torch.Tensor, 
     k_caches / v_caches: one cache per layer, of one shape (layers of other head counts take a
     call of their own), as sequences of tensors or as one tensor with the layers in front; bf16
     or fp8 (V transposed inside each block).  A path must rise (a parent lies below its
-    children); entries that do not, or that lie outside the tree or the cache, move nothing."""
+    children): entry j names a node above j, or j itself, which is in place.  Entries that name
+    none such, and moves from or to a slot outside the table or the cache, move nothing; nor does a
+    sequence of fewer keys than nodes (padding)."""
     stacked = isinstance(k_caches, torch.Tensor) and isinstance(v_caches, torch.Tensor)
     if stacked:
         if k_caches.dim() != 5 or v_caches.dim() != 5:
