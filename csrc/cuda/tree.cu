@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(
 // column), a thread permutes its column in shared memory, and the pieces that a destination
 // lies in go back: byte moves in global memory fetched the same sectors one dependent
 // byte at a time (61 us for 46 layers x 16 sequences of 61 nodes).  A tree that reaches over a
-// third page moves bytes.
+// third page, or whose first page is not there, moves bytes.
 constexpr int TC_LAYERS = 64;   // layers of one launch (their pointers travel as parameters)
 constexpr int TC_MOVES = 256;   // moves of one turn
 constexpr int TC_LD = 132;      // a column's two pages in shared memory (33 words: no bank conflicts)
@@ -649,7 +649,11 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
     }
     const int c0 = (part - 1) * 256, nc = min(256, Hkv * Dv - c0);
     const size_t page_b = (size_t)Hkv * Dv * 64;
-    if ((reach >> 6) > pg0 + 1) {
+    if (reach == 0) continue;
+    int pages[2];
+    for (int g = 0; g < 2; ++g) pages[g] = pg0 + g < bt_cols ? bt[(size_t)b * bt_stride + pg0 + g] : -1;
+    // a tree over a third page, or without the first (moves inside the second are left then)
+    if ((reach >> 6) > pg0 + 1 || pages[0] < 0 || pages[0] >= num_blocks) {
       for (int i = 0; tid < nc && i < cnt; ++i) {
         const int f1 = src[i], t1 = dst[i];
         if (f1 < 0) continue;
@@ -658,9 +662,6 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
       }
       continue;
     }
-    int pages[2];
-    for (int g = 0; g < 2; ++g) pages[g] = pg0 + g < bt_cols ? bt[(size_t)b * bt_stride + pg0 + g] : -1;
-    if (reach == 0 || pages[0] < 0 || pages[0] >= num_blocks) continue;   // (without the first page no source lies in one)
     const bool second = (reach >> 6) > pg0;                               // (its id was checked with the move)
     const int pieces = second ? 8 : 4;
     for (int i = tid; i < nc * pieces; i += 256) {

@@ -827,6 +827,14 @@ def test_commit_cpu_moves_nothing_from_or_to_pages_that_are_not_there(fp8, bad):
     commit_with_bad_pages("cpu", fp8, bad)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("bad", BAD_PAGES)
+def test_commit_moves_k_and_v_alike_beside_pages_that_are_not_there(fp8, bad):
+    """fp8: V lies transposed and takes another way than K; without the first page it was left where it lay."""
+    commit_with_bad_pages("cuda", fp8, bad)
+
+
 # ---------------------------------------------------------------- together
 def two_layer_model(Hq, Hk, D, V, seed, device):
     g = torch.Generator().manual_seed(seed)
