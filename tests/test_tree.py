@@ -1125,6 +1125,34 @@ def test_attention_leaves_out_only_what_it_reports(lens, starts, most, good, spl
         assert torch.equal(out[kept], clean[kept]) and bool((out[~kept] == 7.0).all())
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("window,sinks", [(0, False), (3, True)])
+def test_attention_of_a_padded_batch(device, splits, window, sinks):
+    """Padding sequences: no nodes, or nodes without keys, whose rows are zero; with fewer keys than nodes the keys are
+    the last nodes'.  The other sequences keep their rows."""
+    s = make_attention(4, 2, 64, 64, [9, 4, 0, 5, 6], [70, 0, 0, 130, 0], seed=55, device=device, window=window, sinks=sinks)
+    m = s["meta"]
+    m.num_splits = splits
+    clean = run_attention(s)
+    m.kv_len[1] = 0
+    out = run_attention(s)
+    assert bool((out[9:13] == 0).all()) and torch.equal(out[:9], clean[:9]) and torch.equal(out[13:], clean[13:])
+    # the last two of sequence 4's six nodes, as a tree whose first four nodes nobody sees
+    m.kv_len[4] = 2
+    out = run_attention(s)
+    k, v, pg = s["k"].clone(), s["v"].clone(), int(m.block_table[4, 0])
+    k[pg, :, 4:6], v[pg, :, 4:6] = s["k"][pg, :, :2], s["v"][pg, :, :2]
+    m.mask[18:, 0] &= ~0xF
+    m.kv_len[4] = 6
+    same = run_attention({**s, "k": k, "v": v})
+    # check_attention's bound for each of the two, with sum p |v| <= max |v|
+    assert (out[18:].float() - same[18:].float()).abs().max() <= (2 ** -6 + 2 ** -11) * v[pg, :, 4:6].float().abs().max()
+    assert torch.equal(out[:18], same[:18])
+    if device == "cuda":
+        N.check_status()
+
+
 def test_the_attention_entry_refuses_unaligned_tensors():
     """q, out and the workspace are read and written 16 bytes at a time; the entry says so before it starts anything."""
     base = dict(q=256, o=256, ws=256)

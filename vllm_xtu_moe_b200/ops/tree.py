@@ -162,18 +162,22 @@ def tree_attention_ref(q, k_cache, v_cache, meta: TreeMetadata, scale: float, ou
         r0, n = qs[b], qs[b + 1] - qs[b]
         if n == 0:
             continue
+        if kl[b] <= 0:
+            out[r0:r0 + n] = 0
+            continue
         ctx = kl[b] - n
         k = _gather_kv(k_cache, meta.block_table[b], kl[b]).float().repeat_interleave(G, dim=1)
         v = _gather_kv(v_cache, meta.block_table[b], kl[b]).float().repeat_interleave(G, dim=1)
         node = torch.arange(n, device=q.device)
         tree = (meta.mask[r0:r0 + n].long()[:, node >> 5] >> (node & 31) & 1).bool()            # [i, j]
         see = torch.ones(n, kl[b], dtype=torch.bool, device=q.device)
+        first = max(0, -ctx)          # (fewer keys than nodes, padding: the last nodes' keys are there)
         if window > 0:
             deep = meta.depth[r0:r0 + n].long().clamp(0, n - 1)
             far = deep[:, None] - window
-            see[:, :ctx] = torch.arange(ctx, device=q.device)[None] > ctx + far
+            see[:, :max(0, ctx)] = torch.arange(max(0, ctx), device=q.device)[None] > ctx + far
             tree &= deep[None] > far
-        see[:, ctx:] = tree
+        see[:, max(0, ctx):] = tree[:, first:]
         s = torch.einsum("qhd,khd->hqk", q[r0:r0 + n].float(), k) * scale
         s = s.masked_fill(~see[None], float("-inf"))
         m = s.amax(-1, keepdim=True)
@@ -235,7 +239,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     Keys outside a row's view never reach it, whatever the cache holds there; rows behind the
     last sequence are left as they are.  On the GPU ``_native.check_status`` reports a sequence whose
     rows lie outside q and nodes past ``meta.max_nodes``, whose rows stay as they are too, and keys past
-    the block table, which no row sees.
+    the block table, which no row sees.  Rows of a sequence with a ``kv_len`` of 0 (padding) are zero.
 
     Caches as in :func:`attention.paged_attention`: bf16 ``[blocks, Hkv, 64, D]`` / ``[.., Dv]`` with
     (D, Dv) in ``HEAD_DIMS``, or fp8 (e4m3) K and per-block transposed V with ``FP8_HEAD_DIMS`` (their
