@@ -484,3 +484,23 @@ def test_sigmoid_gate_kernels():
     shared_gate_(y, x, w)
     torch.cuda.synchronize()
     assert (y.float() - ref).abs().max().item() < 2e-2
+
+
+def test_stream_handle_of_every_way_to_name_a_device(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 1000 + i, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    for device, index in ((None, 3), ("cuda", 3), (torch.device("cuda"), 3), (0, 0), (2, 2), ("cuda:1", 1),
+                          (torch.device("cuda", 1), 1)):
+        assert N.stream_ptr(device) == 1000 + index, device
+    for device in ("cpu", torch.device("cpu")):
+        with pytest.raises(ValueError):
+            N.stream_ptr(device)
+
+
+@pytest.mark.gpu
+def test_stream_handle_is_the_current_stream():
+    side = torch.cuda.Stream()
+    for device in (None, 0, "cuda", "cuda:0", torch.device("cuda", 0)):
+        assert N.stream_ptr(device) == torch.cuda.current_stream(device).cuda_stream
+        with torch.cuda.stream(side):
+            assert N.stream_ptr(device) == side.cuda_stream

@@ -204,10 +204,18 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def stream_ptr(device: torch.device | None = None) -> int:
+def stream_ptr(device: torch.device | int | str | None = None) -> int:
     """The current stream of ``device`` (default: the current one) as a handle.  The raw call: the
     ``torch.cuda.Stream`` object that ``current_stream`` builds costs 2.4 us a launch."""
-    index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
+    index = None
+    if device is not None:
+        if not isinstance(device, torch.device):
+            device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"expected a CUDA device, not {device}")
+        index = device.index
+    if index is None:
+        index = torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)
 
 
