@@ -296,15 +296,21 @@ __device__ __forceinline__ void tt_copy16(uint32_t dst, const void* src, bool th
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-// a row's running maximum with the tile that it is of, in one 8-byte access of shared memory
-__device__ __forceinline__ void ta_row_max_to(int2* at, float m, int tile) {
-  asm volatile("st.volatile.shared.v2.b32 [%0], {%1, %2};" ::"r"(smem_u32(at)), "r"(__float_as_int(m)), "r"(tile) : "memory");
+// a row's running maximum with the tile that it is of, as one 64-bit word of shared memory (the parts of a vector
+// access need not be seen together)
+__device__ __forceinline__ void ta_row_max_to(uint64_t* at, float m, int tile) {
+  asm volatile("{\n\t.reg .b64 x;\n\tmov.b64 x, {%1, %2};\n\tst.volatile.shared.b64 [%0], x;\n\t}" ::"r"(smem_u32(at)),
+               "r"(__float_as_int(m)), "r"(tile)
+               : "memory");
 }
-__device__ __forceinline__ float ta_row_max(const int2* at, int tile, bool& ok) {   // waits for that tile, bounded
+__device__ __forceinline__ float ta_row_max(const uint64_t* at, int tile, bool& ok) {   // waits for that tile, bounded
   int m, of, it = 0;
 #pragma unroll 1
   do {
-    asm volatile("ld.volatile.shared.v2.b32 {%0, %1}, [%2];" : "=r"(m), "=r"(of) : "r"(smem_u32(at)) : "memory");
+    asm volatile("{\n\t.reg .b64 x;\n\tld.volatile.shared.b64 x, [%2];\n\tmov.b64 {%0, %1}, x;\n\t}"
+                 : "=r"(m), "=r"(of)
+                 : "r"(smem_u32(at))
+                 : "memory");
   } while (of != tile && ++it < (1 << 24));
   ok = of == tile;
   return __int_as_float(m);
@@ -356,7 +362,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
   int& s_bad = *reinterpret_cast<int*>(tmem_slot + 1);   // a masked tile held a non-finite value
   // SHARE: [128] the rows' running maximum, and the tile that it is of: the unit of the next tile waits for it.  (A
   // barrier and a load behind it took 500 cycles more a tile.)
-  int2* m_row = reinterpret_cast<int2*>(tmem_slot + 2);
+  uint64_t* m_row = reinterpret_cast<uint64_t*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, kh = blockIdx.y;
@@ -403,7 +409,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) tree_attn_tc_kernel(const __gri
     }
     fence_barrier_init();
   }
-  if (C::SHARE && threadIdx.x >= 128 && threadIdx.x < 256) m_row[threadIdx.x - 128] = make_int2(0, -1);
+  if (C::SHARE && threadIdx.x >= 128 && threadIdx.x < 256) ta_row_max_to(&m_row[threadIdx.x - 128], 0.f, -1);
   if (warp == 1) tmem_alloc(tmem_slot, C::COLS);
   tc_fence_before();
   __syncthreads();
