@@ -1153,6 +1153,14 @@ def test_attention_of_a_padded_batch(device, splits, window, sinks):
         N.check_status()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_window_wider_than_any_context(device):
+    s = make_attention(4, 2, 64, 64, [9, 4], [70, 300], seed=56, device=device)
+    clean = run_attention(s)
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        assert torch.equal(run_attention({**s, "window": window}), clean)
+
+
 def test_the_attention_entry_refuses_unaligned_tensors():
     """q, out and the workspace are read and written 16 bytes at a time; the entry says so before it starts anything."""
     base = dict(q=256, o=256, ws=256)

@@ -326,8 +326,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             raise ValueError(f"workspace must be contiguous fp32 on {_name(dev)}, on a 16-byte boundary")
         if ws is None or ws.numel() < need:
             ws = q.new_empty(need, dtype=_F32)
-    N.call_packed("xtu_tree_attention", qp, q_ts, q_hs, kp, vp, fp8, op, q_start.data_ptr(),
-                  kv_len.data_ptr(), bt.data_ptr(), bt_stride, bt_cols, mask.data_ptr(), W, _ptr(meta.depth), window, B,
+    N.call_packed("xtu_tree_attention", qp, q_ts, q_hs, kp, vp, fp8, op, q_start.data_ptr(), kv_len.data_ptr(),
+                  bt.data_ptr(), bt_stride, bt_cols, mask.data_ptr(), W, _ptr(meta.depth), min(window, 2 ** 31 - 1), B,
                   most, T, Hq, Hk, D, Dv, nb, scale, k_scale, v_scale, _ptr(sinks), tiles, splits, _ptr(ws),
                   _status(dev), _stream(dev))
     return out
