@@ -167,8 +167,8 @@ __global__ void __launch_bounds__(32) tree_verify_greedy_kernel(
 // its nodes, their probabilities) 5500, the first steps 3500; then per pass the load of the slice (the
 // first at its node) 3000 to 6000, its weights 1100 with no rejection, 3000 with one and 1100 for each
 // further one (64-bit arithmetic), sums and cluster barrier 2000, the walk 1700; the search for the drawn token 4000.
-// One sequence, V = 151552: 16 us cold.  32 trees of 26 nodes: 31 us for the 30 MB that they read (5 us
-// at the copy rate), in two waves: 18 clusters of 8 fit.
+// One sequence, V = 151552: 16 us cold.  32 trees of 26 nodes: 31 to 39 us (by card and inputs) for the 30 MB
+// that they read (5 us at the copy rate), in two waves: 18 clusters of 8 fit.
 struct TvCmd {
   int op;        // 0 sum the weights, 1 draw, 2 done
   int row;       // row of probs

@@ -221,14 +221,15 @@ __device__ __forceinline__ uint32_t bad_bf16x2(uint32_t w) {
 // much as an N = 128 one), ex2 partly as a cubic on the FMA pipe (no change), the maximum
 // taken between the exponentials (246: registers; with registers moved from the other warps no change).
 // ROWT = 1 takes that chain off the way of S (two units on alternate tiles with an accumulator each: 1.2 us a
-// tile against 0.85; 16 / 2 heads of 256 62.8 -> 57 us).  In long runs the card's power limit binds:
+// tile against 0.85; 16 / 2 heads of 256 62.8 -> 57 us).  V of a masked tile is cleaned after the wait for S: before it,
+// V's arrival cannot be told by the parity of its barrier.  In long runs the card's power limit binds:
 // 1.65 of 1.97 GHz.
 // 4 sequences x 14.6K keys, 96 / 8 heads of 128 (KV 240 MB, 36 us at the copy rate), a call among others:
-//   60 rows a KV head   49 us (0.75 of the copy rate);  192 rows 67;  480 rows 110
-//   732 rows            172 to 190 us (153 GFLOP: 0.51 of the GEMM rate, MMA pipe 52 % busy, XU 53 %)
-//   192 rows over the fp8 cache  79 us: the same chain, and the second read of S that 128 registers
+//   60 rows a KV head   50 us (0.73 of the copy rate);  192 rows 67 to 82;  480 rows 112
+//   732 rows            172 to 204 us (153 GFLOP: 0.45 to 0.53 of the GEMM rate, MMA pipe 52 % busy, XU 52 %)
+//   192 rows over the fp8 cache  79 to 88 us: the same chain, and the second read of S that 128 registers
 //                       force (one read with registers moved: no change); its bytes are 18 us
-// 16 sequences of up to 12K keys, 16 / 2 heads of 256: 57 us (197 MB: 30 us; N = 64 products).  A CTA's start
+// 16 sequences of up to 12K keys, 16 / 2 heads of 256: 55 to 61 us (197 MB: 30 us; N = 64 products).  A CTA's start
 // and end cost about 6 us, and 9 to 16 us is a call over a few pages.  Split counts: ops/tree.py.
 //
 // Masked pages: a tile that hides a key from some row of the CTA (the tree's own, the last, those a

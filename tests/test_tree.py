@@ -311,19 +311,19 @@ def poison_unused(s, bad):
     return kf, vf
 
 
-@pytest.mark.gpu
-@pytest.mark.parametrize("shape,bn,last", [  # BN keys a tile; masked tiles 0 .. last: twice round the V slots and further
+RINGS = [  # shape, keys a tile, last masked tile: twice round the V slots of one row tile and further
     ((4, 2, 64, 64, False), 128, 13), ((24, 2, 128, 128, False), 128, 7), ((16, 2, 192, 128, False), 64, 9),
-    ((16, 2, 256, 256, False), 64, 5), ((4, 2, 64, 64, True), 128, 7), ((24, 2, 128, 128, True), 128, 5)])
+    ((16, 2, 256, 256, False), 64, 5), ((4, 2, 64, 64, True), 128, 7), ((24, 2, 128, 128, True), 128, 5)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,bn,last,tiles", [(*r, t) for r in RINGS for t in (1, 2) if t == 1 or r[0][3] <= 128])
 @pytest.mark.parametrize("splits", [1, 2, 3])
-@pytest.mark.parametrize("tiles", [1, 2])
-def test_attention_of_masked_tiles_at_every_place_of_the_ring(shape, bn, last, splits, tiles, monkeypatch):
+def test_attention_of_masked_tiles_at_every_place_of_the_ring(shape, bn, last, tiles, splits, monkeypatch):
     """The first masked tile is the call's tile 0, 1, .. `last` (within a split: every place up to there), the slots
     behind the last node and a node's V hold NaN and infinities, and shared memory holds NaN from the kernel before:
     a row's value is that of the clean cache bit for bit unless it sees the node."""
     Hq, Hk, D, Dv, fp8 = shape
-    if tiles == 2 and Dv > 128:
-        pytest.skip("heads of 256 take one row tile a CTA")
     ctx = [t * bn + 5 for t in range(last + 1)] + [t * bn + bn - 4 for t in range(last + 1)]
     n = 12
     s = make_attention(Hq, Hk, D, Dv, [n] * len(ctx), ctx, fp8=fp8, seed=16, device="cuda")

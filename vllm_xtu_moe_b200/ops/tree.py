@@ -219,9 +219,9 @@ def tree_plan(num_seqs: int, num_kv_heads: int, rows: int, seen: int, d: int = 1
     One CTA per SM takes one or two 128-row tiles of a (sequence, KV head, split).  In microseconds a
     key tile costs about 1.8 for two row tiles and 0.85 for one (1.55 from fp8, 1.2 of 256-wide heads),
     a CTA's start and end 9 and the merge of the splits 7, so the time is about
-    waves * (key tiles per split * that + 9) + 7.  Measured (4 x 14.6K keys, 8 KV heads), one / two row
-    tiles at their best splits: 192 rows 67 / 72 us, 480 rows 110 / 128, 732 rows 193 / 172; fp8: 192
-    rows 107 / 79, 60 rows 56 / 61."""
+    waves * (key tiles per split * that + 9) + 7.  Measured (4 x 14.6K keys, 8 KV heads, cold caches),
+    one / two row tiles at their best splits: 192 rows 74 / 82 us, 480 rows 115 / 137, 732 rows 184 /
+    182; fp8: 192 rows 117 / 90, 60 rows 66 / 70."""
     one_us = 1.55 if fp8 else 0.85 if dv <= 128 else 1.2
     return _plan(num_seqs * num_kv_heads, rows, -(-seen // (128 if d <= 128 else 64)), dv > 128, one_us, splits, num_sms)
 
@@ -240,6 +240,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     last sequence are left as they are.  On the GPU ``_native.check_status`` reports a sequence whose
     rows lie outside q and nodes past ``meta.max_nodes``, whose rows stay as they are too, and keys past
     the block table, which no row sees.  Rows of a sequence with a ``kv_len`` of 0 (padding) are zero.
+
+    Scores, softmax statistics and sums are held in 32 bits; the weights of the second product are rounded to the
+    type of its operands, bf16 (half a step: 2^-8 of each) over bf16 caches, fp16 (2^-11) over fp8 ones.
 
     Caches as in :func:`attention.paged_attention`: bf16 ``[blocks, Hkv, 64, D]`` / ``[.., Dv]`` with
     (D, Dv) in ``HEAD_DIMS``, or fp8 (e4m3) K and per-block transposed V with ``FP8_HEAD_DIMS`` (their
